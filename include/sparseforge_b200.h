@@ -62,6 +62,12 @@ typedef enum {
     SF_HARD_THRESHOLD = 1 /* mask > 0.5 ('unstructured', :526-527); N:M then only shapes beta mixing and the top-N pull */
 } sf_hard_view;
 
+/* Norms of sf_grad_norm. */
+typedef enum {
+    SF_NORM_L2 = 0,  /* sqrt of the sum of squares */
+    SF_NORM_INF = 1  /* largest magnitude */
+} sf_norm_kind;
+
 SF_API int sf_version(void);
 SF_API const char* sf_last_error_string(void);
 
@@ -497,6 +503,33 @@ SF_API int sf_kl_div_fwd(const void* student, const void* teacher, int dtype, in
 SF_API int sf_kl_div_bwd(const void* student, const void* teacher, int dtype, const float* lse,
                   const float* row_scale, int64_t rows, int64_t vocab, double temperature, double max_logit,
                   void* grad, void* stream);
+
+/*
+ * Global norm of many gradient tensors, and clipping by it.
+ *   replaces: torch.nn.utils.clip_grad_norm_ between backward and optimizer.step of the training loop,
+ *             legacy/main_llama.py:1997-2211.
+ *   norm = sqrt(sum of g^2 over every element of every tensor), or the largest |g| (SF_NORM_INF)
+ *   c    = min(1, max_norm / (norm + 1e-6)),  outs[i] = grads[i] * c, rounded once to the output's type
+ * grads, outs, sizes (elements), dtypes (SF_F32 / SF_BF16) are HOST arrays of `count` entries, read during the
+ * call; the tensors are on the device, dense, of any size and element alignment (16-byte aligned ones move in
+ * 16-byte accesses). norm is one fp32 on the device; scratch has sf_grad_norm_scratch_doubles(count) doubles,
+ * holds nothing between calls, and must not be shared by calls that may run at the same time.
+ * The sum keeps the whole fp32 range (squares that leave it are formed in fp64) and adds in a fixed order. No tensor
+ * at all gives norm 0. An infinite or NaN gradient makes the norm so; clipping by a NaN norm makes every output NaN, by
+ * an infinite one 0 (NaN where the gradient is infinite), as the reference's does.
+ * An output is its own input (clipping in place; with c = 1 it is left alone) or overlaps no other tensor of
+ * the call; a call that breaks this, for example by naming a gradient twice, is refused.
+ * sf_clip_grads takes the norm from the device (for example combined over ranks first); sf_clip_grad_norm forms it
+ * and clips in one call, with the coefficient taken from the unrounded norm.
+ */
+SF_API int64_t sf_grad_norm_scratch_doubles(int64_t count);
+SF_API int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,
+                 float* norm, double* scratch, void* stream);
+SF_API int sf_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dtypes,
+                  const int32_t* out_dtypes, int64_t count, const float* norm, double max_norm, void* stream);
+SF_API int sf_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dtypes,
+                      const int32_t* out_dtypes, int64_t count, int kind, double max_norm, float* norm, double* scratch,
+                      void* stream);
 
 /*
  * Row-sharded layer: the two products whose result has to cross GPUs, with the exchange done by

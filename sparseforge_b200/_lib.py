@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_PKG, "lib", "libsparseforge_b200.so")
 
 SF_F32, SF_BF16, SF_I8 = 0, 1, 2
 METRICS = {"hessian_obd": 0, "hessian_ratio": 1, "magnitude": 2, "hessian": 3, "movement": 4}
+NORM_L2, NORM_INF = 0, 1
 PENALTY_NONE, PENALTY_TOPN, PENALTY_MID = 0, 1, 2
 MSTAT_FLIPS, MSTAT_SUM_M, MSTAT_SUM_M1M, MSTAT_SUM_TOP2, MSTAT_SUM_BOT2, MSTAT_COUNT_LT_HALF = range(6)
 MSTAT_COUNT = 8
@@ -65,6 +66,10 @@ _SIGNATURES = {
     "sf_bias_grad": (c_int, [_P, c_int, _P, c_int64, c_int64, _P]),
     "sf_kl_div_fwd": (c_int, [_P, _P, c_int, c_int64, c_int64, c_double, c_double, _P, _P, _P]),
     "sf_kl_div_bwd": (c_int, [_P, _P, c_int, _P, _P, c_int64, c_int64, c_double, c_double, _P, _P]),
+    "sf_grad_norm_scratch_doubles": (c_int64, [c_int64]),
+    "sf_grad_norm": (c_int, [_P, _P, _P, c_int64, c_int, _P, _P, _P]),
+    "sf_clip_grads": (c_int, [_P, _P, _P, _P, _P, c_int64, _P, c_double, _P]),
+    "sf_clip_grad_norm": (c_int, [_P, _P, _P, _P, _P, c_int64, c_int, c_double, _P, _P, _P]),
     "sf_masked_gemm_fwd_allgather": (c_int, [_P, _P, _P, _P, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_float,
                                              c_int, _P, _P]),
     "sf_mask_update_nm24_frozen": (c_int, [_P, _P, _P, _P, c_double, c_double, c_int, _P, _P, c_int, _P, _P, _P, c_int64,

@@ -1,0 +1,403 @@
+// Global norm of many gradient tensors, and clipping by it.
+//
+//   norm = sqrt(sum over every element of every tensor of g^2)      (or max |g|)
+//   c    = min(1, max_norm / (norm + 1e-6)),   out = g * c           (one rounding, to out's type)
+//
+// The tensors of one call are described by a table that travels in the kernel's parameters: no copy of
+// pointers to the device, so a call is one launch for the norm and one for the scaling, and can be captured.
+// A tensor is cut into chunks of equal length; the chunks of all tensors are numbered through and dealt out
+// round robin to a grid of one resident wave, so 4096-element vectors and 45-million-element matrices share a launch.
+//
+// Range and order of the sum of squares: eight squares are added in fp32 (a bf16 square is exact there), the sums of
+// eight in fp64. Where the fp32 sum of eight leaves [2^-100, 2^120] its elements are squared in fp64 instead, so
+// neither large nor tiny gradients (whose squares leave fp32) change the norm. Partial sums have one slot per block and
+// are added in one fixed order: the result does not depend on timing.
+#include <cstdlib>
+
+#include <algorithm>
+#include <new>
+
+#include "common.cuh"
+
+namespace sf {
+
+constexpr int kGnThreads = 512;
+constexpr int kGnSlots = 1024;       // partial results one launch may write (its largest grid)
+constexpr int kGnVec = 8;            // elements per access group: 16 bytes of bf16, 32 of fp32
+constexpr int kGnChunkUnit = kGnThreads * kGnVec;
+
+enum { GN_L2 = SF_NORM_L2, GN_INF = SF_NORM_INF };
+
+struct GnTensor {
+    const void* in;
+    void* out;
+    int64_t n;
+};
+// kind bits of a table entry
+enum { GN_IN_BF16 = 1, GN_OUT_BF16 = 2, GN_VEC = 4, GN_IN_PLACE = 8 };
+template <int CAP>
+struct GnTable {
+    GnTensor t[CAP];
+    uint32_t first[CAP + 1];  // number of the tensor's first chunk; first[count] = chunks of the launch
+    uint8_t kind[CAP];
+    int count;
+    int chunk;  // elements per chunk, a multiple of kGnChunkUnit
+};
+
+template <int CAP>
+__device__ __forceinline__ int find_tensor(const GnTable<CAP>& tab, uint32_t c) {
+    int lo = 0, hi = tab.count - 1;  // the last tensor whose first chunk is <= c
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (tab.first[mid] <= c) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+struct NormAcc {
+    double sum;
+    uint32_t top;  // bit pattern of the largest |g|: ordered like the values, a NaN above infinity
+};
+
+// MAXNORM: the largest magnitude instead of the sum of squares
+template <bool MAXNORM>
+__device__ __forceinline__ void acc8(NormAcc& a, const float (&x)[8]) {
+    if (MAXNORM) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) a.top = max(a.top, __float_as_uint(x[i]) & 0x7fffffffu);
+        return;
+    }
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        s0 = fmaf(x[i], x[i], s0);
+        s1 = fmaf(x[i + 1], x[i + 1], s1);
+    }
+    const float s = s0 + s1;
+    if (s >= 0x1p-100f && s <= 0x1p120f) {
+        a.sum += (double)s;
+    } else {
+        uint32_t any = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) any |= __float_as_uint(x[i]) << 1;
+        if (any != 0) {  // not eight zeros
+#pragma unroll
+            for (int i = 0; i < 8; ++i) a.sum = fma((double)x[i], (double)x[i], a.sum);
+        }
+    }
+}
+template <bool MAXNORM>
+__device__ __forceinline__ void acc1(NormAcc& a, float x) {
+    if (MAXNORM) a.top = max(a.top, __float_as_uint(x) & 0x7fffffffu);
+    else a.sum = fma((double)x, (double)x, a.sum);
+}
+
+__device__ __forceinline__ void unpack_bf16(const uint4& v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack_f32(const uint4& a, const uint4& b, float (&x)[8]) {
+    x[0] = __uint_as_float(a.x); x[1] = __uint_as_float(a.y); x[2] = __uint_as_float(a.z); x[3] = __uint_as_float(a.w);
+    x[4] = __uint_as_float(b.x); x[5] = __uint_as_float(b.y); x[6] = __uint_as_float(b.z); x[7] = __uint_as_float(b.w);
+}
+
+// All threads of a block: sum (or largest) over the block, in an order fixed by the thread numbers. The result
+// is valid in thread 0.
+__device__ __forceinline__ NormAcc block_merge(NormAcc a, NormAcc* part) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a.sum += __shfl_down_sync(0xffffffffu, a.sum, o);
+        a.top = max(a.top, __shfl_down_sync(0xffffffffu, a.top, o));
+    }
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < kGnThreads / 32; ++w) {
+            a.sum += part[w].sum;
+            a.top = max(a.top, part[w].top);
+        }
+    }
+    return a;
+}
+
+template <int CAP, bool MAXNORM>
+__global__ void __launch_bounds__(kGnThreads)
+grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __restrict__ slots) {
+    __shared__ NormAcc part[kGnThreads / 32];
+    NormAcc acc{0.0, 0u};
+    const uint32_t chunks = tab.first[tab.count];
+    for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        const int ti = find_tensor(tab, c);
+        const int64_t at = (int64_t)(c - tab.first[ti]) * tab.chunk;
+        const int len = (int)min((int64_t)tab.chunk, tab.t[ti].n - at);
+        const int kind = tab.kind[ti];
+        const int nv = (kind & GN_VEC) ? len / kGnVec : 0;
+        if (kind & GN_IN_BF16) {
+            const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(tab.t[ti].in) + at;
+            const uint4* q = reinterpret_cast<const uint4*>(p);
+            for (int v = threadIdx.x; v < nv; v += kGnThreads) {
+                float x[8];
+                unpack_bf16(__ldg(q + v), x);
+                acc8<MAXNORM>(acc, x);
+            }
+            for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) acc1<MAXNORM>(acc, __bfloat162float(p[i]));
+        } else {
+            const float* p = static_cast<const float*>(tab.t[ti].in) + at;
+            const uint4* q = reinterpret_cast<const uint4*>(p);
+            for (int v = threadIdx.x; v < nv; v += kGnThreads) {
+                float x[8];
+                unpack_f32(__ldg(q + 2 * v), __ldg(q + 2 * v + 1), x);
+                acc8<MAXNORM>(acc, x);
+            }
+            for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) acc1<MAXNORM>(acc, p[i]);
+        }
+    }
+    acc = block_merge(acc, part);
+    if (threadIdx.x == 0) slots[blockIdx.x] = MAXNORM ? (double)__uint_as_float(acc.top) : acc.sum;
+}
+
+// The norm from all slots, by every thread block that needs it: each computes the same value. Valid in every thread.
+__device__ __forceinline__ double norm_of_slots(const double* __restrict__ slots, int count, bool maxnorm, NormAcc* part,
+                                                double* shared_norm) {
+    NormAcc a{0.0, 0u};
+    for (int i = threadIdx.x; i < count; i += kGnThreads) {
+        if (maxnorm) a.top = max(a.top, __float_as_uint((float)slots[i]));
+        else a.sum += slots[i];
+    }
+    a = block_merge(a, part);
+    if (threadIdx.x == 0) *shared_norm = maxnorm ? (double)__uint_as_float(a.top) : sqrt(a.sum);
+    __syncthreads();
+    return *shared_norm;
+}
+
+__global__ void __launch_bounds__(kGnThreads)
+grad_norm_final_kernel(const double* __restrict__ slots, int count, int kind, float* __restrict__ norm) {
+    __shared__ NormAcc part[kGnThreads / 32];
+    __shared__ double value;
+    const double v = norm_of_slots(slots, count, kind == GN_INF, part, &value);
+    if (threadIdx.x == 0) *norm = (float)v;
+}
+
+// out = in * c. slots: the norm's partial results, which every block adds up for itself (norm_out gets the
+// value); or, with slots = NULL, the norm is read from norm_in.
+template <int CAP>
+__global__ void __launch_bounds__(kGnThreads)
+grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restrict__ slots, int slot_count, int kind,
+                 const float* norm_in, float* norm_out, double max_norm) {
+    __shared__ NormAcc part[kGnThreads / 32];
+    __shared__ double value;
+    double norm;
+    if (slots != nullptr) {
+        norm = norm_of_slots(slots, slot_count, kind == GN_INF, part, &value);
+        if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+    } else {
+        norm = (double)*norm_in;
+    }
+    const double ratio = max_norm / (norm + 1e-6);
+    const float c = ratio >= 1.0 ? 1.0f : (float)ratio;  // a NaN stays one
+    const uint32_t chunks = tab.first[tab.count];
+    for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
+        const uint32_t ch = chunks - 1 - k;  // backwards: what the norm read last is still in L2
+        const int ti = find_tensor(tab, ch);
+        const int ent = tab.kind[ti];
+        if ((ent & GN_IN_PLACE) && c == 1.0f) continue;
+        const int64_t at = (int64_t)(ch - tab.first[ti]) * tab.chunk;
+        const int len = (int)min((int64_t)tab.chunk, tab.t[ti].n - at);
+        const int nv = (ent & GN_VEC) ? len / kGnVec : 0;
+        const bool ib = ent & GN_IN_BF16, ob = ent & GN_OUT_BF16;
+        const char* ip = static_cast<const char*>(tab.t[ti].in) + at * (ib ? 2 : 4);
+        char* op = static_cast<char*>(tab.t[ti].out) + at * (ob ? 2 : 4);
+        for (int v = threadIdx.x; v < nv; v += kGnThreads) {
+            float x[8];
+            if (ib) unpack_bf16(reinterpret_cast<const uint4*>(ip)[v], x);
+            else unpack_f32(reinterpret_cast<const uint4*>(ip)[2 * v], reinterpret_cast<const uint4*>(ip)[2 * v + 1], x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= c;
+            if (ob) Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(op) + v * kGnVec, x);
+            else Vec8<float>::store(reinterpret_cast<float*>(op) + v * kGnVec, x);
+        }
+        for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) {
+            const float x = (ib ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(ip)[i])
+                                : reinterpret_cast<const float*>(ip)[i]) * c;
+            if (ob) reinterpret_cast<__nv_bfloat16*>(op)[i] = __float2bfloat16_rn(x);
+            else reinterpret_cast<float*>(op)[i] = x;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------------------
+constexpr int kGnCap = 448;  // tensors per launch: a table of 13 KiB, below the 32 KiB of kernel parameters
+
+static int64_t gn_launches(int64_t count) { return count <= 0 ? 1 : (count + kGnCap - 1) / kGnCap; }
+
+static int gn_check(const char* who, const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count) {
+    if (count < 0) return fail(SF_ERR_BAD_ARG, "%s: count must not be negative", who);
+    if (count > (1 << 20)) return fail(SF_ERR_UNSUPPORTED, "%s: more than 2^20 tensors", who);
+    if (count > 0 && (!grads || !sizes || !dtypes)) return fail(SF_ERR_BAD_ARG, "%s: grads, sizes and dtypes must be non-null", who);
+    for (int64_t i = 0; i < count; ++i) {
+        if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 42)) return fail(SF_ERR_BAD_ARG, "%s: size of tensor %lld out of range", who, (long long)i);
+        if (dtypes[i] != SF_F32 && dtypes[i] != SF_BF16)
+            return fail(SF_ERR_BAD_ARG, "%s: dtype of tensor %lld must be SF_F32 or SF_BF16", who, (long long)i);
+        if (sizes[i] > 0 && !grads[i]) return fail(SF_ERR_BAD_ARG, "%s: tensor %lld is null", who, (long long)i);
+        if (reinterpret_cast<uintptr_t>(grads[i]) % (dtypes[i] == SF_BF16 ? 2 : 4))
+            return fail(SF_ERR_ALIGNMENT, "%s: tensor %lld is not aligned to its elements", who, (long long)i);
+    }
+    return SF_OK;
+}
+
+// Every output is either its own input (same address, same type) or overlaps no other tensor of the call: blocks work
+// on the tensors in any order.
+struct GnSpan {
+    uintptr_t begin, end;
+    int writes;
+};
+static int gn_check_overlap(const char* who, const void* const* grads, void* const* outs, const int64_t* sizes,
+                            const int32_t* in_dt, const int32_t* out_dt, int64_t count) {
+    GnSpan* sp = new (std::nothrow) GnSpan[2 * count + 1];
+    if (!sp) return fail(SF_ERR_BAD_ARG, "%s: out of host memory", who);
+    int64_t k = 0;
+    for (int64_t i = 0; i < count; ++i) {
+        if (sizes[i] == 0) continue;
+        const uintptr_t o = reinterpret_cast<uintptr_t>(outs[i]), g = reinterpret_cast<uintptr_t>(grads[i]);
+        sp[k++] = GnSpan{o, o + (uintptr_t)sizes[i] * (out_dt[i] == SF_BF16 ? 2 : 4), 1};
+        if (!(o == g && in_dt[i] == out_dt[i])) sp[k++] = GnSpan{g, g + (uintptr_t)sizes[i] * (in_dt[i] == SF_BF16 ? 2 : 4), 0};
+    }
+    std::sort(sp, sp + k, [](const GnSpan& a, const GnSpan& b) { return a.begin < b.begin; });
+    uintptr_t any_end = 0, out_end = 0;
+    bool bad = false;
+    for (int64_t i = 0; i < k && !bad; ++i) {
+        bad = sp[i].begin < (sp[i].writes ? any_end : out_end);
+        any_end = std::max(any_end, sp[i].end);
+        if (sp[i].writes) out_end = std::max(out_end, sp[i].end);
+    }
+    delete[] sp;
+    if (bad) return fail(SF_ERR_BAD_ARG, "%s: an output overlaps another tensor of the call (the same gradient twice?)", who);
+    return SF_OK;
+}
+
+static int gn_grid(int64_t chunks) {
+    const int64_t cap = std::min<int64_t>(kGnSlots, (int64_t)sm_count() * 4);
+    return (int)std::max<int64_t>(1, std::min(chunks, cap));
+}
+
+// Fills the table with tensors [from, to). Returns the number of chunks.
+static int64_t gn_fill(GnTable<kGnCap>& tab, const void* const* grads, void* const* outs, const int64_t* sizes,
+                       const int32_t* in_dt, const int32_t* out_dt, int64_t from, int64_t to) {
+    int64_t total = 0;
+    for (int64_t i = from; i < to; ++i) total += sizes[i];
+    // the longest chunk that still gives every block of a resident wave some; small sets get short chunks, huge
+    // ones longer chunks so that their number stays a 32-bit one
+    int64_t chunk = kGnChunkUnit;
+    while (chunk < 4 * kGnChunkUnit && total / (2 * chunk) >= (int64_t)sm_count() * 8) chunk *= 2;
+    while (total / chunk > 0x3fffffff) chunk *= 2;
+    tab.chunk = (int)chunk;
+    tab.count = 0;
+    uint32_t c = 0;
+    for (int64_t i = from; i < to; ++i) {
+        if (sizes[i] == 0) continue;
+        const int k = tab.count++;
+        void* o = outs ? outs[i] : nullptr;
+        tab.t[k] = GnTensor{grads[i], o, sizes[i]};
+        const int odt = out_dt ? out_dt[i] : in_dt[i];
+        tab.kind[k] = (uint8_t)((in_dt[i] == SF_BF16 ? GN_IN_BF16 : 0) | (odt == SF_BF16 ? GN_OUT_BF16 : 0) |
+                                (aligned16(grads[i]) && aligned16(o) ? GN_VEC : 0) |
+                                (o == grads[i] && odt == in_dt[i] ? GN_IN_PLACE : 0));
+        tab.first[k] = c;
+        c += (uint32_t)((sizes[i] + chunk - 1) / chunk);
+    }
+    tab.first[tab.count] = c;
+    return c;
+}
+
+// Launches the partial sums of all tensors; *slot_count is the number of slots written.
+static int gn_partials(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,
+                       double* scratch, int* slot_count, cudaStream_t st) {
+    int slots = 0;
+    for (int64_t from = 0; from < count; from += kGnCap) {
+        GnTable<kGnCap> tab;
+        const int64_t chunks = gn_fill(tab, grads, nullptr, sizes, dtypes, nullptr, from, std::min(count, from + kGnCap));
+        if (chunks == 0) continue;
+        const int grid = gn_grid(chunks);
+        if (kind == GN_INF) grad_norm_partial_kernel<kGnCap, true><<<grid, kGnThreads, 0, st>>>(tab, scratch + slots);
+        else grad_norm_partial_kernel<kGnCap, false><<<grid, kGnThreads, 0, st>>>(tab, scratch + slots);
+        SF_CHECK_CUDA(cudaGetLastError());
+        slots += grid;
+    }
+    *slot_count = slots;
+    return SF_OK;
+}
+
+static int gn_scale(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dt,
+                    const int32_t* out_dt, int64_t count, const double* slots, int slot_count, int kind,
+                    const float* norm_in, float* norm_out, double max_norm, cudaStream_t st) {
+    // the tensors the norm read last come first
+    for (int64_t part = gn_launches(count) - 1; part >= 0; --part) {
+        GnTable<kGnCap> tab;
+        const int64_t from = part * kGnCap;
+        const int64_t chunks = gn_fill(tab, grads, outs, sizes, in_dt, out_dt, from, std::min(count, from + kGnCap));
+        grad_clip_kernel<kGnCap><<<gn_grid(chunks), kGnThreads, 0, st>>>(tab, slots, slot_count, kind, norm_in,
+                                                                        part == 0 ? norm_out : nullptr, max_norm);
+        SF_CHECK_CUDA(cudaGetLastError());
+    }
+    return SF_OK;
+}
+
+}  // namespace sf
+
+using namespace sf;
+
+extern "C" {
+
+int64_t sf_grad_norm_scratch_doubles(int64_t count) { return gn_launches(count) * kGnSlots; }
+
+int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,
+                 float* norm, double* scratch, void* stream) {
+    if (int rc = gn_check("sf_grad_norm", grads, sizes, dtypes, count)) return rc;
+    SF_CHECK_ARG(kind == GN_L2 || kind == GN_INF, "sf_grad_norm: kind must be SF_NORM_L2 or SF_NORM_INF");
+    SF_CHECK_ARG(norm && scratch, "sf_grad_norm: norm and scratch must be non-null");
+    cudaStream_t st = (cudaStream_t)stream;
+    int slots = 0;
+    if (int rc = gn_partials(grads, sizes, dtypes, count, kind, scratch, &slots, st)) return rc;
+    grad_norm_final_kernel<<<1, kGnThreads, 0, st>>>(scratch, slots, kind, norm);
+    SF_CHECK_CUDA(cudaGetLastError());
+    return SF_OK;
+}
+
+static int clip_impl(const char* who, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dt,
+                     const int32_t* out_dt, int64_t count, double max_norm) {
+    if (int rc = gn_check(who, grads, sizes, in_dt, count)) return rc;
+    if (count > 0 && (!outs || !out_dt)) return fail(SF_ERR_BAD_ARG, "%s: outs and their dtypes must be non-null", who);
+    if (int rc = gn_check(who, const_cast<const void* const*>(outs), sizes, out_dt, count)) return rc;
+    if (!(max_norm >= 0.0)) return fail(SF_ERR_BAD_ARG, "%s: max_norm must not be negative or NaN", who);
+    return gn_check_overlap(who, grads, outs, sizes, in_dt, out_dt, count);
+}
+
+int sf_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dtypes,
+                  const int32_t* out_dtypes, int64_t count, const float* norm, double max_norm, void* stream) {
+    if (int rc = clip_impl("sf_clip_grads", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm)) return rc;
+    SF_CHECK_ARG(norm != nullptr, "sf_clip_grads: norm must be non-null");
+    if (count == 0) return SF_OK;
+    return gn_scale(grads, outs, sizes, in_dtypes, out_dtypes, count, nullptr, 0, GN_L2, norm, nullptr, max_norm,
+                    (cudaStream_t)stream);
+}
+
+int sf_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dtypes,
+                      const int32_t* out_dtypes, int64_t count, int kind, double max_norm, float* norm, double* scratch,
+                      void* stream) {
+    if (int rc = clip_impl("sf_clip_grad_norm", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm)) return rc;
+    SF_CHECK_ARG(kind == GN_L2 || kind == GN_INF, "sf_clip_grad_norm: kind must be SF_NORM_L2 or SF_NORM_INF");
+    SF_CHECK_ARG(norm && scratch, "sf_clip_grad_norm: norm and scratch must be non-null");
+    cudaStream_t st = (cudaStream_t)stream;
+    int slots = 0;
+    if (int rc = gn_partials(grads, sizes, in_dtypes, count, kind, scratch, &slots, st)) return rc;
+    return gn_scale(grads, outs, sizes, in_dtypes, out_dtypes, count, scratch, slots, kind, nullptr, norm, max_norm, st);
+}
+
+}  // extern "C"

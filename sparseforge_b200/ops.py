@@ -5,6 +5,9 @@ torch is used here for device memory and streams only; the arithmetic is in the 
 """
 from __future__ import annotations
 
+import ctypes
+import math
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -411,6 +414,118 @@ def kl_div_bwd(student2d, teacher2d, lse, row_scale, temperature=2.0, max_logit=
     check(lib().sf_kl_div_bwd(_p(student2d), _p(teacher2d), _dt(student2d), _p(lse), _p(row_scale), rows, vocab,
                               float(temperature), float(max_logit), _p(grad), _stream()), "sf_kl_div_bwd")
     return grad
+
+
+# ----------------------------------------------------------------------------------------
+# global gradient norm and clipping
+# ----------------------------------------------------------------------------------------
+def _on_device_of(t: torch.Tensor):
+    """Context that makes ``t``'s device the current one (launches and ``_stream`` go there)."""
+    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else nullcontext()
+
+
+def _dense_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with its dimensions in memory order: contiguous whenever ``t`` fills its memory without gaps."""
+    order = sorted(range(t.dim()), key=lambda d: (t.stride(d), t.size(d)), reverse=True)
+    return t.permute(order)
+
+
+def _grad_arrays(ts, what):
+    """(addresses, element counts, dtype codes) of a list of gradients as C arrays, after checking them."""
+    n = len(ts)
+    try:
+        codes = [_DT[t.dtype] for t in ts]
+    except KeyError:
+        raise TypeError(f"{what}: gradients must be float32 or bfloat16, got {sorted({str(t.dtype) for t in ts})}") from None
+    if SF_I8 in codes:
+        raise TypeError(f"{what}: gradients must be float32 or bfloat16")
+    dev = ts[0].device
+    for t in ts:
+        if t.device != dev or not t.is_cuda:
+            _cuda(t)
+            raise ValueError(f"{what}: all gradients of a call must live on one device")
+        if t.layout != torch.strided:
+            raise RuntimeError(f"{what}: sparse gradients are not supported")
+        if not t.is_contiguous() and not _dense_view(t).is_contiguous():
+            raise RuntimeError("sparseforge_b200: tensors must be contiguous (or a dense permutation)")
+    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]), (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
+            (ctypes.c_int32 * n)(*codes))
+
+
+def _norm_kind(norm_type) -> int:
+    p = float(norm_type)
+    if p == 2.0:
+        return _lib.NORM_L2
+    if p == math.inf:
+        return _lib.NORM_INF
+    raise NotImplementedError(f"gradient norm of type {norm_type!r}: 2 and inf are built")
+
+
+def _clip_outputs(grads, out, what):
+    if out is None:
+        return grads
+    out = list(out)
+    if len(out) != len(grads):
+        raise ValueError(f"{what}: {len(grads)} gradients, {len(out)} outputs")
+    for g, o in zip(grads, out):
+        if o.shape != g.shape or not (o.stride() == g.stride() or (o.is_contiguous() and g.is_contiguous())):
+            raise ValueError(f"{what}: an output must have its gradient's shape and strides")
+    return out
+
+
+def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
+    """Norm over every element of all tensors in ``grads`` (fp32 / bf16, mixed) as one fp32 scalar on their device:
+    ``norm_type`` 2 (root of the sum of squares) or ``math.inf``. Nothing is read back."""
+    grads = list(grads)
+    kind = _norm_kind(norm_type)
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device="cuda")
+    ptrs, sizes, codes = _grad_arrays(grads, "grad_norm")
+    n = len(grads)
+    with _on_device_of(grads[0]):
+        norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=grads[0].device)
+        check(lib().sf_grad_norm(ptrs, sizes, codes, n, kind, _p(norm), _p(scratch), _stream()), "sf_grad_norm")
+    return norm
+
+
+def clip_grads(grads, norm, max_norm, out=None) -> None:
+    """``out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))`` with ``norm`` an fp32 scalar on the device (for
+    example ``grad_norm``'s, or one combined over ranks). In place without ``out``; an output may have the other
+    of the two dtypes (bf16 gradients from fp32 accumulators)."""
+    grads = list(grads)
+    if not grads:
+        return
+    out = _clip_outputs(grads, out, "clip_grads")
+    ptrs, sizes, codes = _grad_arrays(grads, "clip_grads")
+    optrs, _, ocodes = (ptrs, sizes, codes) if out is grads else _grad_arrays(out, "clip_grads")
+    _cuda(norm)
+    if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != grads[0].device or out[0].device != norm.device:
+        raise TypeError("clip_grads: norm must be one float32 on the gradients' device")
+    with _on_device_of(norm):
+        check(lib().sf_clip_grads(ptrs, optrs, sizes, codes, ocodes, len(grads), _p(norm), float(max_norm), _stream()),
+              "sf_clip_grads")
+
+
+def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
+    """``grad_norm`` and ``clip_grads`` in one call; returns the norm (before clipping)."""
+    grads = list(grads)
+    kind = _norm_kind(norm_type)
+    if not grads:
+        return torch.zeros((), dtype=torch.float32, device="cuda")
+    out = _clip_outputs(grads, out, "clip_grad_norm")
+    ptrs, sizes, codes = _grad_arrays(grads, "clip_grad_norm")
+    optrs, _, ocodes = (ptrs, sizes, codes) if out is grads else _grad_arrays(out, "clip_grad_norm")
+    dev = grads[0].device
+    if out[0].device != dev:
+        raise ValueError("clip_grad_norm: outputs must live on the gradients' device")
+    n = len(grads)
+    with _on_device_of(grads[0]):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=dev)
+        check(lib().sf_clip_grad_norm(ptrs, optrs, sizes, codes, ocodes, n, kind, float(max_norm), _p(norm), _p(scratch),
+                                      _stream()), "sf_clip_grad_norm")
+    return norm
 
 
 def _gemm_dtype(*ts) -> int:

@@ -156,6 +156,37 @@ def grad_sync_context(model, is_last_micro: bool):
     return contextlib.nullcontext()
 
 
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
+    """Scales the gradients of ``parameters`` in place so that their common norm is at most ``max_norm`` and returns
+    the norm they had; the training loop's call between ``backward`` and ``optimizer.step``
+    (legacy/main_llama.py:1997-2211), with the arguments of ``torch.nn.utils.clip_grad_norm_``.
+
+    Two launches for up to 448 gradients. The norm is one fp32 scalar on the device that was never rounded to the
+    gradients' dtype; gradients that need no scaling are read once and not written. ``norm_type``: 2 or ``inf``.
+    ``error_if_nonfinite`` reads the norm back. ``foreach`` is accepted and ignored. A parameter named twice is
+    counted and scaled once. With row shards the norm is this rank's: combine ``ops.grad_norm`` over the ranks and
+    call ``ops.clip_grads`` instead."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads, seen = [], set()
+    for p in parameters:
+        if p.grad is not None and id(p) not in seen:
+            seen.add(id(p))
+            grads.append(p.grad)
+    if not grads:
+        return torch.tensor(0.0)
+    if error_if_nonfinite:
+        norm = ops.grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
+                               "non-finite, so it cannot be clipped. To disable this error and scale the gradients "
+                               "by the non-finite norm anyway, set `error_if_nonfinite=False`")
+        ops.clip_grads(grads, norm, max_norm)
+        return norm
+    return ops.clip_grad_norm(grads, max_norm, norm_type)
+
+
 def _identify_glu_pairs(sparse_modules_dict):
     """{gate name: up name} of the GLU pairs whose gate layer asks for a joint mask
     (``...mlp.gate_proj`` / ``up_proj`` and ``...mlp.w1`` / ``w3``): legacy/utils.py:313-360."""

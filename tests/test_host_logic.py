@@ -318,3 +318,42 @@ def test_bench_schedules_and_host_threads():
     assert bench.schedule(5)[1] == pytest.approx(1.0 - 4 / 9)
     assert 1 <= bench.host_threads() <= (os.cpu_count() or 1)
     assert bench.layer_flops(8192, 4096, 4096) == pytest.approx(824.63e9, rel=1e-4)
+
+
+def test_gradient_clipping_refusals_without_a_gpu():
+    """Bad tables are refused on the host: nothing is launched, the code and message come back."""
+    import ctypes
+
+    from sparseforge_b200 import _lib, ops, utils
+
+    lib = _lib.lib()
+    P = (ctypes.c_void_p * 2)(4096, 4096)
+    S = (ctypes.c_int64 * 2)(16, 16)
+    D = (ctypes.c_int32 * 2)(_lib.SF_F32, _lib.SF_F32)
+    B = (ctypes.c_int32 * 2)(_lib.SF_F32, _lib.SF_I8)
+    odd = (ctypes.c_void_p * 2)(4096, 8194)
+    assert lib.sf_grad_norm(P, S, D, -1, 0, 16, 16, None) == -1
+    assert lib.sf_grad_norm(None, S, D, 2, 0, 16, 16, None) == -1
+    assert lib.sf_grad_norm(P, S, B, 2, 0, 16, 16, None) == -1
+    assert lib.sf_grad_norm(odd, S, D, 2, 0, 16, 16, None) == -3
+    assert lib.sf_grad_norm(P, S, D, 2, 2, 16, 16, None) == -1
+    assert lib.sf_grad_norm(P, S, D, 2, 0, None, 16, None) == -1
+    assert lib.sf_clip_grad_norm(P, P, S, D, D, 2, 0, 1.0, 16, 16, None) == -1  # the same gradient twice
+    assert b"overlaps" in lib.sf_last_error_string()
+    part = (ctypes.c_void_p * 2)(4096, 4096 + 32)
+    assert lib.sf_clip_grads(part, part, S, D, D, 2, 16, 1.0, None) == -1  # 16 floats reach 64 bytes
+    far = (ctypes.c_void_p * 2)(4096, 8192)
+    swapped = (ctypes.c_void_p * 2)(8192, 4096)
+    assert lib.sf_clip_grads(far, swapped, S, D, D, 2, 16, 1.0, None) == -1
+    assert lib.sf_clip_grads(far, far, S, D, D, 2, 16, -1.0, None) == -1
+    assert lib.sf_clip_grads(far, far, S, D, D, 2, None, 1.0, None) == -1
+    assert int(lib.sf_grad_norm_scratch_doubles(449)) == 2 * int(lib.sf_grad_norm_scratch_doubles(1))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.grad_norm([torch.zeros(8)])
+    with pytest.raises(NotImplementedError):
+        ops.grad_norm([torch.zeros(8)], 3.0)
+    p = torch.nn.Parameter(torch.zeros(8))
+    assert float(utils.clip_grad_norm_([p], 1.0)) == 0.0  # no gradient at all
+    p.grad = torch.zeros(8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        utils.clip_grad_norm_([p], 1.0)
