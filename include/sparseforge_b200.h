@@ -505,6 +505,31 @@ SF_API int sf_kl_div_bwd(const void* student, const void* teacher, int dtype, co
                   void* grad, void* stream);
 
 /*
+ * Linear layer in 8-bit integers with a scale per token and per output channel: the weights of a finalised layer
+ * stored and multiplied in 8 bits (legacy/eval_wiki_ppl.py:548-651 bakes the mask in and runs the dense product; no
+ * counterpart in the reference).
+ *   sf_int8_quantize_rows: a = max_k |x[r, k]|, scale[r] = a / 127, q[r, k] = round_half_even(127 x[r, k] / a), decided
+ *     as if the quotient were exact; a row of zeros gets scale 0, a row holding an infinity or NaN gets scale NaN (what
+ *     it produces is NaN) and zeros. x: [rows, cols] of `dtype` with row stride ld (elements); q: rows of
+ *     sf_int8_pitch(cols) bytes (cols rounded up to 16), the padding zero.
+ *   sf_int8_gemm: y[t, n] = float(sum_k xq[t, k] wq[n, k]) * x_scale[t] * w_scale[n] + bias[n]; xq [rows, pitch], wq
+ *     [out, pitch] with zero padding beyond `in`, bias (or NULL) and y [rows, out] of `dtype`. The sum is an exact
+ *     32-bit integer (in <= SF_INT8_MAX_IN), the rest fp32 with one rounding to y: a row's values do not depend on the other rows.
+ *   sf_int8_linear: both, for x of y's dtype (rows of stride ld); workspace of sf_int8_linear_workspace_bytes
+ *     bytes, 16-byte aligned, holds nothing between calls; calls that may run at the same time need one each.
+ * Any rows >= 0, in and out >= 1. 8-bit operands are 16-byte aligned. status as in sf_masked_gemm_fwd.
+ */
+#define SF_INT8_MAX_IN ((int64_t)131056)
+SF_API int64_t sf_int8_pitch(int64_t cols);
+SF_API int sf_int8_quantize_rows(const void* x, int dtype, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                          void* stream);
+SF_API int sf_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq, const float* w_scale, const void* bias,
+                 void* y, int dtype, int64_t rows, int64_t in, int64_t out, int32_t* status, void* stream);
+SF_API int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in);
+SF_API int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_scale, const void* bias, void* y,
+                   int dtype, int64_t rows, int64_t in, int64_t out, void* workspace, int32_t* status, void* stream);
+
+/*
  * Global norm of many gradient tensors, and clipping by it.
  *   replaces: torch.nn.utils.clip_grad_norm_ between backward and optimizer.step of the training loop,
  *             legacy/main_llama.py:1997-2211.

@@ -66,6 +66,11 @@ _SIGNATURES = {
     "sf_bias_grad": (c_int, [_P, c_int, _P, c_int64, c_int64, _P]),
     "sf_kl_div_fwd": (c_int, [_P, _P, c_int, c_int64, c_int64, c_double, c_double, _P, _P, _P]),
     "sf_kl_div_bwd": (c_int, [_P, _P, c_int, _P, _P, c_int64, c_int64, c_double, c_double, _P, _P]),
+    "sf_int8_pitch": (c_int64, [c_int64]),
+    "sf_int8_quantize_rows": (c_int, [_P, c_int, c_int64, _P, _P, c_int64, c_int64, _P]),
+    "sf_int8_gemm": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P]),
+    "sf_int8_linear_workspace_bytes": (c_int64, [c_int64, c_int64]),
+    "sf_int8_linear": (c_int, [_P, c_int64, _P, _P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P]),
     "sf_grad_norm_scratch_doubles": (c_int64, [c_int64]),
     "sf_grad_norm": (c_int, [_P, _P, _P, c_int64, c_int, _P, _P, _P]),
     "sf_clip_grads": (c_int, [_P, _P, _P, _P, _P, c_int64, _P, c_double, _P]),

@@ -24,6 +24,11 @@ namespace sf {
 constexpr int kGnThreads = 512;
 constexpr int kGnSlots = 1024;       // partial results one launch may write (its largest grid)
 constexpr int kGnVec = 8;            // elements per access group: 16 bytes of bf16, 32 of fp32
+// Loads in flight. Norm: 4 blocks of 512 threads per SM with two 16-byte loads each (bf16, four decoder layers, 1.62 GB:
+// 265 us = 6.1 TB/s; 2 blocks with four loads 282 us, 3 blocks with four 421 us, 2 blocks with eight 495 us). Scaling: 2
+// blocks with four (fp32 in and out, one layer: 256 us; 4 blocks with two 313 us; bf16 the same either way).
+constexpr int kGnNormBlocks = 4, kGnNormBatch = 2;
+constexpr int kGnClipBlocks = 2, kGnClipBatch = 4;
 constexpr int kGnChunkUnit = kGnThreads * kGnVec;
 
 enum { GN_L2 = SF_NORM_L2, GN_INF = SF_NORM_INF };
@@ -40,6 +45,8 @@ struct GnTable {
     GnTensor t[CAP];
     uint32_t first[CAP + 1];  // number of the tensor's first chunk; first[count] = chunks of the launch
     uint8_t kind[CAP];
+    uint32_t keep_from;       // chunks from here on are read again soon (the scaling starts with them)
+    int all_in_place;         // with a coefficient of 1 there is nothing to do
     int count;
     int chunk;  // elements per chunk, a multiple of kGnChunkUnit
 };
@@ -125,8 +132,14 @@ __device__ __forceinline__ NormAcc block_merge(NormAcc a, NormAcc* part) {
     return a;
 }
 
+// Read-only loads of the norm: the chunks that the scaling will read first (the last ones) are left in L2 as usual,
+// those before them are marked as the first to go.
+__device__ __forceinline__ uint4 ld_norm(const uint4* p, bool keep) {
+    return keep ? __ldg(p) : __ldcs(p);
+}
+
 template <int CAP, bool MAXNORM>
-__global__ void __launch_bounds__(kGnThreads)
+__global__ void __launch_bounds__(kGnThreads, kGnNormBlocks)
 grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __restrict__ slots) {
     __shared__ NormAcc part[kGnThreads / 32];
     NormAcc acc{0.0, 0u};
@@ -137,26 +150,48 @@ grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __res
         const int len = (int)min((int64_t)tab.chunk, tab.t[ti].n - at);
         const int kind = tab.kind[ti];
         const int nv = (kind & GN_VEC) ? len / kGnVec : 0;
+        const bool keep = c >= tab.keep_from;
         if (kind & GN_IN_BF16) {
             const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(tab.t[ti].in) + at;
             const uint4* q = reinterpret_cast<const uint4*>(p);
-            for (int v = threadIdx.x; v < nv; v += kGnThreads) {
-                float x[8];
-                unpack_bf16(__ldg(q + v), x);
-                acc8<MAXNORM>(acc, x);
+            for (int v = threadIdx.x; v < nv; v += kGnNormBatch * kGnThreads) {
+                uint4 r[kGnNormBatch];  // loads of a batch are in flight together
+#pragma unroll
+                for (int u = 0; u < kGnNormBatch; ++u)
+                    if (v + u * kGnThreads < nv) r[u] = ld_norm(q + v + u * kGnThreads, keep);
+#pragma unroll
+                for (int u = 0; u < kGnNormBatch; ++u)
+                    if (v + u * kGnThreads < nv) {
+                        float x[8];
+                        unpack_bf16(r[u], x);
+                        acc8<MAXNORM>(acc, x);
+                    }
             }
             for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) acc1<MAXNORM>(acc, __bfloat162float(p[i]));
         } else {
             const float* p = static_cast<const float*>(tab.t[ti].in) + at;
             const uint4* q = reinterpret_cast<const uint4*>(p);
-            for (int v = threadIdx.x; v < nv; v += kGnThreads) {
-                float x[8];
-                unpack_f32(__ldg(q + 2 * v), __ldg(q + 2 * v + 1), x);
-                acc8<MAXNORM>(acc, x);
+            for (int v = threadIdx.x; v < nv; v += kGnNormBatch / 2 * kGnThreads) {
+                uint4 r[kGnNormBatch];
+#pragma unroll
+                for (int u = 0; u < kGnNormBatch / 2; ++u)
+                    if (v + u * kGnThreads < nv) {
+                        r[2 * u] = ld_norm(q + 2 * (v + u * kGnThreads), keep);
+                        r[2 * u + 1] = ld_norm(q + 2 * (v + u * kGnThreads) + 1, keep);
+                    }
+#pragma unroll
+                for (int u = 0; u < kGnNormBatch / 2; ++u)
+                    if (v + u * kGnThreads < nv) {
+                        float x[8];
+                        unpack_f32(r[2 * u], r[2 * u + 1], x);
+                        acc8<MAXNORM>(acc, x);
+                    }
             }
             for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) acc1<MAXNORM>(acc, p[i]);
         }
     }
+    // the kernel behind this one may be set up meanwhile; it waits for these slots
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     acc = block_merge(acc, part);
     if (threadIdx.x == 0) slots[blockIdx.x] = MAXNORM ? (double)__uint_as_float(acc.top) : acc.sum;
 }
@@ -179,6 +214,7 @@ __global__ void __launch_bounds__(kGnThreads)
 grad_norm_final_kernel(const double* __restrict__ slots, int count, int kind, float* __restrict__ norm) {
     __shared__ NormAcc part[kGnThreads / 32];
     __shared__ double value;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const double v = norm_of_slots(slots, count, kind == GN_INF, part, &value);
     if (threadIdx.x == 0) *norm = (float)v;
 }
@@ -186,11 +222,12 @@ grad_norm_final_kernel(const double* __restrict__ slots, int count, int kind, fl
 // out = in * c. slots: the norm's partial results, which every block adds up for itself (norm_out gets the
 // value); or, with slots = NULL, the norm is read from norm_in.
 template <int CAP>
-__global__ void __launch_bounds__(kGnThreads)
+__global__ void __launch_bounds__(kGnThreads, kGnClipBlocks)
 grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restrict__ slots, int slot_count, int kind,
                  const float* norm_in, float* norm_out, double max_norm) {
     __shared__ NormAcc part[kGnThreads / 32];
     __shared__ double value;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     double norm;
     if (slots != nullptr) {
         norm = norm_of_slots(slots, slot_count, kind == GN_INF, part, &value);
@@ -200,6 +237,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
     }
     const double ratio = max_norm / (norm + 1e-6);
     const float c = ratio >= 1.0 ? 1.0f : (float)ratio;  // a NaN stays one
+    if (c == 1.0f && tab.all_in_place) return;
     const uint32_t chunks = tab.first[tab.count];
     for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
         const uint32_t ch = chunks - 1 - k;  // backwards: what the norm read last is still in L2
@@ -212,14 +250,33 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
         const bool ib = ent & GN_IN_BF16, ob = ent & GN_OUT_BF16;
         const char* ip = static_cast<const char*>(tab.t[ti].in) + at * (ib ? 2 : 4);
         char* op = static_cast<char*>(tab.t[ti].out) + at * (ob ? 2 : 4);
-        for (int v = threadIdx.x; v < nv; v += kGnThreads) {
-            float x[8];
-            if (ib) unpack_bf16(reinterpret_cast<const uint4*>(ip)[v], x);
-            else unpack_f32(reinterpret_cast<const uint4*>(ip)[2 * v], reinterpret_cast<const uint4*>(ip)[2 * v + 1], x);
+        if (ib && ob) {
+            const uint4* q = reinterpret_cast<const uint4*>(ip);
+            for (int v = threadIdx.x; v < nv; v += kGnClipBatch * kGnThreads) {
+                uint4 r[kGnClipBatch];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= c;
-            if (ob) Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(op) + v * kGnVec, x);
-            else Vec8<float>::store(reinterpret_cast<float*>(op) + v * kGnVec, x);
+                for (int u = 0; u < kGnClipBatch; ++u)
+                    if (v + u * kGnThreads < nv) r[u] = q[v + u * kGnThreads];
+#pragma unroll
+                for (int u = 0; u < kGnClipBatch; ++u)
+                    if (v + u * kGnThreads < nv) {
+                        float x[8];
+                        unpack_bf16(r[u], x);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) x[i] *= c;
+                        Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(op) + (v + u * kGnThreads) * kGnVec, x);
+                    }
+            }
+        } else {
+            for (int v = threadIdx.x; v < nv; v += kGnThreads) {
+                float x[8];
+                if (ib) unpack_bf16(reinterpret_cast<const uint4*>(ip)[v], x);
+                else unpack_f32(reinterpret_cast<const uint4*>(ip)[2 * v], reinterpret_cast<const uint4*>(ip)[2 * v + 1], x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= c;
+                if (ob) Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(op) + v * kGnVec, x);
+                else Vec8<float>::store(reinterpret_cast<float*>(op) + v * kGnVec, x);
+            }
         }
         for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) {
             const float x = (ib ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(ip)[i])
@@ -233,7 +290,9 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
 // ---------------------------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------------------------
-constexpr int kGnCap = 448;  // tensors per launch: a table of 13 KiB, below the 32 KiB of kernel parameters
+constexpr int kGnCap = 448;       // tensors per launch: a table of 13 KiB, below the 32 KiB of kernel parameters
+constexpr int kGnCapSmall = 32;   // a table of 1 KiB for short lists
+constexpr int64_t kGnKeepBytes = 32 << 20;  // what the norm leaves in the 126 MB L2 for the scaling
 
 static int64_t gn_launches(int64_t count) { return count <= 0 ? 1 : (count + kGnCap - 1) / kGnCap; }
 
@@ -282,13 +341,14 @@ static int gn_check_overlap(const char* who, const void* const* grads, void* con
     return SF_OK;
 }
 
-static int gn_grid(int64_t chunks) {
-    const int64_t cap = std::min<int64_t>(kGnSlots, (int64_t)sm_count() * 4);
+static int gn_grid(int64_t chunks, int blocks_per_sm) {
+    const int64_t cap = std::min<int64_t>(kGnSlots, (int64_t)sm_count() * blocks_per_sm);
     return (int)std::max<int64_t>(1, std::min(chunks, cap));
 }
 
 // Fills the table with tensors [from, to). Returns the number of chunks.
-static int64_t gn_fill(GnTable<kGnCap>& tab, const void* const* grads, void* const* outs, const int64_t* sizes,
+template <int CAP>
+static int64_t gn_fill(GnTable<CAP>& tab, const void* const* grads, void* const* outs, const int64_t* sizes,
                        const int32_t* in_dt, const int32_t* out_dt, int64_t from, int64_t to) {
     int64_t total = 0;
     for (int64_t i = from; i < to; ++i) total += sizes[i];
@@ -299,6 +359,7 @@ static int64_t gn_fill(GnTable<kGnCap>& tab, const void* const* grads, void* con
     while (total / chunk > 0x3fffffff) chunk *= 2;
     tab.chunk = (int)chunk;
     tab.count = 0;
+    tab.all_in_place = 1;
     uint32_t c = 0;
     for (int64_t i = from; i < to; ++i) {
         if (sizes[i] == 0) continue;
@@ -309,42 +370,89 @@ static int64_t gn_fill(GnTable<kGnCap>& tab, const void* const* grads, void* con
         tab.kind[k] = (uint8_t)((in_dt[i] == SF_BF16 ? GN_IN_BF16 : 0) | (odt == SF_BF16 ? GN_OUT_BF16 : 0) |
                                 (aligned16(grads[i]) && aligned16(o) ? GN_VEC : 0) |
                                 (o == grads[i] && odt == in_dt[i] ? GN_IN_PLACE : 0));
+        tab.all_in_place &= (tab.kind[k] & GN_IN_PLACE) != 0;
         tab.first[k] = c;
         c += (uint32_t)((sizes[i] + chunk - 1) / chunk);
     }
     tab.first[tab.count] = c;
+    const int64_t keep = kGnKeepBytes / (chunk * 2);
+    tab.keep_from = (uint32_t)std::max<int64_t>(0, (int64_t)c - keep);
     return c;
 }
 
-// Launches the partial sums of all tensors; *slot_count is the number of slots written.
+// Launch behind the kernel before it in the stream: set up while that one still runs, waits for its results.
+template <typename... KArgs, typename... Args>
+static cudaError_t gn_launch_dependent(void (*kern)(KArgs...), int grid, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(kGnThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+// Launches the partial sums of tensors [from, to); *slots grows by the number of slots written.
+template <int CAP>
+static int gn_partials_part(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t from, int64_t to,
+                            int kind, double* scratch, int* slots, cudaStream_t st) {
+    GnTable<CAP> tab;
+    const int64_t chunks = gn_fill(tab, grads, nullptr, sizes, dtypes, nullptr, from, to);
+    if (chunks == 0) return SF_OK;
+    const int grid = gn_grid(chunks, kGnNormBlocks);
+    if (kind == GN_INF) grad_norm_partial_kernel<CAP, true><<<grid, kGnThreads, 0, st>>>(tab, scratch + *slots);
+    else grad_norm_partial_kernel<CAP, false><<<grid, kGnThreads, 0, st>>>(tab, scratch + *slots);
+    SF_CHECK_CUDA(cudaGetLastError());
+    *slots += grid;
+    return SF_OK;
+}
+
 static int gn_partials(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,
-                       double* scratch, int* slot_count, cudaStream_t st) {
-    int slots = 0;
+                       double* scratch, int* slots, cudaStream_t st) {
+    *slots = 0;
     for (int64_t from = 0; from < count; from += kGnCap) {
-        GnTable<kGnCap> tab;
-        const int64_t chunks = gn_fill(tab, grads, nullptr, sizes, dtypes, nullptr, from, std::min(count, from + kGnCap));
-        if (chunks == 0) continue;
-        const int grid = gn_grid(chunks);
-        if (kind == GN_INF) grad_norm_partial_kernel<kGnCap, true><<<grid, kGnThreads, 0, st>>>(tab, scratch + slots);
-        else grad_norm_partial_kernel<kGnCap, false><<<grid, kGnThreads, 0, st>>>(tab, scratch + slots);
-        SF_CHECK_CUDA(cudaGetLastError());
-        slots += grid;
+        const int64_t to = std::min(count, from + kGnCap);
+        const int rc = to - from <= kGnCapSmall
+                           ? gn_partials_part<kGnCapSmall>(grads, sizes, dtypes, from, to, kind, scratch, slots, st)
+                           : gn_partials_part<kGnCap>(grads, sizes, dtypes, from, to, kind, scratch, slots, st);
+        if (rc) return rc;
     }
-    *slot_count = slots;
+    return SF_OK;
+}
+
+template <int CAP>
+static int gn_scale_part(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dt,
+                         const int32_t* out_dt, int64_t from, int64_t to, const double* slots, int slot_count, int kind,
+                         const float* norm_in, float* norm_out, double max_norm, bool dependent, cudaStream_t st) {
+    GnTable<CAP> tab;
+    const int grid = gn_grid(gn_fill(tab, grads, outs, sizes, in_dt, out_dt, from, to), kGnClipBlocks);
+    if (dependent)
+        SF_CHECK_CUDA(gn_launch_dependent(grad_clip_kernel<CAP>, grid, st, tab, slots, slot_count, kind, norm_in,
+                                          norm_out, max_norm));
+    else
+        grad_clip_kernel<CAP><<<grid, kGnThreads, 0, st>>>(tab, slots, slot_count, kind, norm_in, norm_out, max_norm);
+    SF_CHECK_CUDA(cudaGetLastError());
     return SF_OK;
 }
 
 static int gn_scale(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dt,
                     const int32_t* out_dt, int64_t count, const double* slots, int slot_count, int kind,
                     const float* norm_in, float* norm_out, double max_norm, cudaStream_t st) {
-    // the tensors the norm read last come first
-    for (int64_t part = gn_launches(count) - 1; part >= 0; --part) {
-        GnTable<kGnCap> tab;
-        const int64_t from = part * kGnCap;
-        const int64_t chunks = gn_fill(tab, grads, outs, sizes, in_dt, out_dt, from, std::min(count, from + kGnCap));
-        grad_clip_kernel<kGnCap><<<gn_grid(chunks), kGnThreads, 0, st>>>(tab, slots, slot_count, kind, norm_in,
-                                                                        part == 0 ? norm_out : nullptr, max_norm);
-        SF_CHECK_CUDA(cudaGetLastError());
+    const int64_t parts = gn_launches(count);
+    // the tensors the norm read last come first; only the first of the launches follows the norm directly
+    for (int64_t part = parts - 1; part >= 0; --part) {
+        const int64_t from = part * kGnCap, to = std::min(count, from + kGnCap);
+        float* no = part == 0 ? norm_out : nullptr;
+        const bool dep = slot_count > 0 && part == parts - 1;
+        const int rc = to - from <= kGnCapSmall
+                           ? gn_scale_part<kGnCapSmall>(grads, outs, sizes, in_dt, out_dt, from, to, slots, slot_count, kind,
+                                                        norm_in, no, max_norm, dep, st)
+                           : gn_scale_part<kGnCap>(grads, outs, sizes, in_dt, out_dt, from, to, slots, slot_count, kind,
+                                                   norm_in, no, max_norm, dep, st);
+        if (rc) return rc;
     }
     return SF_OK;
 }
@@ -365,7 +473,8 @@ int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* 
     cudaStream_t st = (cudaStream_t)stream;
     int slots = 0;
     if (int rc = gn_partials(grads, sizes, dtypes, count, kind, scratch, &slots, st)) return rc;
-    grad_norm_final_kernel<<<1, kGnThreads, 0, st>>>(scratch, slots, kind, norm);
+    if (slots > 0) SF_CHECK_CUDA(gn_launch_dependent(grad_norm_final_kernel, 1, st, scratch, slots, kind, norm));
+    else grad_norm_final_kernel<<<1, kGnThreads, 0, st>>>(scratch, slots, kind, norm);
     SF_CHECK_CUDA(cudaGetLastError());
     return SF_OK;
 }

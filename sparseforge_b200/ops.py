@@ -5,8 +5,8 @@ torch is used here for device memory and streams only; the arithmetic is in the 
 """
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from contextlib import nullcontext
 from typing import Optional
 
@@ -15,6 +15,8 @@ import torch
 from . import _lib
 from ._lib import SF_BF16, SF_F32, SF_I8, check, lib
 
+_GET_DTYPE, _GET_SHAPE = torch.Tensor.dtype.__get__, torch.Tensor.shape.__get__
+_GRAD_DTYPES = {torch.float32, torch.bfloat16}
 _DT = {torch.float32: SF_F32, torch.bfloat16: SF_BF16, torch.int8: SF_I8}
 
 
@@ -431,25 +433,41 @@ def _dense_view(t: torch.Tensor) -> torch.Tensor:
 
 
 def _grad_arrays(ts, what):
-    """(addresses, element counts, dtype codes) of a list of gradients as C arrays, after checking them."""
-    n = len(ts)
-    try:
-        codes = [_DT[t.dtype] for t in ts]
-    except KeyError:
-        raise TypeError(f"{what}: gradients must be float32 or bfloat16, got {sorted({str(t.dtype) for t in ts})}") from None
-    if SF_I8 in codes:
-        raise TypeError(f"{what}: gradients must be float32 or bfloat16")
-    dev = ts[0].device
-    for t in ts:
-        if t.device != dev or not t.is_cuda:
-            _cuda(t)
-            raise ValueError(f"{what}: all gradients of a call must live on one device")
-        if t.layout != torch.strided:
-            raise RuntimeError(f"{what}: sparse gradients are not supported")
-        if not t.is_contiguous() and not _dense_view(t).is_contiguous():
-            raise RuntimeError("sparseforge_b200: tensors must be contiguous (or a dense permutation)")
-    return ((ctypes.c_void_p * n)(*[t.data_ptr() for t in ts]), (ctypes.c_int64 * n)(*[t.numel() for t in ts]),
-            (ctypes.c_int32 * n)(*codes))
+    """(addresses, element counts, dtype codes, all contiguous) of a list of gradients, after checking them. Models
+    have hundreds of gradients: whole-list calls cost the host a third of a loop over attributes."""
+    devices = set(map(torch.Tensor.get_device, ts))
+    if len(devices) != 1 or -1 in devices:
+        _cuda(*ts)
+        raise ValueError(f"{what}: all gradients of a call must live on one device")
+    dtypes = list(map(_GET_DTYPE, ts))
+    if not _GRAD_DTYPES.issuperset(dtypes):
+        raise TypeError(f"{what}: gradients must be float32 or bfloat16, got {sorted(map(str, set(dtypes)))}")
+    contiguous = all(map(torch.Tensor.is_contiguous, ts))  # raises for sparse layouts
+    if not contiguous and not all(_dense_view(t).is_contiguous() for t in ts):
+        raise RuntimeError("sparseforge_b200: tensors must be contiguous (or a dense permutation)")
+    return (array("Q", map(torch.Tensor.data_ptr, ts)), array("q", map(torch.Tensor.numel, ts)),
+            array("i", map(_DT.__getitem__, dtypes)), contiguous)
+
+
+def _clip_arrays(grads, out, what):
+    """The C arrays of gradients and outputs: (addresses, output addresses, counts, dtypes, output dtypes)."""
+    ptrs, sizes, codes, dense = _grad_arrays(grads, what)
+    if out is None:
+        return ptrs, ptrs, sizes, codes, codes
+    out = list(out)
+    if len(out) != len(grads):
+        raise ValueError(f"{what}: {len(grads)} gradients, {len(out)} outputs")
+    optrs, _, ocodes, odense = _grad_arrays(out, what)
+    if out[0].device != grads[0].device:
+        raise ValueError(f"{what}: outputs must live on the gradients' device")
+    if list(map(_GET_SHAPE, out)) != list(map(_GET_SHAPE, grads)) or (
+            not (dense and odense) and any(o.stride() != g.stride() for g, o in zip(grads, out))):
+        raise ValueError(f"{what}: an output must have its gradient's shape and strides")
+    return ptrs, optrs, sizes, codes, ocodes
+
+
+def _addr(a: array) -> int:
+    return a.buffer_info()[0]
 
 
 def _norm_kind(norm_type) -> int:
@@ -461,18 +479,6 @@ def _norm_kind(norm_type) -> int:
     raise NotImplementedError(f"gradient norm of type {norm_type!r}: 2 and inf are built")
 
 
-def _clip_outputs(grads, out, what):
-    if out is None:
-        return grads
-    out = list(out)
-    if len(out) != len(grads):
-        raise ValueError(f"{what}: {len(grads)} gradients, {len(out)} outputs")
-    for g, o in zip(grads, out):
-        if o.shape != g.shape or not (o.stride() == g.stride() or (o.is_contiguous() and g.is_contiguous())):
-            raise ValueError(f"{what}: an output must have its gradient's shape and strides")
-    return out
-
-
 def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     """Norm over every element of all tensors in ``grads`` (fp32 / bf16, mixed) as one fp32 scalar on their device:
     ``norm_type`` 2 (root of the sum of squares) or ``math.inf``. Nothing is read back."""
@@ -480,12 +486,12 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     kind = _norm_kind(norm_type)
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda")
-    ptrs, sizes, codes = _grad_arrays(grads, "grad_norm")
+    ptrs, sizes, codes, _ = _grad_arrays(grads, "grad_norm")
     n = len(grads)
     with _on_device_of(grads[0]):
         norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
         scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=grads[0].device)
-        check(lib().sf_grad_norm(ptrs, sizes, codes, n, kind, _p(norm), _p(scratch), _stream()), "sf_grad_norm")
+        check(lib().sf_grad_norm(_addr(ptrs), _addr(sizes), _addr(codes), n, kind, _p(norm), _p(scratch), _stream()), "sf_grad_norm")
     return norm
 
 
@@ -496,15 +502,13 @@ def clip_grads(grads, norm, max_norm, out=None) -> None:
     grads = list(grads)
     if not grads:
         return
-    out = _clip_outputs(grads, out, "clip_grads")
-    ptrs, sizes, codes = _grad_arrays(grads, "clip_grads")
-    optrs, _, ocodes = (ptrs, sizes, codes) if out is grads else _grad_arrays(out, "clip_grads")
+    ptrs, optrs, sizes, codes, ocodes = _clip_arrays(grads, out, "clip_grads")
     _cuda(norm)
-    if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != grads[0].device or out[0].device != norm.device:
+    if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != grads[0].device:
         raise TypeError("clip_grads: norm must be one float32 on the gradients' device")
     with _on_device_of(norm):
-        check(lib().sf_clip_grads(ptrs, optrs, sizes, codes, ocodes, len(grads), _p(norm), float(max_norm), _stream()),
-              "sf_clip_grads")
+        check(lib().sf_clip_grads(_addr(ptrs), _addr(optrs), _addr(sizes), _addr(codes), _addr(ocodes), len(grads),
+                                  _p(norm), float(max_norm), _stream()), "sf_clip_grads")
 
 
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
@@ -513,18 +517,13 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
     kind = _norm_kind(norm_type)
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda")
-    out = _clip_outputs(grads, out, "clip_grad_norm")
-    ptrs, sizes, codes = _grad_arrays(grads, "clip_grad_norm")
-    optrs, _, ocodes = (ptrs, sizes, codes) if out is grads else _grad_arrays(out, "clip_grad_norm")
-    dev = grads[0].device
-    if out[0].device != dev:
-        raise ValueError("clip_grad_norm: outputs must live on the gradients' device")
-    n = len(grads)
+    ptrs, optrs, sizes, codes, ocodes = _clip_arrays(grads, out, "clip_grad_norm")
+    dev, n = grads[0].device, len(grads)
     with _on_device_of(grads[0]):
         norm = torch.empty((), dtype=torch.float32, device=dev)
         scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=dev)
-        check(lib().sf_clip_grad_norm(ptrs, optrs, sizes, codes, ocodes, n, kind, float(max_norm), _p(norm), _p(scratch),
-                                      _stream()), "sf_clip_grad_norm")
+        check(lib().sf_clip_grad_norm(_addr(ptrs), _addr(optrs), _addr(sizes), _addr(codes), _addr(ocodes), n, kind,
+                                      float(max_norm), _p(norm), _p(scratch), _stream()), "sf_clip_grad_norm")
     return norm
 
 
@@ -694,6 +693,96 @@ def sparse24_gemm(x2d, values, meta_tc, bias=None, status=None, splits=0):
         return y
     check(lib().sf_sparse24_gemm(_p(x2d), _p(values), _p(meta_tc), _p(bias), _p(y), T, k, out, _p(status), _stream()),
           "sf_sparse24_gemm")
+    return y
+
+
+# ----------------------------------------------------------------------------------------
+# 8-bit integer products with a scale per token and per output channel
+# ----------------------------------------------------------------------------------------
+def _int8_rows(x2d, what):
+    """Row stride of a 2-D float32 / bfloat16 CUDA tensor whose rows are contiguous."""
+    if not x2d.is_cuda:
+        _cuda(x2d)
+    if x2d.dim() != 2 or x2d.dtype not in _GRAD_DTYPES:
+        raise TypeError(f"{what}: a 2-D float32 or bfloat16 tensor expected, got {x2d.dim()}-D {x2d.dtype}")
+    rows, cols = x2d.shape
+    if cols == 0:
+        raise ValueError(f"{what}: rows must hold at least one element")
+    if (cols > 1 and x2d.stride(1) != 1) or (rows > 1 and x2d.stride(0) < cols):
+        raise RuntimeError(f"{what}: rows must be contiguous and must not overlap (strides {tuple(x2d.stride())})")
+    return max(x2d.stride(0), cols)
+
+
+def _int8_weight(wq, w_scale, k, dev, what):
+    """(out, ctypes-ready checks) of an 8-bit weight [out, k rounded up to 16] with its scales."""
+    _cuda(wq, w_scale)
+    if wq.dtype != torch.int8 or w_scale.dtype != torch.float32 or wq.dim() != 2 or w_scale.shape != wq.shape[:1]:
+        raise TypeError(f"{what}: weight int8 [out, pitch] and float32 scales [out] expected")
+    if wq.shape[1] != (k + 15) // 16 * 16:
+        raise ValueError(f"{what}: x has {k} features, weight rows of {wq.shape[1]} bytes (expected {(k + 15) // 16 * 16})")
+    if wq.device != dev or w_scale.device != dev:
+        raise ValueError(f"{what}: all tensors of a call must live on one device")
+    return wq.shape[0]
+
+
+def _int8_bias(bias, out, dtype, dev, what):
+    if bias is None:
+        return
+    _cuda(bias)
+    if bias.dtype != dtype or bias.shape != (out,) or bias.device != dev:
+        raise TypeError(f"{what}: bias must be {dtype} [{out}] on {dev}")
+
+
+def int8_quantize_rows(x2d):
+    """(q int8 [rows, cols rounded up to 16], scale float32 [rows]): every row divided by its largest magnitude over
+    127 and rounded (half to even). Rows may be strided. See ``sf_int8_quantize_rows``."""
+    ld = _int8_rows(x2d, "int8_quantize_rows")
+    rows, cols = x2d.shape
+    q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=x2d.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=x2d.device)
+    with _on_device_of(x2d):
+        check(lib().sf_int8_quantize_rows(_p(x2d), _dt(x2d), ld, _p(q), _p(scale), rows, cols, _stream()),
+              "sf_int8_quantize_rows")
+    return q, scale
+
+
+def int8_gemm(xq, x_scale, wq, w_scale, bias=None, out_dtype=torch.bfloat16, status=None):
+    """y[T, out] = (xq @ wq^T) * x_scale[:, None] * w_scale (+ bias) for operands of ``int8_quantize_rows``; the
+    sum is an exact 32-bit integer."""
+    _cuda(xq, x_scale, status)
+    if xq.dtype != torch.int8 or x_scale.dtype != torch.float32 or xq.dim() != 2 or x_scale.shape != xq.shape[:1]:
+        raise TypeError("int8_gemm: xq int8 [rows, pitch] and float32 scales [rows] expected")
+    if out_dtype not in _GRAD_DTYPES:
+        raise TypeError("int8_gemm: out_dtype must be float32 or bfloat16")
+    T, k = xq.shape
+    dev = xq.device
+    if x_scale.device != dev:
+        raise ValueError("int8_gemm: all tensors of a call must live on one device")
+    out = _int8_weight(wq, w_scale, k, dev, "int8_gemm")
+    _int8_bias(bias, out, out_dtype, dev, "int8_gemm")
+    y = torch.empty((T, out), dtype=out_dtype, device=dev)
+    with _on_device_of(xq):
+        check(lib().sf_int8_gemm(_p(xq), _p(x_scale), _p(wq), _p(w_scale), _p(bias), _p(y), _DT[out_dtype], T, k, out,
+                                 _p(status), _stream()), "sf_int8_gemm")
+    return y
+
+
+def int8_linear(x2d, wq, w_scale, bias=None, status=None):
+    """y[T, out] = x2d @ dequantised(wq)^T (+ bias) in x2d's dtype: the rows of x2d are quantised on the fly
+    (``int8_quantize_rows``) and multiplied in 8 bits (``int8_gemm``)."""
+    ld = _int8_rows(x2d, "int8_linear")
+    T, k = x2d.shape
+    dev = x2d.device
+    out = _int8_weight(wq, w_scale, k, dev, "int8_linear")
+    _int8_bias(bias, out, x2d.dtype, dev, "int8_linear")
+    y = torch.empty((T, out), dtype=x2d.dtype, device=dev)
+    if T == 0:
+        return y
+    # a workspace of its own per call: calls on two streams, or in two captured graphs, never share one
+    ws = torch.empty(int(lib().sf_int8_linear_workspace_bytes(T, k)), dtype=torch.uint8, device=dev)
+    with _on_device_of(x2d):
+        check(lib().sf_int8_linear(_p(x2d), ld, _p(wq), _p(w_scale), _p(bias), _p(y), _dt(x2d), T, k, out, _p(ws),
+                                   _p(status), _stream()), "sf_int8_linear")
     return y
 
 

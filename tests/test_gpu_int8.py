@@ -1,0 +1,276 @@
+"""8-bit linear layer against a 64-bit computation from its definition.
+
+The quantised integers have to be equal. Tolerances of the product: the scale of a row is a / 127 rounded once (2^-24),
+converting the integer sum rounds once, each of the two multiplications by a scale rounds once, and both scales are
+rounded: 5 * 2^-24 relative before the bias; adding the bias rounds once more (2^-24 of the result), storing to bf16
+half a step (finfo.eps / 2).
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+MAX_IN = 131056
+DT = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def _ops():
+    from sparseforge_b200 import ops
+
+    return ops
+
+
+def _quantise64(x):
+    x = x.double()
+    a = x.abs().amax(dim=1, keepdim=True)
+    q = torch.where(a > 0, 127.0 * x / torch.where(a > 0, a, torch.ones_like(a)), torch.zeros_like(x)).round()
+    return q, (a / 127.0).squeeze(1)
+
+
+def _exact(x, w, bias=None):
+    """(y, magnitude before the bias) in 64 bits."""
+    xq, xs = _quantise64(x)
+    wq, ws = _quantise64(w)
+    y = (xq @ wq.t()) * xs[:, None] * ws
+    return (y if bias is None else y + bias.double()), y.abs()
+
+
+def _check(y, want, mag, dtype):
+    got = y.double()
+    tol = 6 * U * mag + (U + torch.finfo(dtype).eps / 2) * want.abs() + 1e-37
+    bad = (got - want).abs() > tol
+    assert not bad.any(), (int(bad.sum()), float(((got - want).abs() / tol).max()), bad.nonzero()[:4].tolist())
+
+
+def _inputs(T, k, n, dtype, bias=False, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 131 * T + 7 * k + n)
+    x = torch.randn(T, k, device="cuda", generator=g)
+    x[:, torch.randint(0, k, (max(1, k // 200),), device="cuda", generator=g)] *= 9.0
+    w = torch.randn(n, k, device="cuda", generator=g) * 0.05
+    b = (torch.randn(n, device="cuda", generator=g)).to(dtype) if bias else None
+    return x.to(dtype), w.to(torch.bfloat16), b
+
+
+# ------------------------------------------------------------------------------------------------ rows
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols", [1, 3, 8, 15, 16, 17, 64, 255, 1000, 1003, 2048, 4096, 4104, 11008, 16384, 16391, 70001])
+def test_quantised_rows(cols, dtype):
+    g = torch.Generator(device="cuda").manual_seed(cols)
+    x = torch.randn(9, cols, device="cuda", generator=g).to(DT[dtype])
+    x[3] = 0.0
+    x[4] *= 1e-30
+    x[5] = (torch.randint(-508, 509, (cols,), device="cuda", generator=g) / 4.0).to(DT[dtype])  # ties, where max is 127
+    x[5, 0] = 127.0
+    x[5].clamp_(-127.0, 127.0)
+    x[6, cols // 2] = 1e20
+    q, s = _ops().int8_quantize_rows(x)
+    want, scale = _quantise64(x)
+    assert q.shape == (9, (cols + 15) // 16 * 16) and q.dtype == torch.int8
+    assert torch.equal(q[:, :cols].double(), want)
+    assert not q[:, cols:].any()
+    assert ((s.double() - scale).abs() <= U * scale).all()
+    assert float(s[3]) == 0.0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantised_rows_near_and_on_halves(dtype):
+    """Quotients exactly half-way go to the even integer; the neighbours of such values go to their own side."""
+    rows = []
+    for a in (127.0, 254.0, 1.9921875, 0.49609375, 2.0 ** -100 * 127, 2.0 ** 100 * 127, 3.0, 1.4140625):
+        a_t = torch.tensor(a, dtype=DT[dtype]).double()
+        h = (torch.arange(0, 127, dtype=torch.float64) + 0.5) * a_t / 127.0
+        near = torch.cat([h, torch.nextafter(h.float(), torch.tensor(math.inf)).double(),
+                          torch.nextafter(h.float(), torch.tensor(-math.inf)).double()]).to(DT[dtype])
+        near[-1] = a_t.to(DT[dtype])
+        rows.append(near.clamp(max=float(a_t)))
+    x = torch.stack(rows).cuda()
+    x = torch.cat([x, -x])
+    q, _ = _ops().int8_quantize_rows(x)
+    want, _ = _quantise64(x)
+    assert torch.equal(q[:, :x.shape[1]].double(), want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_quantised_rows_at_the_ends_of_the_range(dtype):
+    top = torch.finfo(DT[dtype]).max
+    tiny = 2.0 ** -133 if dtype == "bf16" else 2.0 ** -149
+    for a in (top, top / 2, 1e37, 1e-36, 1e-37, 1e-38, 64 * tiny, 3 * tiny, tiny):
+        x = (torch.linspace(-1.0, 1.0, 301, dtype=torch.float64) * a).to(DT[dtype]).cuda()[None]
+        q, s = _ops().int8_quantize_rows(x)
+        want, scale = _quantise64(x)
+        assert torch.equal(q[:, :301].double(), want), a
+        assert abs(float(s[0]) - float(scale[0])) <= U * float(scale[0]) + 2.0 ** -150
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [3, 6, 200])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_rows_with_infinities(bad, T, dtype):
+    """Such a row's result is NaN throughout; the other rows are what they are without it."""
+    x, w, b = _inputs(T, 100, 50, DT[dtype], bias=True)
+    ops = _ops()
+    wq, ws = ops.int8_quantize_rows(w)
+    clean = ops.int8_linear(x, wq, ws, b)
+    x[1, 99] = bad
+    q, s = ops.int8_quantize_rows(x)
+    assert math.isnan(float(s[1])) and not q[1].any()
+    y = ops.int8_linear(x, wq, ws, b)
+    assert torch.isnan(y[1]).all()
+    keep = [t for t in range(T) if t != 1]
+    assert torch.equal(y[keep], clean[keep])
+
+
+def test_strided_rows():
+    ops = _ops()
+    big = torch.randn(40, 300, device="cuda").bfloat16()
+    for view in (big[:, :64], big[:, 1:100], big[::2, 3:203], big[5:6, 7:]):
+        q, s = ops.int8_quantize_rows(view)
+        q2, s2 = ops.int8_quantize_rows(view.contiguous())
+        assert torch.equal(q, q2) and torch.equal(s, s2)
+        w = torch.randn(33, view.shape[1], device="cuda").bfloat16()
+        wq, ws = ops.int8_quantize_rows(w)
+        assert torch.equal(ops.int8_linear(view, wq, ws), ops.int8_linear(view.contiguous(), wq, ws))
+
+
+# ------------------------------------------------------------------------------------------------ product
+ROWS = [1, 2, 3, 4, 5, 8, 15, 16, 17, 31, 33, 64, 65, 127, 128, 129, 200, 256, 257, 511]
+SHAPES = [(16, 1), (1, 7), (100, 130), (128, 128), (256, 264), (500, 1000), (1003, 333), (2048, 96), (4096, 512)]
+
+
+@pytest.mark.parametrize("dtype,bias", [("bf16", False), ("bf16", True), ("f32", True)])
+@pytest.mark.parametrize("T", ROWS)
+def test_linear(T, dtype, bias):
+    ops = _ops()
+    for k, n in SHAPES:
+        x, w, b = _inputs(T, k, n, DT[dtype], bias)
+        wq, ws = ops.int8_quantize_rows(w)
+        y = ops.int8_linear(x, wq, ws, b)
+        assert y.shape == (T, n) and y.dtype == x.dtype
+        _check(y, *_exact(x, w, b), DT[dtype])
+        xq, xs = ops.int8_quantize_rows(x)
+        assert torch.equal(y, ops.int8_gemm(xq, xs, wq, ws, b, out_dtype=DT[dtype]))
+
+
+@pytest.mark.parametrize("T,k,n", [(1, 4096, 4096), (1, 11008, 4096), (3, 4096, 11008), (16, 4096, 11008), (100, 11008, 4096),
+                                   (512, 4096, 4096), (1000, 1500, 4096), (2048, 768, 2304), (4096, 4096, 1111)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_linear_at_real_sizes(T, k, n, dtype):
+    ops = _ops()
+    x, w, b = _inputs(T, k, n, DT[dtype], True, seed=9)
+    wq, ws = ops.int8_quantize_rows(w)
+    y = ops.int8_linear(x, wq, ws, b)
+    _check(y, *_exact(x, w, b), DT[dtype])
+    # a row's values do not depend on the rows beside it, whichever kernel the number of rows selects
+    for rows in (1, 2, 7, 40, 130, 300):
+        if rows < T:
+            assert torch.equal(ops.int8_linear(x[:rows], wq, ws, b), y[:rows]), rows
+    assert torch.equal(ops.int8_linear(x[T - 1:], wq, ws, b), y[T - 1:])
+
+
+@pytest.mark.parametrize("T", [1, 4, 9, 40, 300])
+def test_extreme_integers(T):
+    """-128 and 127 everywhere, at the largest reduction: the 32-bit sum is exact to its end."""
+    ops = _ops()
+    for k in (144, MAX_IN):
+        xq = torch.full((T, k), -128, dtype=torch.int8, device="cuda")
+        wq = torch.full((70, k), -128, dtype=torch.int8, device="cuda")
+        wq[1] = 127
+        wq[2, ::2] = 0
+        xs = torch.full((T,), 2.0 ** -10, device="cuda")
+        ws = torch.full((70,), 2.0 ** -8, device="cuda")
+        y = ops.int8_gemm(xq, xs, wq, ws, out_dtype=torch.float32)
+        want = torch.full((70,), 16384.0 * k, dtype=torch.float64)
+        want[1] = -128.0 * 127.0 * k
+        want[2] = 8192.0 * k
+        want = (want * 2.0 ** -18).cuda().expand(T, 70)
+        assert ((y.double() - want).abs() <= U * want.abs()).all()
+
+
+def test_no_rows_and_refusals():
+    ops = _ops()
+    x, w, b = _inputs(4, 64, 32, torch.bfloat16, True)
+    wq, ws = ops.int8_quantize_rows(w)
+    assert ops.int8_linear(x[:0], wq, ws).shape == (0, 32)
+    assert ops.int8_gemm(*ops.int8_quantize_rows(x[:0]), wq, ws).shape == (0, 32)
+    with pytest.raises(ValueError):
+        ops.int8_linear(x[:, :40], wq, ws)
+    with pytest.raises(TypeError):
+        ops.int8_linear(x.half(), wq, ws)
+    with pytest.raises(TypeError):
+        ops.int8_linear(x[0], wq, ws)
+    with pytest.raises(TypeError):
+        ops.int8_linear(x, wq.float(), ws)
+    with pytest.raises(TypeError):
+        ops.int8_linear(x, wq, ws[:-1])
+    with pytest.raises(TypeError):
+        ops.int8_linear(x, wq, ws, b.float())
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.int8_linear(x.t().contiguous().t(), wq, ws)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.int8_linear(x[:1].expand(4, 64), wq, ws)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.int8_linear(x, wq[:, ::2], ws)
+    with pytest.raises(RuntimeError, match="overflow"):
+        ops.int8_gemm(torch.zeros(1, MAX_IN + 16, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"),
+                      torch.zeros(1, MAX_IN + 16, dtype=torch.int8, device="cuda"), torch.ones(1, device="cuda"))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.int8_linear(x.cpu(), wq, ws)
+    buf = torch.zeros(64 * 32 + 1, dtype=torch.int8, device="cuda")[1:].view(32, 64)
+    with pytest.raises(RuntimeError, match="aligned"):
+        ops.int8_linear(x, buf, ws)
+
+
+@pytest.mark.parametrize("T", [1, 6, 40, 300])
+def test_rows_behind_the_last_are_left_alone(T):
+    from sparseforge_b200 import _lib
+
+    ops = _ops()
+    k, n = 200, 77
+    x, w, _ = _inputs(T, k, n, torch.bfloat16)
+    wq, ws = ops.int8_quantize_rows(w)
+    want = ops.int8_linear(x, wq, ws)
+    y = torch.full((T + 2, n), 5.0, device="cuda", dtype=torch.bfloat16)
+    work = torch.empty(int(_lib.lib().sf_int8_linear_workspace_bytes(T, k)), dtype=torch.uint8, device="cuda")
+    rc = _lib.lib().sf_int8_linear(x.data_ptr(), k, wq.data_ptr(), ws.data_ptr(), None, y[1:].data_ptr(), _lib.SF_BF16, T, k, n,
+                                   work.data_ptr(), None, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert torch.equal(y[1:T + 1], want) and (y[0] == 5.0).all() and (y[T + 1] == 5.0).all()
+
+
+def test_streams_and_graph_replay():
+    ops = _ops()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    cases = []
+    for T in (1, 7, 100, 400):
+        x, w, b = _inputs(T, 1000, 520, torch.bfloat16, True, seed=T)
+        wq, ws = ops.int8_quantize_rows(w)
+        cases.append((x, wq, ws, b, ops.int8_linear(x, wq, ws, b)))
+    torch.cuda.synchronize()
+    got = []
+    for rep in range(4):
+        for i, (x, wq, ws, b, want) in enumerate(cases):
+            with torch.cuda.stream((s1, s2)[(i + rep) % 2]):
+                got.append((ops.int8_linear(x, wq, ws, b), want))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for y, want in got)
+    graphs = []
+    for x, wq, ws, b, _ in cases:
+        ops.int8_linear(x, wq, ws, b)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ops.int8_linear(x, wq, ws, b)
+        graphs.append((g, y))
+    for rep in range(3):
+        for x, *_ in cases:
+            x.copy_(torch.randn_like(x))
+        torch.cuda.synchronize()
+        for i, (g, _) in enumerate(graphs):
+            with torch.cuda.stream((s1, s2)[i % 2]):
+                g.replay()
+        torch.cuda.synchronize()
+        for (x, wq, ws, b, _), (_, y) in zip(cases, graphs):
+            assert torch.equal(y, ops.int8_linear(x, wq, ws, b))
