@@ -758,6 +758,23 @@ int make_meta_tensor_map(CUtensorMap* map, const void* ptr, int64_t rows, int bo
     return SF_OK;
 }
 
+// Tensor map over a row-major byte matrix [outer, pitch] with a 128-byte-swizzled box of 128 bytes x box_outer rows
+// (8-bit operands; bytes and rows beyond the matrix read as zero). Encoded anew for every call.
+int make_byte_tensor_map(CUtensorMap* map, const void* ptr, int64_t pitch, int64_t outer, int box_outer) {
+    if (int rc = ensure_context()) return rc;
+    EncodeTiledFn fn = encode_tiled_fn();
+    if (!fn) return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)outer};
+    cuuint64_t strides[1] = {(cuuint64_t)pitch};
+    cuuint32_t box[2] = {128, (cuuint32_t)box_outer};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(SF_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit operand) failed with CUresult %d", (int)r);
+    return SF_OK;
+}
+
 // D[M,N] = alpha * A . B^T (+bias). a_mn / b_mn: operand stored with its M / N index contiguous
 // (as [K, M] / [K, N] row-major with leading dimension lda / ldb), else as [M, K] / [N, K].
 // The CTA-pair kernel serves every problem with more than one 128-row tile; setting

@@ -18,6 +18,7 @@
 #include <new>
 
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 
 namespace sf {
 
@@ -191,7 +192,7 @@ grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __res
         }
     }
     // the kernel behind this one may be set up meanwhile; it waits for these slots
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    ptx::launch_dependents();
     acc = block_merge(acc, part);
     if (threadIdx.x == 0) slots[blockIdx.x] = MAXNORM ? (double)__uint_as_float(acc.top) : acc.sum;
 }
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(kGnThreads)
 grad_norm_final_kernel(const double* __restrict__ slots, int count, int kind, float* __restrict__ norm) {
     __shared__ NormAcc part[kGnThreads / 32];
     __shared__ double value;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    ptx::dependency_wait();
     const double v = norm_of_slots(slots, count, kind == GN_INF, part, &value);
     if (threadIdx.x == 0) *norm = (float)v;
 }
@@ -227,7 +228,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
                  const float* norm_in, float* norm_out, double max_norm) {
     __shared__ NormAcc part[kGnThreads / 32];
     __shared__ double value;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    ptx::dependency_wait();
     double norm;
     if (slots != nullptr) {
         norm = norm_of_slots(slots, slot_count, kind == GN_INF, part, &value);

@@ -6,9 +6,16 @@
 // Rows of 8-bit operands are padded with zeros to a multiple of 16 bytes (pitch = cols rounded up). The
 // sum is an exact 32-bit integer (in <= 131056 keeps it below 2^31 for every pair of 8-bit values), so a value
 // does not depend on how the reduction is split, nor on the number of rows of the call.
+#include <cuda.h>
+
+#include <algorithm>
+
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 
 namespace sf {
+
+int make_byte_tensor_map(CUtensorMap* map, const void* ptr, int64_t pitch, int64_t outer, int box_outer);
 
 constexpr int kQThreads = 256;
 
@@ -52,6 +59,7 @@ __global__ void __launch_bounds__(kQThreads)
 int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int cols,
                      int pitch) {
     __shared__ uint32_t part[kQThreads / 32];
+    ptx::launch_dependents();
     const T* row = x + (int64_t)blockIdx.x * ld;
     uint32_t top = 0;  // bit pattern of the largest magnitude: a NaN is above infinity
     for (int k = threadIdx.x; k < cols; k += kQThreads) top = max(top, __float_as_uint(as_f32(row[k])) & 0x7fffffffu);
@@ -69,43 +77,415 @@ int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q
         out[k] = (int8_t)(k < cols && finite && top != 0 ? quantise(T(), as_f32(row[k]), rs) : 0);
 }
 
-// One place for the arithmetic behind the sum, so that every kernel rounds alike.
-__device__ __forceinline__ float int8_scaled(int acc, float xs, float ws) { return __int2float_rn(acc) * xs * ws; }
+// One place for the arithmetic behind the sum, so that every kernel rounds alike (bias 0 where there is none).
+__device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bias) {
+    return __fmaf_rn(__fmul_rn(__int2float_rn(acc), xs), ws, bias);
+}
 
-constexpr int kSimpleTile = 32;
-template <typename T>
-__global__ void __launch_bounds__(256)
-int8_gemm_simple_kernel(const int8_t* __restrict__ xq, const float* __restrict__ xs, const int8_t* __restrict__ wq,
-                        const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y, int rows, int pitch,
-                        int out) {
-    __shared__ int a[kSimpleTile][5], b[kSimpleTile][5];
-    const int t0 = blockIdx.y * kSimpleTile, n0 = blockIdx.x * kSimpleTile;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    int acc[4] = {0, 0, 0, 0};
-    for (int k = 0; k < pitch; k += 16) {
-        if (threadIdx.x < 128) {
-            const int r = threadIdx.x >> 2, w = threadIdx.x & 3;
-            a[r][w] = t0 + r < rows ? *reinterpret_cast<const int*>(xq + (int64_t)(t0 + r) * pitch + k + 4 * w) : 0;
-        } else {
-            const int r = (threadIdx.x - 128) >> 2, w = threadIdx.x & 3;
-            b[r][w] = n0 + r < out ? *reinterpret_cast<const int*>(wq + (int64_t)(n0 + r) * pitch + k + 4 * w) : 0;
+// ---------------------------------------------------------------------------------------------------------
+// Many rows: persistent CTA pairs, 256 x 256 tiles, tcgen05.mma.cta_group::2.kind::i8.
+//
+// A = xq (rows x K), B = wq (out x K), both K-contiguous: the bytes of a stage are those of the bf16 pair
+// kernel (128 bytes of K = 128 integers instead of 64 bf16; 16 KiB of A and 16 KiB of B per CTA, six stages), an
+// instruction covers 32 of K at the bf16 instruction's cycle count. Two accumulators of 256 columns fill the tensor memory:
+// the epilogue (integer -> float, two scales, bias, store) of a tile runs under the next tile's products.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int I8_BK = 128;                      // bytes = integers of K per stage: one 128-byte swizzled row
+constexpr int I8_THREADS = 192;
+constexpr int I8_STAGES = 6;
+constexpr int I8_OPERAND_BYTES = 128 * I8_BK;   // 16 KiB: this CTA's 128 rows of A, and its half of B's 256 rows
+constexpr int I8_STAGE_BYTES = 2 * I8_OPERAND_BYTES;
+constexpr int I8_EPI_BYTES = 2 * 256 * 4;       // per epilogue warp: scales and bias of the tile's columns
+constexpr int I8_PAIR_SMEM = I8_STAGES * I8_STAGE_BYTES + 4 * I8_EPI_BYTES + 1024 + 256;
+constexpr int I8_RASTER_M = 16;                 // tile rows per raster group: panels are shared in L2
+
+struct I8PairTail {
+    uint64_t full[I8_STAGES];
+    uint64_t empty[I8_STAGES];
+    uint64_t tmem_full[2];
+    uint64_t tmem_empty[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+__device__ __forceinline__ void i8_tile_coords(int tile, int tiles_m, int tiles_n, int& tm, int& tn) {
+    const int per_group = I8_RASTER_M * tiles_n;
+    const int g = tile / per_group, first = g * I8_RASTER_M;
+    const int gm = min(I8_RASTER_M, tiles_m - first), r = tile - g * per_group;
+    tm = first + r % gm;
+    tn = r / gm;
+}
+
+// Stores 32 consecutive columns of one row. vec: the row starts on a 16-byte boundary and all 32 columns exist.
+__device__ __forceinline__ void store_cols32(__nv_bfloat16* dst, const float (&v)[32], int valid, bool vec) {
+    if (vec && valid >= 32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+                w[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+            *reinterpret_cast<uint4*>(dst + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        __syncthreads();
+    } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) acc[i] = __dp4a(a[ty * 4 + i][w], b[tx][w], acc[i]);
-        __syncthreads();
+        for (int j = 0; j < 32; ++j)
+            if (j < valid) dst[j] = __float2bfloat16_rn(v[j]);
     }
-    const int n = n0 + tx;
+}
+__device__ __forceinline__ void store_cols32(float* dst, const float (&v)[32], int valid, bool vec) {
+    if (vec && valid >= 32) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t = t0 + ty * 4 + i;
-        if (t < rows && n < out) {
-            float v = int8_scaled(acc[i], xs[t], ws[n]);
-            if (bias) v += as_f32(bias[n]);
-            y[(int64_t)t * out + n] = (T)v;
+        for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<float4*>(dst + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (j < valid) dst[j] = v[j];
+    }
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
+int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                 const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
+                 int rows, int out, int pitch, int32_t* status) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+    const uint32_t base = (raw_addr + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - raw_addr);
+    float* epi = reinterpret_cast<float*>(base_ptr + I8_STAGES * I8_STAGE_BYTES);
+    I8PairTail* tail = reinterpret_cast<I8PairTail*>(base_ptr + I8_STAGES * I8_STAGE_BYTES + 4 * I8_EPI_BYTES);
+    volatile int* abort_flag = &tail->abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t cta = ptx::cluster_ctarank();
+    const int pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+    const int tiles_m = (rows + 255) / 256, tiles_n = (out + 255) / 256;
+    const int total_tiles = tiles_m * tiles_n;
+    const int num_kb = (pitch + I8_BK - 1) / I8_BK;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < I8_STAGES; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), 1);
         }
+        for (int a = 0; a < 2; ++a) {
+            ptx::mbar_init(ptx::smem_u32(&tail->tmem_full[a]), 1);
+            ptx::mbar_init(ptx::smem_u32(&tail->tmem_empty[a]), 8);
+        }
+        tail->abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(&tail->tmem_base), 512);
+        ptx::tmem_relinquish_pair();
+    }
+    if (warp == 0 && lane == 0) {
+        ptx::prefetch_tensormap(&tmA);
+        ptx::prefetch_tensormap(&tmB);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync_all();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tail->tmem_base;
+    ptx::dependency_wait();  // the quantised rows are complete from here on
+
+    if (warp == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int tile = pair; tile < total_tiles && ok; tile += num_pairs) {
+            int tm, tn;
+            i8_tile_coords(tile, tiles_m, tiles_n, tm, tn);
+            const int m0 = tm * 256 + (int)cta * 128, n0 = tn * 256 + (int)cta * 128;
+            for (int kb = 0; kb < num_kb; ++kb) {
+                ok = ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), phase ^ 1u, abort_flag, status, 41);
+                if (!ok) break;
+                if (lane == 0) {
+                    const uint32_t local_bar = ptx::smem_u32(&tail->full[stage]);
+                    const uint32_t bar = ptx::map_to_cta(local_bar, 0);
+                    const uint32_t sa = base + stage * I8_STAGE_BYTES, sb = sa + I8_OPERAND_BYTES;
+                    if (cta == 0) ptx::mbar_arrive_expect_tx(local_bar, 2 * I8_STAGE_BYTES);
+                    ptx::tma_load_2d_pair(sa, &tmA, bar, kb * I8_BK, m0);
+                    ptx::tma_load_2d_pair(sb, &tmB, bar, kb * I8_BK, n0);
+                }
+                __syncwarp();
+                if (++stage == I8_STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+        if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else if (warp == 1) {
+        if (cta == 0) {
+            constexpr uint32_t idesc = ptx::make_idesc_i8(256, 256);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            int t = 0;
+            for (int tile = pair; tile < total_tiles && ok; tile += num_pairs, ++t) {
+                const int acc = t & 1;
+                ok = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_empty[acc]), ((uint32_t)(t >> 1) & 1u) ^ 1u, abort_flag, status, 43);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                const uint32_t tmem_d = tmem_base + (uint32_t)(acc * 256);
+                for (int kb = 0; kb < num_kb; ++kb) {
+                    ok = ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), phase, abort_flag, status, 42);
+                    if (!ok) break;
+                    ptx::tc_fence_after();
+                    if (lane == 0) {
+                        const uint32_t sa = base + stage * I8_STAGE_BYTES, sb = sa + I8_OPERAND_BYTES;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)  // 32 integers = 32 bytes inside the 128-byte swizzled row
+                            ptx::mma_i8_ss_pair(tmem_d, ptx::make_smem_desc(sa + k * 32, 16, 1024, 2),
+                                                ptx::make_smem_desc(sb + k * 32, 16, 1024, 2), idesc, (kb | k) != 0 ? 1u : 0u);
+                        ptx::mma_commit_pair(ptx::smem_u32(&tail->empty[stage]), (uint16_t)3);
+                    }
+                    __syncwarp();
+                    if (++stage == I8_STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                if (lane == 0) ptx::mma_commit_pair(ptx::smem_u32(&tail->tmem_full[acc]), (uint16_t)3);
+                __syncwarp();
+            }
+        }
+    } else {
+        const int q = warp & 3;
+        const uint32_t leader_empty0 = ptx::map_to_cta(ptx::smem_u32(&tail->tmem_empty[0]), 0);
+        const uint32_t leader_empty1 = ptx::map_to_cta(ptx::smem_u32(&tail->tmem_empty[1]), 0);
+        float* cs = epi + (warp - 2) * 512;  // scales of the tile's 256 columns, then their bias
+        const bool vec = ((int64_t)out * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
+        bool ok = true;
+        int t = 0;
+        for (int tile = pair; tile < total_tiles && ok; tile += num_pairs, ++t) {
+            int tm, tn;
+            i8_tile_coords(tile, tiles_m, tiles_n, tm, tn);
+            const int row = tm * 256 + (int)cta * 128 + q * 32 + lane, n0 = tn * 256;
+            const float rs = row < rows ? xs[row] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int n = n0 + i * 32 + lane;
+                cs[i * 32 + lane] = n < out ? ws[n] : 0.0f;
+                cs[256 + i * 32 + lane] = bias != nullptr && n < out ? as_f32(bias[n]) : 0.0f;
+            }
+            __syncwarp();
+            const int acc = t & 1;
+            ok = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full[acc]), (uint32_t)(t >> 1) & 1u, abort_flag, status, 44);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            T* drow = y + (int64_t)row * out + n0;
+            const uint32_t taddr = tmem_base + (uint32_t)(acc * 256) + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t r[32];
+                ptx::tmem_ld_32x32b_x32(taddr + (uint32_t)(c * 32), r);
+                ptx::tmem_ld_wait();
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = int8_out((int)r[j], rs, cs[c * 32 + j], cs[256 + c * 32 + j]);
+                if (row < rows) store_cols32(drow + c * 32, v, out - n0 - c * 32, vec);
+            }
+            ptx::tc_fence_before();
+            __syncwarp();  // also: the column scales may be overwritten
+            if (lane == 0) ptx::mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+        }
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::cluster_sync_all();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------
+// Few rows: D[128 output channels, BN tokens] = wq . xq^T, the reduction cut over the CTAs of a cluster.
+//
+// The weight is what has to be read, so it is the 128-row operand and the tokens are the narrow one. A tile's K range
+// is cut over S CTAs (a cluster of S) so that about all SMs stream weights; each CTA leaves its partial sums (exact
+// integers) in its shared memory, and after a cluster barrier every CTA adds up BN / S of the token columns over all
+// S and writes them: one launch, no workspace, any order of arrival gives the same sum.
+// The weight loads of the first stages are issued before the kernel waits for the quantised rows.
+// ---------------------------------------------------------------------------------------------------------
+template <int BN>
+struct I8Few {
+    static constexpr int STAGES = BN >= 128 ? 6 : (BN >= 64 ? 4 : 5);  // two CTAs per SM up to 64 tokens
+    static constexpr int X_BYTES = BN * I8_BK;
+    static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_BYTES;
+    static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+    static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "partial sums reuse the ring");
+};
+constexpr int I8_MAX_SPLIT = 8;
+
+template <int STAGES>
+struct I8FewTail {
+    uint64_t full[STAGES];
+    uint64_t empty[STAGES];
+    uint64_t tmem_full;
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(I8_THREADS, BN >= 128 ? 1 : 2)
+int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+                const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
+                int rows, int out, int pitch, int split, int tiles_t, int32_t* status) {
+    using C = I8Few<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = ptx::smem_u32(smem_raw);
+    const uint32_t base = (raw_addr + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - raw_addr);
+    auto* tail = reinterpret_cast<I8FewTail<C::STAGES>*>(base_ptr + C::STAGES * C::STAGE_BYTES);
+    volatile int* abort_flag = &tail->abort_flag;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = split > 1 ? (int)ptx::cluster_ctarank() : 0;
+    const int tile = blockIdx.x / split;
+    const int n0 = tile / tiles_t * 128, t0 = tile % tiles_t * BN;
+    const int num_kb = (pitch + I8_BK - 1) / I8_BK;
+    const int kb0 = (int)((int64_t)num_kb * rank / split), kb1 = (int)((int64_t)num_kb * (rank + 1) / split);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < C::STAGES; ++s) {
+            ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
+            ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), 1);
+        }
+        ptx::mbar_init(ptx::smem_u32(&tail->tmem_full), 1);
+        tail->abort_flag = 0;
+        ptx::fence_barrier_init();
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(ptx::smem_u32(&tail->tmem_base), C::TMEM_COLS);
+        ptx::tmem_relinquish();
+    }
+    if (warp == 0 && lane == 0) {
+        ptx::prefetch_tensormap(&tmW);
+        ptx::prefetch_tensormap(&tmX);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem_base = tail->tmem_base;
+
+    if (warp == 0) {
+        const int ahead = min(C::STAGES, kb1 - kb0);
+        if (lane == 0)
+            for (int s = 0; s < ahead; ++s) {
+                const uint32_t bar = ptx::smem_u32(&tail->full[s]);
+                ptx::mbar_arrive_expect_tx(bar, C::STAGE_BYTES);
+                ptx::tma_load_2d(base + s * C::STAGE_BYTES, &tmW, bar, (kb0 + s) * I8_BK, n0);
+            }
+        ptx::dependency_wait();
+        if (lane == 0)
+            for (int s = 0; s < ahead; ++s)
+                ptx::tma_load_2d(base + s * C::STAGE_BYTES + I8_OPERAND_BYTES, &tmX, ptx::smem_u32(&tail->full[s]),
+                                 (kb0 + s) * I8_BK, t0);
+        __syncwarp();
+        int stage = 0;
+        uint32_t phase = 0;  // the first round of the ring is under way: wait for its release
+        bool ok = true;
+        for (int kb = kb0 + ahead; kb < kb1; ++kb) {
+            ok = ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), phase, abort_flag, status, 51);
+            if (!ok) break;
+            if (lane == 0) {
+                const uint32_t bar = ptx::smem_u32(&tail->full[stage]);
+                const uint32_t sw = base + stage * C::STAGE_BYTES;
+                ptx::mbar_arrive_expect_tx(bar, C::STAGE_BYTES);
+                ptx::tma_load_2d(sw, &tmW, bar, kb * I8_BK, n0);
+                ptx::tma_load_2d(sw + I8_OPERAND_BYTES, &tmX, bar, kb * I8_BK, t0);
+            }
+            __syncwarp();
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = ptx::make_idesc_i8(128, BN);
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; ++kb) {
+            ok = ptx::mbar_wait(ptx::smem_u32(&tail->full[stage]), phase, abort_flag, status, 52);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            if (lane == 0) {
+                const uint32_t sw = base + stage * C::STAGE_BYTES, sx = sw + I8_OPERAND_BYTES;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    ptx::mma_i8_ss(tmem_base, ptx::make_smem_desc(sw + k * 32, 16, 1024, 2),
+                                   ptx::make_smem_desc(sx + k * 32, 16, 1024, 2), idesc, (kb != kb0 || k != 0) ? 1u : 0u);
+                ptx::mma_commit(ptx::smem_u32(&tail->empty[stage]));
+            }
+            __syncwarp();
+            if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
+        }
+        if (ok && lane == 0) ptx::mma_commit(ptx::smem_u32(&tail->tmem_full));
+        __syncwarp();
+    }
+    // everything the MMAs read has been read once the accumulator is complete: the ring is free for partial sums
+    int* part = reinterpret_cast<int*>(base_ptr);
+    const int q = warp & 3;
+    const int n = n0 + q * 32 + lane;
+    bool done = false;
+    float cs = 0.0f, cb = 0.0f;
+    if (warp >= 2) {
+        ptx::dependency_wait();
+        if (n < out) {
+            cs = ws[n];
+            if (bias != nullptr) cb = as_f32(bias[n]);
+        }
+        done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
+        if (done) {
+            ptx::tc_fence_after();
+            const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+#pragma unroll 1
+            for (int c = 0; c < BN; c += 16) {
+                uint32_t r[16];
+                ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)c, r);
+                ptx::tmem_ld_wait();
+                if (split == 1) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int t = t0 + c + j;
+                        if (t < rows && n < out) y[(int64_t)t * out + n] = (T)int8_out((int)r[j], xs[t], cs, cb);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) part[(c + j) * 128 + q * 32 + lane] = (int)r[j];
+                }
+            }
+        }
+    }
+    ptx::tc_fence_before();
+    if (split > 1) {
+        __syncwarp();
+        ptx::cluster_sync_all();
+        if (done) {
+            const uint32_t mine = ptx::smem_u32(part) + (uint32_t)(q * 32 + lane) * 4u;
+            uint32_t peer[I8_MAX_SPLIT];
+#pragma unroll
+            for (int s = 0; s < I8_MAX_SPLIT; ++s) peer[s] = ptx::map_to_cta(mine, (uint32_t)(s < split ? s : 0));
+            const int last = min(BN, rows - t0);
+            for (int c = rank; c < last; c += split) {
+                int sum = 0;
+#pragma unroll
+                for (int s = 0; s < I8_MAX_SPLIT; ++s)
+                    if (s < split) sum += ptx::ld_shared_cluster_s32(peer[s] + (uint32_t)c * 512u);
+                if (n < out) y[(int64_t)(t0 + c) * out + n] = (T)int8_out(sum, xs[t0 + c], cs, cb);
+            }
+        }
+        __syncwarp();
+        ptx::cluster_sync_all();  // the partial sums of this CTA are read no more
+    }
+    __syncthreads();
+    if (warp == 1) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
 }
 
@@ -129,18 +509,97 @@ static int quantize_impl(const void* x, int dtype, int64_t ld, int8_t* q, float*
     return SF_OK;
 }
 
-static int gemm_impl(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y, int dtype,
-                     int64_t rows, int64_t in, int64_t out, int32_t* status, cudaStream_t st) {
-    const int pitch = (int)((in + 15) / 16 * 16);
-    dim3 grid((unsigned)((out + kSimpleTile - 1) / kSimpleTile), (unsigned)((rows + kSimpleTile - 1) / kSimpleTile));
-    (void)status;
-    if (grid.y > 65535) return fail(SF_ERR_UNSUPPORTED, "int8 product: too many rows");
-    if (dtype == SF_F32)
-        int8_gemm_simple_kernel<float><<<grid, 256, 0, st>>>(xq, xs, wq, ws, (const float*)bias, (float*)y, (int)rows, pitch, (int)out);
-    else
-        int8_gemm_simple_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(xq, xs, wq, ws, (const __nv_bfloat16*)bias, (__nv_bfloat16*)y, (int)rows, pitch, (int)out);
-    SF_CHECK_CUDA(cudaGetLastError());
+// dependent: the launch may be set up, and load weights, while the kernel before it in the stream still runs. Only behind
+// this file's quantiser, which is itself an ordinary launch: whatever wrote the weights before it is complete then.
+template <typename... KArgs, typename... Args>
+static cudaError_t launch_dependent(void (*kern)(KArgs...), int grid, int threads, int smem, int cluster, bool dependent,
+                                    cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (dependent) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)cluster;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    cfg.numAttrs = (unsigned)n;
+    cfg.attrs = attr;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+// Raises a kernel's dynamic shared memory limit once per device and thread.
+#define SF_I8_SMEM(kern, bytes)                                                                                     \
+    do {                                                                                                            \
+        static thread_local int configured_dev = -1;                                                                \
+        int dev = 0;                                                                                                \
+        SF_CHECK_CUDA(cudaGetDevice(&dev));                                                                         \
+        if (configured_dev != dev) {                                                                                \
+            SF_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));          \
+            configured_dev = dev;                                                                                   \
+        }                                                                                                           \
+    } while (0)
+
+template <typename T>
+static int launch_pair(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
+                       int64_t rows, int pitch, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
+    CUtensorMap tmA, tmB;
+    if (int rc = make_byte_tensor_map(&tmA, xq, pitch, rows, 128)) return rc;
+    if (int rc = make_byte_tensor_map(&tmB, wq, pitch, out, 128)) return rc;
+    const int64_t tiles = ((rows + 255) / 256) * ((out + 255) / 256);
+    if (tiles > 0x3fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: more than 2^30 tiles");
+    const int pairs = (int)std::min<int64_t>(tiles, sm_count() / 2);
+    auto kern = int8_pair_kernel<T>;
+    SF_I8_SMEM(kern, I8_PAIR_SMEM);
+    // the kernel's own cluster attribute (two CTAs) holds
+    SF_CHECK_CUDA(launch_dependent(kern, 2 * pairs, I8_THREADS, I8_PAIR_SMEM, 0, dependent, st, tmA, tmB, xs, ws, (const T*)bias, (T*)y,
+                                   (int)rows, (int)out, pitch, status));
     return SF_OK;
+}
+
+template <typename T, int BN>
+static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
+                      int64_t rows, int pitch, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
+    CUtensorMap tmW, tmX;
+    if (int rc = make_byte_tensor_map(&tmW, wq, pitch, out, 128)) return rc;
+    if (int rc = make_byte_tensor_map(&tmX, xq, pitch, rows, BN)) return rc;
+    const int64_t tiles_t = (rows + BN - 1) / BN, tiles = (out + 127) / 128 * tiles_t;
+    if (tiles * I8_MAX_SPLIT > 0x7fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: too many tiles");
+    // doubled until most SMs stream weights, as long as every CTA keeps a block of K
+    const int num_kb = (pitch + I8_BK - 1) / I8_BK;
+    int split = 1;
+    while (split < I8_MAX_SPLIT && tiles * split * 4 < (int64_t)sm_count() * 3 && 2 * split <= num_kb) split *= 2;
+    auto kern = int8_few_kernel<T, BN>;
+    SF_I8_SMEM(kern, I8Few<BN>::SMEM);
+    SF_CHECK_CUDA(launch_dependent(kern, (int)(tiles * split), I8_THREADS, I8Few<BN>::SMEM, split, dependent, st, tmW, tmX, xs, ws,
+                                   (const T*)bias, (T*)y, (int)rows, (int)out, pitch, split, (int)tiles_t, status));
+    return SF_OK;
+}
+
+template <typename T>
+static int gemm_typed(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
+                      int64_t rows, int64_t in, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
+    const int pitch = (int)((in + 15) / 16 * 16);
+    if (rows <= 16) return launch_few<T, 16>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    if (rows <= 32) return launch_few<T, 32>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    if (rows <= 64) return launch_few<T, 64>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    const int64_t pair_tiles = ((rows + 255) / 256) * ((out + 255) / 256);
+    if (pair_tiles * 2 < sm_count() / 2) return launch_few<T, 128>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    return launch_pair<T>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+}
+
+static int gemm_impl(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y, int dtype,
+                     int64_t rows, int64_t in, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
+    return dtype == SF_F32 ? gemm_typed<float>(xq, xs, wq, ws, bias, y, rows, in, out, status, dependent, st)
+                           : gemm_typed<__nv_bfloat16>(xq, xs, wq, ws, bias, y, rows, in, out, status, dependent, st);
 }
 
 }  // namespace sf
@@ -178,7 +637,7 @@ int sf_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq, const
     if (rows == 0) return SF_OK;
     SF_CHECK_ARG(xq && x_scale, "sf_int8_gemm: xq and x_scale must be non-null");
     if (!aligned16(xq)) return fail(SF_ERR_ALIGNMENT, "sf_int8_gemm: 8-bit operands must be 16-byte aligned");
-    return gemm_impl(xq, x_scale, wq, w_scale, bias, y, dtype, rows, in, out, status, (cudaStream_t)stream);
+    return gemm_impl(xq, x_scale, wq, w_scale, bias, y, dtype, rows, in, out, status, false, (cudaStream_t)stream);
 }
 
 int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in) {
@@ -195,7 +654,7 @@ int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_s
     int8_t* xq = static_cast<int8_t*>(workspace);
     float* xs = reinterpret_cast<float*>(xq + rows * sf_int8_pitch(in));
     if (int rc = quantize_impl(x, dtype, ld, xq, xs, rows, in, (cudaStream_t)stream)) return rc;
-    return gemm_impl(xq, xs, wq, w_scale, bias, y, dtype, rows, in, out, status, (cudaStream_t)stream);
+    return gemm_impl(xq, xs, wq, w_scale, bias, y, dtype, rows, in, out, status, true, (cudaStream_t)stream);
 }
 
 }  // extern "C"
