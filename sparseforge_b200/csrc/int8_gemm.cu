@@ -53,7 +53,110 @@ __device__ __forceinline__ int quantise(T tag, float x, const RowScale& r) {
 template <typename T>
 __device__ __forceinline__ float as_f32(T v) { return (float)v; }
 
-// One block per row. A row whose largest magnitude is infinite or NaN gets a NaN scale and zeros.
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float nan_f32() { return __uint_as_float(0x7fffffffu); }
+
+// Eight elements as they lie in memory (16 bytes of bf16, 32 of fp32).
+template <typename T>
+struct Raw8;
+template <>
+struct Raw8<__nv_bfloat16> {
+    uint4 v;
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void unpack(float (&x)[8]) const {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+};
+template <>
+struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float* p) {
+        a = __ldg(reinterpret_cast<const float4*>(p));
+        b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+    __device__ __forceinline__ void unpack(float (&x)[8]) const {
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    }
+};
+template <typename T>
+__device__ __forceinline__ uint32_t top8(const Raw8<T>& r, uint32_t top) {
+    float x[8];
+    r.unpack(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(x[i]));
+    return top;
+}
+
+// Eight integers, one per byte. Adding 3 * 2^22 rounds to an integer (half to even) and leaves it in the low byte; what the
+// rounding moved says whether any of the eight needs its quotient: about five instructions per element.
+template <typename T>
+__device__ __forceinline__ uint2 quantise8(const Raw8<T>& r, const RowScale& rs) {
+    constexpr float magic = 12582912.0f;
+    float x[8];
+    r.unpack(x);
+    uint32_t u[8];
+    float moved = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float t = __fmaf_rn(x[i], rs.inv, magic);
+        moved = fmaxf(moved, fabsf(__fmaf_rn(x[i], rs.inv, -(t - magic))));
+        u[i] = __float_as_uint(t);
+    }
+    if (rs.doubt || moved > 0.5f - 0x1p-12f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = (uint32_t)quotient(T(), x[i], rs.a);
+    }
+    const uint32_t lo0 = __byte_perm(u[0], u[1], 0x0040), lo1 = __byte_perm(u[2], u[3], 0x0040);
+    const uint32_t hi0 = __byte_perm(u[4], u[5], 0x0040), hi1 = __byte_perm(u[6], u[7], 0x0040);
+    return make_uint2(__byte_perm(lo0, lo1, 0x5410), __byte_perm(hi0, hi1, 0x5410));
+}
+
+// A row whose largest magnitude is infinite or NaN gets a NaN scale and zeros.
+// Rows on 16-byte boundaries, a multiple of 8 long: TPR threads hold a row in registers (NV groups of eight each)
+// between finding its largest magnitude and rounding it: one read, one write.
+template <typename T, int TPR, int NV>
+__global__ void __launch_bounds__(kQThreads)
+int8_quantize_vec_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
+                         int cols, int pitch) {
+    __shared__ uint32_t part[kQThreads / 32];
+    ptx::launch_dependents();
+    const int64_t row = (int64_t)blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
+    const int lane = threadIdx.x % TPR, nv = cols >> 3;
+    const bool live = row < rows;
+    const T* src = x + row * ld;
+    Raw8<T> r[NV];
+    uint32_t top = 0;  // bit pattern of the largest magnitude: a NaN is above infinity
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && lane + i * TPR < nv) r[i].load(src + 8 * (lane + i * TPR));
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (live && lane + i * TPR < nv) top = top8(r[i], top);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (TPR > 32) {
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) top = max(top, part[w]);
+    }
+    if (!live) return;
+    const bool usable = top < 0x7f800000u && top != 0;
+    const RowScale rs = row_scale(__uint_as_float(top));
+    if (lane == 0) scale[row] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
+    uint2* dst = reinterpret_cast<uint2*>(q + row * pitch);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (lane + i * TPR < nv) dst[lane + i * TPR] = usable ? quantise8(r[i], rs) : make_uint2(0u, 0u);
+    if (lane == 0 && (nv & 1)) dst[nv] = make_uint2(0u, 0u);
+}
+
+// Any other row: one block per row, read twice (the second time from a cache), element by element.
 template <typename T>
 __global__ void __launch_bounds__(kQThreads)
 int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int cols,
@@ -61,20 +164,21 @@ int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q
     __shared__ uint32_t part[kQThreads / 32];
     ptx::launch_dependents();
     const T* row = x + (int64_t)blockIdx.x * ld;
-    uint32_t top = 0;  // bit pattern of the largest magnitude: a NaN is above infinity
-    for (int k = threadIdx.x; k < cols; k += kQThreads) top = max(top, __float_as_uint(as_f32(row[k])) & 0x7fffffffu);
+    uint32_t top = 0;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < cols; k += kQThreads) top = max(top, magnitude_bits(as_f32(row[k])));
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kQThreads / 32; ++w) top = max(top, part[w]);
-    const bool finite = top < 0x7f800000u;
-    const float a = __uint_as_float(top);
-    const RowScale rs = row_scale(a);
-    if (threadIdx.x == 0) scale[blockIdx.x] = finite ? __fdiv_rn(a, 127.0f) : __uint_as_float(0x7fffffffu);
+    const bool usable = top < 0x7f800000u && top != 0;
+    const RowScale rs = row_scale(__uint_as_float(top));
+    if (threadIdx.x == 0) scale[blockIdx.x] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
     int8_t* out = q + (int64_t)blockIdx.x * pitch;
+#pragma unroll 4
     for (int k = threadIdx.x; k < pitch; k += kQThreads)
-        out[k] = (int8_t)(k < cols && finite && top != 0 ? quantise(T(), as_f32(row[k]), rs) : 0);
+        out[k] = (int8_t)(k < cols && usable ? quantise(T(), as_f32(row[k]), rs) : 0);
 }
 
 // One place for the arithmetic behind the sum, so that every kernel rounds alike (bias 0 where there is none).
@@ -303,6 +407,144 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------------------------------------
+// One to four rows: no tensor cores, one launch. Every warp streams whole weight rows through a ring of its own in
+// shared memory (untiled bulk copies, 2 KiB each, 160 KiB in flight per SM: an SM's share of a [4096, 4096] weight is 113 KiB, so
+// all of it is on its way before the first product). While the first copies travel, the block quantises the
+// tokens into shared memory: each block repeats that small work, which saves a launch and a wait.
+// A lane multiplies 16 bytes at a time (dp4a) and a row's sum is added up over the warp.
+// ---------------------------------------------------------------------------------------------------------
+constexpr int GV_WARPS = 8, GV_THREADS = 32 * GV_WARPS;
+constexpr int GV_CHUNK = 2048, GV_SLOTS = 10;
+constexpr int GV_X_BYTES = 48 * 1024;  // quantised tokens
+constexpr int GV_SMEM_FIXED = GV_WARPS * GV_SLOTS * GV_CHUNK + GV_WARPS * GV_SLOTS * 8;
+constexpr int GV_MAX_ROWS = 4;
+
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(GV_THREADS, 1)
+int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict__ wq, const float* __restrict__ ws,
+                   const T* __restrict__ bias, T* __restrict__ y, int in, int out, int pitch, int vec, int32_t* status) {
+    extern __shared__ __align__(128) uint8_t gv_smem[];
+    __shared__ uint32_t part[ROWS][GV_WARPS];
+    __shared__ int abort_shared;
+    volatile int* abort_flag = &abort_shared;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* ring = gv_smem + warp * (GV_SLOTS * GV_CHUNK);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(gv_smem + GV_WARPS * GV_SLOTS * GV_CHUNK) + warp * GV_SLOTS;
+    uint8_t* xq = gv_smem + GV_SMEM_FIXED;
+
+    // this warp's weight rows: first, first + step, ...; item = one chunk of one row
+    const int first = warp * gridDim.x + blockIdx.x, step = GV_WARPS * gridDim.x;
+    const int my_rows = first < out ? (out - 1 - first) / step + 1 : 0;
+    const int chunks = (pitch + GV_CHUNK - 1) / GV_CHUNK;
+    const int64_t items = (int64_t)my_rows * chunks;
+    if (threadIdx.x == 0) abort_shared = 0;
+    int load_row = first, load_chunk = 0;  // the next item to fetch (lane 0)
+    auto fetch = [&](int slot) {
+        const int at = load_chunk * GV_CHUNK;
+        const uint32_t bytes = (uint32_t)min(GV_CHUNK, pitch - at);
+        const uint32_t bar = ptx::smem_u32(&bars[slot]);
+        ptx::mbar_arrive_expect_tx(bar, bytes);
+        ptx::bulk_load(ptx::smem_u32(ring + slot * GV_CHUNK), wq + (int64_t)load_row * pitch + at, bytes, bar);
+        if (++load_chunk == chunks) { load_chunk = 0; load_row += step; }
+    };
+    if (lane == 0) {
+        for (int s = 0; s < GV_SLOTS; ++s) ptx::mbar_init(ptx::smem_u32(&bars[s]), 1);
+        ptx::fence_barrier_init();
+        for (int s = 0; s < GV_SLOTS && s < items; ++s) fetch(s);
+    }
+    __syncwarp();
+
+    // the tokens, quantised
+    uint32_t top[ROWS];
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) top[t] = 0;
+    const int nv = vec ? in >> 3 : 0;
+    for (int v = threadIdx.x; v < nv; v += GV_THREADS) {
+        Raw8<T> r[ROWS];
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) r[t].load(x + t * ld + 8 * v);
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) top[t] = top8(r[t], top[t]);
+    }
+    for (int k = 8 * nv + threadIdx.x; k < in; k += GV_THREADS)
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) top[t] = max(top[t], magnitude_bits(as_f32(x[t * ld + k])));
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+        top[t] = __reduce_max_sync(0xffffffffu, top[t]);
+        if (lane == 0) part[t][warp] = top[t];
+    }
+    __syncthreads();
+    RowScale rs[ROWS];
+    float xs[ROWS];
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) {
+#pragma unroll
+        for (int w = 0; w < GV_WARPS; ++w) top[t] = max(top[t], part[t][w]);
+        rs[t] = row_scale(__uint_as_float(top[t]));
+        xs[t] = top[t] < 0x7f800000u ? __fdiv_rn(rs[t].a, 127.0f) : nan_f32();
+    }
+    for (int v = threadIdx.x; v < nv; v += GV_THREADS) {
+        Raw8<T> r[ROWS];
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) r[t].load(x + t * ld + 8 * v);
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t)
+            *reinterpret_cast<uint2*>(xq + t * pitch + 8 * v) =
+                top[t] < 0x7f800000u && top[t] != 0 ? quantise8(r[t], rs[t]) : make_uint2(0u, 0u);
+    }
+    for (int k = 8 * nv + threadIdx.x; k < pitch; k += GV_THREADS)
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t)
+            xq[t * pitch + k] = (uint8_t)(k < in && top[t] < 0x7f800000u && top[t] != 0
+                                              ? quantise(T(), as_f32(x[t * ld + k]), rs[t]) : 0);
+    __syncthreads();
+
+    int slot = 0;
+    uint32_t phase = 0;
+    int64_t item = 0;
+    bool ok = true;
+    for (int i = 0; i < my_rows && ok; ++i) {
+        const int n = first + i * step;
+        int acc[ROWS];
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) acc[t] = 0;
+        for (int c = 0; c < chunks; ++c, ++item) {
+            ok = ptx::mbar_wait(ptx::smem_u32(&bars[slot]), phase, abort_flag, status, 61);
+            if (!ok) break;
+            const int at = c * GV_CHUNK, len = min(GV_CHUNK, pitch - at);
+            const uint8_t* wrow = ring + slot * GV_CHUNK;
+#pragma unroll
+            for (int j = 0; j < GV_CHUNK / 512; ++j) {
+                const int off = j * 512 + lane * 16;
+                if (off < len) {
+                    const int4 w = *reinterpret_cast<const int4*>(wrow + off);
+#pragma unroll
+                    for (int t = 0; t < ROWS; ++t) {
+                        const int4 v = *reinterpret_cast<const int4*>(xq + t * pitch + at + off);
+                        acc[t] = __dp4a(w.x, v.x, acc[t]);
+                        acc[t] = __dp4a(w.y, v.y, acc[t]);
+                        acc[t] = __dp4a(w.z, v.z, acc[t]);
+                        acc[t] = __dp4a(w.w, v.w, acc[t]);
+                    }
+                }
+            }
+            __syncwarp();  // the slot has been read by every lane
+            if (lane == 0 && item + GV_SLOTS < items) fetch(slot);
+            if (++slot == GV_SLOTS) { slot = 0; phase ^= 1u; }
+        }
+        if (!ok) break;
+        const float cs = ws[n], cb = bias != nullptr ? as_f32(bias[n]) : 0.0f;
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+            if (lane == t) y[(int64_t)t * out + n] = (T)int8_out(sum, xs[t], cs, cb);
+        }
+    }
+    if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies in flight land before shared memory is released
+}
+
+// ---------------------------------------------------------------------------------------------------------
 // Few rows: D[128 output channels, BN tokens] = wq . xq^T, the reduction cut over the CTAs of a cluster.
 //
 // The weight is what has to be read, so it is the 128-row operand and the tokens are the narrow one. A tile's K range
@@ -498,15 +740,35 @@ static int check_int8(const char* who, int64_t rows, int64_t in, int64_t out) {
     return SF_OK;
 }
 
-static int quantize_impl(const void* x, int dtype, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
-                         cudaStream_t st) {
+// Rows that start on 16-byte boundaries and are a multiple of 8 long move in 16-byte accesses.
+static bool rows_vectorise(const void* x, int dtype, int64_t ld, int64_t rows, int64_t cols) {
+    const int64_t esize = dtype == SF_F32 ? 4 : 2;
+    return aligned16(x) && cols % 8 == 0 && (rows == 1 || ld * esize % 16 == 0);
+}
+
+template <typename T>
+static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                          cudaStream_t st) {
     const int pitch = (int)((cols + 15) / 16 * 16);
-    if (dtype == SF_F32)
-        int8_quantize_kernel<float><<<(int)rows, kQThreads, 0, st>>>((const float*)x, ld, q, scale, (int)cols, pitch);
-    else
-        int8_quantize_kernel<__nv_bfloat16><<<(int)rows, kQThreads, 0, st>>>((const __nv_bfloat16*)x, ld, q, scale, (int)cols, pitch);
+    // a warp per row up to 1024 elements, a block per row up to 16384 (all of the row in registers)
+    if (vec && cols <= 1024) {
+        const int grid = (int)((rows + kQThreads / 32 - 1) / (kQThreads / 32));
+        int8_quantize_vec_kernel<T, 32, 4><<<grid, kQThreads, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);
+    } else if (vec && cols <= 4096) {
+        int8_quantize_vec_kernel<T, kQThreads, 2><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);
+    } else if (vec && cols <= 16384) {
+        int8_quantize_vec_kernel<T, kQThreads, 8><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);
+    } else {
+        int8_quantize_kernel<T><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)cols, pitch);
+    }
     SF_CHECK_CUDA(cudaGetLastError());
     return SF_OK;
+}
+static int quantize_impl(const void* x, int dtype, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                         cudaStream_t st) {
+    const bool vec = rows_vectorise(x, dtype, ld, rows, cols);
+    return dtype == SF_F32 ? quantize_typed((const float*)x, vec, ld, q, scale, rows, cols, st)
+                           : quantize_typed((const __nv_bfloat16*)x, vec, ld, q, scale, rows, cols, st);
 }
 
 // dependent: the launch may be set up, and load weights, while the kernel before it in the stream still runs. Only behind
@@ -584,6 +846,29 @@ static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const
     return SF_OK;
 }
 
+template <typename T, int ROWS>
+static int launch_stream(const void* x, int64_t ld, const int8_t* wq, const float* ws, const void* bias, void* y, int64_t in,
+                         int64_t out, bool vec, int32_t* status, cudaStream_t st) {
+    const int pitch = (int)((in + 15) / 16 * 16);
+    const int smem = GV_SMEM_FIXED + ROWS * pitch;
+    auto kern = int8_stream_kernel<T, ROWS>;
+    SF_I8_SMEM(kern, GV_SMEM_FIXED + GV_X_BYTES);
+    const int grid = (int)std::min<int64_t>(sm_count(), (out + GV_WARPS - 1) / GV_WARPS);
+    kern<<<grid, GV_THREADS, smem, st>>>((const T*)x, ld, wq, ws, (const T*)bias, (T*)y, (int)in, (int)out, pitch, vec ? 1 : 0, status);
+    SF_CHECK_CUDA(cudaGetLastError());
+    return SF_OK;
+}
+template <typename T>
+static int stream_typed(const void* x, int64_t ld, const int8_t* wq, const float* ws, const void* bias, void* y, int64_t rows,
+                        int64_t in, int64_t out, bool vec, int32_t* status, cudaStream_t st) {
+    switch (rows) {
+        case 1: return launch_stream<T, 1>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
+        case 2: return launch_stream<T, 2>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
+        case 3: return launch_stream<T, 3>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
+        default: return launch_stream<T, 4>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
+    }
+}
+
 template <typename T>
 static int gemm_typed(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
                       int64_t rows, int64_t in, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
@@ -651,6 +936,11 @@ int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_s
     SF_CHECK_ARG(x && workspace, "sf_int8_linear: x and workspace must be non-null");
     SF_CHECK_ARG(ld >= in || rows == 1, "sf_int8_linear: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(workspace)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: workspace must be 16-byte aligned");
+    if (rows <= GV_MAX_ROWS && rows * sf_int8_pitch(in) <= GV_X_BYTES) {
+        const bool vec = rows_vectorise(x, dtype, ld, rows, in);
+        return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, (cudaStream_t)stream)
+                               : stream_typed<__nv_bfloat16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, (cudaStream_t)stream);
+    }
     int8_t* xq = static_cast<int8_t*>(workspace);
     float* xs = reinterpret_cast<float*>(xq + rows * sf_int8_pitch(in));
     if (int rc = quantize_impl(x, dtype, ld, xq, xs, rows, in, (cudaStream_t)stream)) return rc;
