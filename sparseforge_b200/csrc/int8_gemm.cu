@@ -407,65 +407,52 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// One to four rows: no tensor cores, one launch. Every warp streams whole weight rows through a ring of its own in
-// shared memory (untiled bulk copies, 2 KiB each, 160 KiB in flight per SM: an SM's share of a [4096, 4096] weight is 113 KiB, so
-// all of it is on its way before the first product). While the first copies travel, the block quantises the
-// tokens into shared memory: each block repeats that small work, which saves a launch and a wait.
-// A lane multiplies 16 bytes at a time (dp4a) and a row's sum is added up over the warp.
+// One row or two: no tensor cores, one launch. A warp takes a whole weight row in pieces of 4 KiB, eight 16-byte loads
+// per lane straight into registers; 32 warps per SM keep 128 KiB in flight, as much as an SM's share of a [4096, 4096]
+// weight. The first piece is under way before the block quantises the tokens into shared memory: each block
+// repeats that small work, which saves a launch and a wait. A row's sum (dp4a) is added up over the warp.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int GV_WARPS = 8, GV_THREADS = 32 * GV_WARPS;
-constexpr int GV_CHUNK = 2048, GV_SLOTS = 10;
-constexpr int GV_X_BYTES = 48 * 1024;  // quantised tokens
-constexpr int GV_SMEM_FIXED = GV_WARPS * GV_SLOTS * GV_CHUNK + GV_WARPS * GV_SLOTS * 8;
-constexpr int GV_MAX_ROWS = 4;
+constexpr int GV_WARPS = 32, GV_THREADS = 32 * GV_WARPS;
+constexpr int GV_LOADS = 8, GV_PIECE = GV_LOADS * 512;
+constexpr int GV_X_BYTES = 128 * 1024;  // room for the quantised tokens
+constexpr int GV_MAX_ROWS = 2;
+
+__device__ __forceinline__ int4 ld_weights(const int8_t* p) {
+    int4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(GV_THREADS, 1)
 int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict__ wq, const float* __restrict__ ws,
-                   const T* __restrict__ bias, T* __restrict__ y, int in, int out, int pitch, int vec, int32_t* status) {
-    extern __shared__ __align__(128) uint8_t gv_smem[];
+                   const T* __restrict__ bias, T* __restrict__ y, int in, int out, int pitch, int vec) {
+    extern __shared__ __align__(16) uint8_t xq[];  // [ROWS][pitch]
     __shared__ uint32_t part[ROWS][GV_WARPS];
-    __shared__ int abort_shared;
-    volatile int* abort_flag = &abort_shared;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint8_t* ring = gv_smem + warp * (GV_SLOTS * GV_CHUNK);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(gv_smem + GV_WARPS * GV_SLOTS * GV_CHUNK) + warp * GV_SLOTS;
-    uint8_t* xq = gv_smem + GV_SMEM_FIXED;
-
-    // this warp's weight rows: first, first + step, ...; item = one chunk of one row
-    const int first = warp * gridDim.x + blockIdx.x, step = GV_WARPS * gridDim.x;
-    const int my_rows = first < out ? (out - 1 - first) / step + 1 : 0;
-    const int chunks = (pitch + GV_CHUNK - 1) / GV_CHUNK;
-    const int64_t items = (int64_t)my_rows * chunks;
-    if (threadIdx.x == 0) abort_shared = 0;
-    int load_row = first, load_chunk = 0;  // the next item to fetch (lane 0)
-    auto fetch = [&](int slot) {
-        const int at = load_chunk * GV_CHUNK;
-        const uint32_t bytes = (uint32_t)min(GV_CHUNK, pitch - at);
-        const uint32_t bar = ptx::smem_u32(&bars[slot]);
-        ptx::mbar_arrive_expect_tx(bar, bytes);
-        ptx::bulk_load(ptx::smem_u32(ring + slot * GV_CHUNK), wq + (int64_t)load_row * pitch + at, bytes, bar);
-        if (++load_chunk == chunks) { load_chunk = 0; load_row += step; }
+    const int step = GV_WARPS * gridDim.x;
+    int n = warp * gridDim.x + blockIdx.x, at = lane * 16;
+    int4 w[GV_LOADS];
+    auto fetch = [&]() {
+        const int8_t* src = wq + (int64_t)n * pitch + at;
+#pragma unroll
+        for (int j = 0; j < GV_LOADS; ++j) w[j] = n < out && at + j * 512 < pitch ? ld_weights(src + j * 512) : make_int4(0, 0, 0, 0);
     };
-    if (lane == 0) {
-        for (int s = 0; s < GV_SLOTS; ++s) ptx::mbar_init(ptx::smem_u32(&bars[s]), 1);
-        ptx::fence_barrier_init();
-        for (int s = 0; s < GV_SLOTS && s < items; ++s) fetch(s);
-    }
-    __syncwarp();
+    fetch();
 
     // the tokens, quantised
     uint32_t top[ROWS];
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) top[t] = 0;
     const int nv = vec ? in >> 3 : 0;
-    for (int v = threadIdx.x; v < nv; v += GV_THREADS) {
-        Raw8<T> r[ROWS];
+    for (int v = threadIdx.x; v < nv; v += GV_THREADS)
 #pragma unroll
-        for (int t = 0; t < ROWS; ++t) r[t].load(x + t * ld + 8 * v);
-#pragma unroll
-        for (int t = 0; t < ROWS; ++t) top[t] = top8(r[t], top[t]);
-    }
+        for (int t = 0; t < ROWS; ++t) {
+            Raw8<T> r;
+            r.load(x + t * ld + 8 * v);
+            top[t] = top8(r, top[t]);
+        }
     for (int k = 8 * nv + threadIdx.x; k < in; k += GV_THREADS)
 #pragma unroll
         for (int t = 0; t < ROWS; ++t) top[t] = max(top[t], magnitude_bits(as_f32(x[t * ld + k])));
@@ -475,73 +462,57 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
         if (lane == 0) part[t][warp] = top[t];
     }
     __syncthreads();
-    RowScale rs[ROWS];
     float xs[ROWS];
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {
-#pragma unroll
-        for (int w = 0; w < GV_WARPS; ++w) top[t] = max(top[t], part[t][w]);
-        rs[t] = row_scale(__uint_as_float(top[t]));
-        xs[t] = top[t] < 0x7f800000u ? __fdiv_rn(rs[t].a, 127.0f) : nan_f32();
+        top[t] = __reduce_max_sync(0xffffffffu, part[t][lane]);
+        const RowScale rs = row_scale(__uint_as_float(top[t]));
+        const bool usable = top[t] < 0x7f800000u && top[t] != 0;
+        xs[t] = top[t] < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
+        for (int v = threadIdx.x; v < nv; v += GV_THREADS) {
+            Raw8<T> r;
+            r.load(x + t * ld + 8 * v);
+            *reinterpret_cast<uint2*>(xq + t * pitch + 8 * v) = usable ? quantise8(r, rs) : make_uint2(0u, 0u);
+        }
+        for (int k = 8 * nv + threadIdx.x; k < pitch; k += GV_THREADS)
+            xq[t * pitch + k] = (uint8_t)(k < in && usable ? quantise(T(), as_f32(x[t * ld + k]), rs) : 0);
     }
-    for (int v = threadIdx.x; v < nv; v += GV_THREADS) {
-        Raw8<T> r[ROWS];
-#pragma unroll
-        for (int t = 0; t < ROWS; ++t) r[t].load(x + t * ld + 8 * v);
-#pragma unroll
-        for (int t = 0; t < ROWS; ++t)
-            *reinterpret_cast<uint2*>(xq + t * pitch + 8 * v) =
-                top[t] < 0x7f800000u && top[t] != 0 ? quantise8(r[t], rs[t]) : make_uint2(0u, 0u);
-    }
-    for (int k = 8 * nv + threadIdx.x; k < pitch; k += GV_THREADS)
-#pragma unroll
-        for (int t = 0; t < ROWS; ++t)
-            xq[t * pitch + k] = (uint8_t)(k < in && top[t] < 0x7f800000u && top[t] != 0
-                                              ? quantise(T(), as_f32(x[t * ld + k]), rs[t]) : 0);
     __syncthreads();
 
-    int slot = 0;
-    uint32_t phase = 0;
-    int64_t item = 0;
-    bool ok = true;
-    for (int i = 0; i < my_rows && ok; ++i) {
-        const int n = first + i * step;
-        int acc[ROWS];
+    int acc[ROWS];
 #pragma unroll
-        for (int t = 0; t < ROWS; ++t) acc[t] = 0;
-        for (int c = 0; c < chunks; ++c, ++item) {
-            ok = ptx::mbar_wait(ptx::smem_u32(&bars[slot]), phase, abort_flag, status, 61);
-            if (!ok) break;
-            const int at = c * GV_CHUNK, len = min(GV_CHUNK, pitch - at);
-            const uint8_t* wrow = ring + slot * GV_CHUNK;
+    for (int t = 0; t < ROWS; ++t) acc[t] = 0;
+    while (n < out) {
 #pragma unroll
-            for (int j = 0; j < GV_CHUNK / 512; ++j) {
-                const int off = j * 512 + lane * 16;
-                if (off < len) {
-                    const int4 w = *reinterpret_cast<const int4*>(wrow + off);
+        for (int j = 0; j < GV_LOADS; ++j)
+            if (at + j * 512 < pitch) {
 #pragma unroll
-                    for (int t = 0; t < ROWS; ++t) {
-                        const int4 v = *reinterpret_cast<const int4*>(xq + t * pitch + at + off);
-                        acc[t] = __dp4a(w.x, v.x, acc[t]);
-                        acc[t] = __dp4a(w.y, v.y, acc[t]);
-                        acc[t] = __dp4a(w.z, v.z, acc[t]);
-                        acc[t] = __dp4a(w.w, v.w, acc[t]);
-                    }
+                for (int t = 0; t < ROWS; ++t) {
+                    const int4 v = *reinterpret_cast<const int4*>(xq + t * pitch + at + j * 512);
+                    acc[t] = __dp4a(w[j].x, v.x, acc[t]);
+                    acc[t] = __dp4a(w[j].y, v.y, acc[t]);
+                    acc[t] = __dp4a(w[j].z, v.z, acc[t]);
+                    acc[t] = __dp4a(w[j].w, v.w, acc[t]);
                 }
             }
-            __syncwarp();  // the slot has been read by every lane
-            if (lane == 0 && item + GV_SLOTS < items) fetch(slot);
-            if (++slot == GV_SLOTS) { slot = 0; phase ^= 1u; }
+        const int row = n;
+        at += GV_PIECE;
+        const bool whole = at - lane * 16 >= pitch;
+        if (whole) {
+            at = lane * 16;
+            n += step;
         }
-        if (!ok) break;
-        const float cs = ws[n], cb = bias != nullptr ? as_f32(bias[n]) : 0.0f;
+        fetch();
+        if (whole) {
+            const float cs = ws[row], cb = bias != nullptr ? as_f32(bias[row]) : 0.0f;
 #pragma unroll
-        for (int t = 0; t < ROWS; ++t) {
-            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
-            if (lane == t) y[(int64_t)t * out + n] = (T)int8_out(sum, xs[t], cs, cb);
+            for (int t = 0; t < ROWS; ++t) {
+                const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+                if (lane == t) y[(int64_t)t * out + row] = (T)int8_out(sum, xs[t], cs, cb);
+                acc[t] = 0;
+            }
         }
     }
-    if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);  // copies in flight land before shared memory is released
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -848,25 +819,21 @@ static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const
 
 template <typename T, int ROWS>
 static int launch_stream(const void* x, int64_t ld, const int8_t* wq, const float* ws, const void* bias, void* y, int64_t in,
-                         int64_t out, bool vec, int32_t* status, cudaStream_t st) {
+                         int64_t out, bool vec, cudaStream_t st) {
     const int pitch = (int)((in + 15) / 16 * 16);
-    const int smem = GV_SMEM_FIXED + ROWS * pitch;
+    const int smem = ROWS * pitch;
     auto kern = int8_stream_kernel<T, ROWS>;
-    SF_I8_SMEM(kern, GV_SMEM_FIXED + GV_X_BYTES);
+    SF_I8_SMEM(kern, GV_X_BYTES);
     const int grid = (int)std::min<int64_t>(sm_count(), (out + GV_WARPS - 1) / GV_WARPS);
-    kern<<<grid, GV_THREADS, smem, st>>>((const T*)x, ld, wq, ws, (const T*)bias, (T*)y, (int)in, (int)out, pitch, vec ? 1 : 0, status);
+    kern<<<grid, GV_THREADS, smem, st>>>((const T*)x, ld, wq, ws, (const T*)bias, (T*)y, (int)in, (int)out, pitch, vec ? 1 : 0);
     SF_CHECK_CUDA(cudaGetLastError());
     return SF_OK;
 }
 template <typename T>
 static int stream_typed(const void* x, int64_t ld, const int8_t* wq, const float* ws, const void* bias, void* y, int64_t rows,
-                        int64_t in, int64_t out, bool vec, int32_t* status, cudaStream_t st) {
-    switch (rows) {
-        case 1: return launch_stream<T, 1>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
-        case 2: return launch_stream<T, 2>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
-        case 3: return launch_stream<T, 3>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
-        default: return launch_stream<T, 4>(x, ld, wq, ws, bias, y, in, out, vec, status, st);
-    }
+                        int64_t in, int64_t out, bool vec, cudaStream_t st) {
+    return rows == 1 ? launch_stream<T, 1>(x, ld, wq, ws, bias, y, in, out, vec, st)
+                     : launch_stream<T, 2>(x, ld, wq, ws, bias, y, in, out, vec, st);
 }
 
 template <typename T>
@@ -938,8 +905,8 @@ int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_s
     if (!aligned16(workspace)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: workspace must be 16-byte aligned");
     if (rows <= GV_MAX_ROWS && rows * sf_int8_pitch(in) <= GV_X_BYTES) {
         const bool vec = rows_vectorise(x, dtype, ld, rows, in);
-        return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, (cudaStream_t)stream)
-                               : stream_typed<__nv_bfloat16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, (cudaStream_t)stream);
+        return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream)
+                               : stream_typed<__nv_bfloat16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream);
     }
     int8_t* xq = static_cast<int8_t*>(workspace);
     float* xs = reinterpret_cast<float*>(xq + rows * sf_int8_pitch(in));
