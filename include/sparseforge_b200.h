@@ -516,7 +516,8 @@ SF_API int sf_kl_div_bwd(const void* student, const void* teacher, int dtype, co
  *     [out, pitch] with zero padding beyond `in`, bias (or NULL) and y [rows, out] of `dtype`. The sum is an exact
  *     32-bit integer (in <= SF_INT8_MAX_IN), the rest fp32 with one rounding to y: a row's values do not depend on the other rows.
  *   sf_int8_linear: both, for x of y's dtype (rows of stride ld); workspace of sf_int8_linear_workspace_bytes
- *     bytes, 16-byte aligned, holds nothing between calls; calls that may run at the same time need one each.
+ *     bytes (may be 0: one or two rows need none), 16-byte aligned, holds nothing between calls; calls that may run at
+ *     the same time need one each.
  * Any rows >= 0, in and out >= 1. 8-bit operands are 16-byte aligned. status as in sf_masked_gemm_fwd.
  */
 #define SF_INT8_MAX_IN ((int64_t)131056)

@@ -18,23 +18,29 @@ namespace sf {
 int make_byte_tensor_map(CUtensorMap* map, const void* ptr, int64_t pitch, int64_t outer, int box_outer);
 
 constexpr int kQThreads = 256;
+constexpr int kQVecResident = 2048;  // threads per SM of the register-resident quantiser
 
-// The integer nearest to 127 x / a (ties to even) for |x| <= a, decided as if the quotient were exact: a
-// multiplication by the rounded 127 / a is within 2^-16 of it; where that leaves doubt (closer than 2^-12 to a half, or a row
-// so small that 127 / a overflows) the quotient itself is formed.
-//  bf16: 127 x has 15 significant bits, so it is exact in fp32; a quotient of such numbers that is not half-way between
-//        integers is at least 1 / (2^9 * 2^gap) away (gap: how many powers of two |x| is below a, the quotient
-//        being about 2^(7 - gap)), while the rounded fp32 quotient is within 2^(7 - gap - 24) of it.
-//  fp32: product and quotient in fp64 (31 and 53 bits, the same argument).
+// The integer nearest to 127 x / a (ties to even) for |x| <= a, decided as if the quotient were exact, from a
+// multiplication by an approximate 127 / a (relative error below 2^-22: the reciprocal's 2^-23, two roundings).
+//  bf16: with gap the number of powers of two that |x| is below a, the quotient is about 2^(7 - gap); 127 x and a being integers of
+//        15 and 8 bits times a power of two, a quotient that is not half-way between integers is at least 2^-(9 + gap) away
+//        from it, and the product is within 2^-(15 + gap): it decides all but ties. A tie needs 254 x / a odd: x = a / 2
+//        (63.5, to the even 64), since 127 divides no 8-bit significand but 254. So the factor is raised by 2^-21,
+//        more than its error, which sends ties away from zero; rows whose a has the significand 254 take quotients.
+//  fp32: where the product is closer than 2^-14 to a half the quotient is formed, in fp64 (31 and 53 bits, as above).
+// Where the reciprocal would leave the normal range every element of the row takes the quotient.
+constexpr float kClear = 0.5f - 0x1p-14f;  // a rounding that moved the value by no more leaves no doubt
 struct RowScale {
     float a, inv;
     bool doubt;  // every element takes the quotient
 };
+template <typename T>
 __device__ __forceinline__ RowScale row_scale(float a) {
+    constexpr bool bf16 = sizeof(T) == 2;
     RowScale r;
     r.a = a;
-    r.inv = __fdiv_rn(127.0f, a);
-    r.doubt = a < 0x1p-118f;
+    r.inv = (bf16 ? 127.0f * (1.0f + 0x1p-21f) : 127.0f) * fast_rcp(a);
+    r.doubt = a < 0x1p-118f || a > 0x1p118f || (bf16 && (__float_as_uint(a) & 0x007f0000u) == 0x007e0000u);
     return r;
 }
 __device__ __forceinline__ int quotient(__nv_bfloat16, float x, float a) {
@@ -46,7 +52,7 @@ __device__ __forceinline__ int quotient(float, float x, float a) { return __doub
 template <typename T>
 __device__ __forceinline__ int quantise(T tag, float x, const RowScale& r) {
     const float v = x * r.inv, n = rintf(v);
-    if (r.doubt || fabsf(v - n) > 0.5f - 0x1p-12f) return quotient(tag, x, r.a);
+    if (r.doubt || (sizeof(T) == 4 && fabsf(v - n) > kClear)) return quotient(tag, x, r.a);
     return __float2int_rn(n);
 }
 
@@ -84,20 +90,43 @@ struct Raw8<float> {
         x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
 };
-template <typename T>
-__device__ __forceinline__ uint32_t top8(const Raw8<T>& r, uint32_t top) {
+// The largest magnitude so far as a bit pattern, ordered like the values with a NaN above infinity. bf16: two patterns of
+// 16 bits side by side; top_bits() gives the fp32 pattern.
+__device__ __forceinline__ uint32_t top8(const Raw8<__nv_bfloat16>& r, uint32_t top) {
+    const uint32_t m = 0x7fff7fffu;
+    return __vmaxu2(__vmaxu2(__vmaxu2(r.v.x & m, r.v.y & m), __vmaxu2(r.v.z & m, r.v.w & m)), top);
+}
+__device__ __forceinline__ uint32_t top8(const Raw8<float>& r, uint32_t top) {
     float x[8];
     r.unpack(x);
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, magnitude_bits(x[i]));
     return top;
 }
+__device__ __forceinline__ uint32_t top_bits(__nv_bfloat16, uint32_t top) { return max(top << 16, top & 0xffff0000u); }
+__device__ __forceinline__ uint32_t top_bits(float, uint32_t top) { return top; }
 
-// Eight integers, one per byte. Adding 3 * 2^22 rounds to an integer (half to even) and leaves it in the low byte; what the
-// rounding moved says whether any of the eight needs its quotient: about five instructions per element.
+__device__ __forceinline__ uint2 pack8(const uint32_t (&u)[8]) {  // the low byte of each
+    const uint32_t a0 = __byte_perm(u[0], u[1], 0x0040), a1 = __byte_perm(u[2], u[3], 0x0040);
+    const uint32_t b0 = __byte_perm(u[4], u[5], 0x0040), b1 = __byte_perm(u[6], u[7], 0x0040);
+    return make_uint2(__byte_perm(a0, a1, 0x5410), __byte_perm(b0, b1, 0x5410));
+}
+template <typename T>
+__device__ __noinline__ uint2 quotient8(Raw8<T> r, float a) {
+    float x[8];
+    uint32_t u[8];
+    r.unpack(x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = (uint32_t)quotient(T(), x[i], a);
+    return pack8(u);
+}
+
+// Eight integers, one per byte. Adding 3 * 2^22 rounds to an integer and leaves it in the low byte: one multiply-add
+// per element. fp32: what the rounding moved says whether any of the eight is in doubt (three more).
 template <typename T>
 __device__ __forceinline__ uint2 quantise8(const Raw8<T>& r, const RowScale& rs) {
     constexpr float magic = 12582912.0f;
+    if (rs.doubt) return quotient8(r, rs.a);
     float x[8];
     r.unpack(x);
     uint32_t u[8];
@@ -105,55 +134,59 @@ __device__ __forceinline__ uint2 quantise8(const Raw8<T>& r, const RowScale& rs)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float t = __fmaf_rn(x[i], rs.inv, magic);
-        moved = fmaxf(moved, fabsf(__fmaf_rn(x[i], rs.inv, -(t - magic))));
+        if (sizeof(T) == 4) moved = fmaxf(moved, fabsf(__fmaf_rn(x[i], rs.inv, -(t - magic))));
         u[i] = __float_as_uint(t);
     }
-    if (rs.doubt || moved > 0.5f - 0x1p-12f) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = (uint32_t)quotient(T(), x[i], rs.a);
-    }
-    const uint32_t lo0 = __byte_perm(u[0], u[1], 0x0040), lo1 = __byte_perm(u[2], u[3], 0x0040);
-    const uint32_t hi0 = __byte_perm(u[4], u[5], 0x0040), hi1 = __byte_perm(u[6], u[7], 0x0040);
-    return make_uint2(__byte_perm(lo0, lo1, 0x5410), __byte_perm(hi0, hi1, 0x5410));
+    if (sizeof(T) == 4 && moved > kClear) return quotient8(r, rs.a);
+    return pack8(u);
 }
 
 // A row whose largest magnitude is infinite or NaN gets a NaN scale and zeros.
 // Rows on 16-byte boundaries, a multiple of 8 long: TPR threads hold a row in registers (NV groups of eight each)
-// between finding its largest magnitude and rounding it: one read, one write.
-template <typename T, int TPR, int NV>
-__global__ void __launch_bounds__(kQThreads)
+// between finding its largest magnitude and rounding it: one read, one write. Blocks stay and take row after row; the
+// loads of the next are issued before the present one is reduced, so that the memory system is never left idle.
+template <typename T, int THREADS, int TPR, int NV>
+__global__ void __launch_bounds__(THREADS)
 int8_quantize_vec_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
                          int cols, int pitch) {
-    __shared__ uint32_t part[kQThreads / 32];
+    __shared__ uint32_t part[2][THREADS / 32];
     ptx::launch_dependents();
-    const int64_t row = (int64_t)blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
+    constexpr int PER_BLOCK = THREADS / TPR;
     const int lane = threadIdx.x % TPR, nv = cols >> 3;
-    const bool live = row < rows;
-    const T* src = x + row * ld;
-    Raw8<T> r[NV];
-    uint32_t top = 0;  // bit pattern of the largest magnitude: a NaN is above infinity
+    int row = blockIdx.x * PER_BLOCK + threadIdx.x / TPR;
+    const int step = gridDim.x * PER_BLOCK;
+    Raw8<T> next[NV];
+    auto fetch = [&](int from) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (live && lane + i * TPR < nv) r[i].load(src + 8 * (lane + i * TPR));
+        for (int i = 0; i < NV; ++i)
+            if (from < rows && lane + i * TPR < nv) next[i].load(x + from * ld + 8 * (lane + i * TPR));
+    };
+    fetch(row);
+    for (int turn = 0; row < rows; row += step, turn ^= 1) {  // all threads of a row, with TPR > 32 of the block, alike
+        Raw8<T> r[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (live && lane + i * TPR < nv) top = top8(r[i], top);
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (TPR > 32) {
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-        __syncthreads();
+        for (int i = 0; i < NV; ++i) r[i] = next[i];
+        if (row < rows - step) fetch(row + step);
+        uint32_t top = 0;  // bit pattern of the largest magnitude: a NaN is above infinity
 #pragma unroll
-        for (int w = 0; w < TPR / 32; ++w) top = max(top, part[w]);
+        for (int i = 0; i < NV; ++i)
+            if (lane + i * TPR < nv) top = top8(r[i], top);
+        top = __reduce_max_sync(0xffffffffu, top_bits(T(), top));
+        if (TPR > 32) {
+            if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = top;
+            __syncthreads();  // the other half of `part` is still being read by slower warps
+#pragma unroll
+            for (int w = 0; w < TPR / 32; ++w) top = max(top, part[turn][w]);
+        }
+        const bool usable = top < 0x7f800000u && top != 0;
+        const RowScale rs = row_scale<T>(__uint_as_float(top));
+        if (lane == 0) scale[row] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
+        uint2* dst = reinterpret_cast<uint2*>(q + (int64_t)row * pitch);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + i * TPR < nv) dst[lane + i * TPR] = usable ? quantise8(r[i], rs) : make_uint2(0u, 0u);
+        if (lane == 0 && (nv & 1)) dst[nv] = make_uint2(0u, 0u);
     }
-    if (!live) return;
-    const bool usable = top < 0x7f800000u && top != 0;
-    const RowScale rs = row_scale(__uint_as_float(top));
-    if (lane == 0) scale[row] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
-    uint2* dst = reinterpret_cast<uint2*>(q + row * pitch);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        if (lane + i * TPR < nv) dst[lane + i * TPR] = usable ? quantise8(r[i], rs) : make_uint2(0u, 0u);
-    if (lane == 0 && (nv & 1)) dst[nv] = make_uint2(0u, 0u);
 }
 
 // Any other row: one block per row, read twice (the second time from a cache), element by element.
@@ -173,7 +206,7 @@ int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q
 #pragma unroll
     for (int w = 0; w < kQThreads / 32; ++w) top = max(top, part[w]);
     const bool usable = top < 0x7f800000u && top != 0;
-    const RowScale rs = row_scale(__uint_as_float(top));
+    const RowScale rs = row_scale<T>(__uint_as_float(top));
     if (threadIdx.x == 0) scale[blockIdx.x] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
     int8_t* out = q + (int64_t)blockIdx.x * pitch;
 #pragma unroll 4
@@ -453,6 +486,8 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
             r.load(x + t * ld + 8 * v);
             top[t] = top8(r, top[t]);
         }
+#pragma unroll
+    for (int t = 0; t < ROWS; ++t) top[t] = top_bits(T(), top[t]);
     for (int k = 8 * nv + threadIdx.x; k < in; k += GV_THREADS)
 #pragma unroll
         for (int t = 0; t < ROWS; ++t) top[t] = max(top[t], magnitude_bits(as_f32(x[t * ld + k])));
@@ -466,7 +501,7 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
 #pragma unroll
     for (int t = 0; t < ROWS; ++t) {
         top[t] = __reduce_max_sync(0xffffffffu, part[t][lane]);
-        const RowScale rs = row_scale(__uint_as_float(top[t]));
+        const RowScale rs = row_scale<T>(__uint_as_float(top[t]));
         const bool usable = top[t] < 0x7f800000u && top[t] != 0;
         xs[t] = top[t] < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
         for (int v = threadIdx.x; v < nv; v += GV_THREADS) {
@@ -702,6 +737,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     }
 }
 
+// One row or two, whose quantised form fits into shared memory, take the kernel without a workspace.
+static bool takes_stream(int64_t rows, int64_t in) { return rows <= GV_MAX_ROWS && rows * ((in + 15) / 16 * 16) <= GV_X_BYTES; }
+
 static int check_int8(const char* who, int64_t rows, int64_t in, int64_t out) {
     if (rows < 0 || in <= 0 || out <= 0) return fail(SF_ERR_BAD_ARG, "%s: rows must not be negative, in and out positive", who);
     if (rows > 0x7fffff00 || out > 0x7fffff00) return fail(SF_ERR_UNSUPPORTED, "%s: dimension beyond 2^31", who);
@@ -721,14 +759,24 @@ template <typename T>
 static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
                           cudaStream_t st) {
     const int pitch = (int)((cols + 15) / 16 * 16);
-    // a warp per row up to 1024 elements, a block per row up to 16384 (all of the row in registers)
+    // A warp per row up to 1024 elements, a block per row up to 16384, all of the row in registers. [8192, 4096] bf16: 17.7 us
+    // (5.7 TB/s) with 128 threads per row, 18.9 with 256, 21.5 with 512; [8192, 11008]: 44.3 us (6.1 TB/s).
+#define SF_I8_QUANT(THREADS, TPR, NV)                                                                                 \
+    do {                                                                                                              \
+        auto kern = int8_quantize_vec_kernel<T, THREADS, TPR, NV>;                                                    \
+        const int64_t need = (rows + THREADS / TPR - 1) / (THREADS / TPR);                                            \
+        const int grid = (int)std::min<int64_t>(need, (int64_t)sm_count() * (kQVecResident / THREADS));               \
+        kern<<<grid, THREADS, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);                                 \
+    } while (0)
     if (vec && cols <= 1024) {
-        const int grid = (int)((rows + kQThreads / 32 - 1) / (kQThreads / 32));
-        int8_quantize_vec_kernel<T, 32, 4><<<grid, kQThreads, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);
+        SF_I8_QUANT(256, 32, 4);
     } else if (vec && cols <= 4096) {
-        int8_quantize_vec_kernel<T, kQThreads, 2><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);
+        SF_I8_QUANT(128, 128, 4);
+    } else if (vec && cols <= 12288) {
+        SF_I8_QUANT(256, 256, 6);
     } else if (vec && cols <= 16384) {
-        int8_quantize_vec_kernel<T, kQThreads, 8><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);
+        SF_I8_QUANT(512, 512, 4);
+#undef SF_I8_QUANT
     } else {
         int8_quantize_kernel<T><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)cols, pitch);
     }
@@ -893,17 +941,19 @@ int sf_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq, const
 }
 
 int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in) {
-    return rows <= 0 || in <= 0 ? 0 : rows * ((in + 15) / 16 * 16) + rows * 4;
+    if (rows <= 0 || in <= 0 || takes_stream(rows, in)) return 0;
+    return rows * sf_int8_pitch(in) + rows * 4;
 }
 
 int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_scale, const void* bias, void* y, int dtype,
                    int64_t rows, int64_t in, int64_t out, void* workspace, int32_t* status, void* stream) {
     if (int rc = check_product("sf_int8_linear", wq, w_scale, y, dtype, rows, in, out)) return rc;
     if (rows == 0) return SF_OK;
-    SF_CHECK_ARG(x && workspace, "sf_int8_linear: x and workspace must be non-null");
+    const bool stream_rows = takes_stream(rows, in);
+    SF_CHECK_ARG(x && (workspace || stream_rows), "sf_int8_linear: x and workspace must be non-null");
     SF_CHECK_ARG(ld >= in || rows == 1, "sf_int8_linear: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(workspace)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: workspace must be 16-byte aligned");
-    if (rows <= GV_MAX_ROWS && rows * sf_int8_pitch(in) <= GV_X_BYTES) {
+    if (stream_rows) {
         const bool vec = rows_vectorise(x, dtype, ld, rows, in);
         return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream)
                                : stream_typed<__nv_bfloat16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream);

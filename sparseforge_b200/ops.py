@@ -421,9 +421,13 @@ def kl_div_bwd(student2d, teacher2d, lse, row_scale, temperature=2.0, max_logit=
 # ----------------------------------------------------------------------------------------
 # global gradient norm and clipping
 # ----------------------------------------------------------------------------------------
+_HERE = nullcontext()
+
+
 def _on_device_of(t: torch.Tensor):
     """Context that makes ``t``'s device the current one (launches and ``_stream`` go there)."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else nullcontext()
+    index = t.get_device()
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 def _dense_view(t: torch.Tensor) -> torch.Tensor:
@@ -708,29 +712,29 @@ def _int8_rows(x2d, what):
     rows, cols = x2d.shape
     if cols == 0:
         raise ValueError(f"{what}: rows must hold at least one element")
-    if (cols > 1 and x2d.stride(1) != 1) or (rows > 1 and x2d.stride(0) < cols):
-        raise RuntimeError(f"{what}: rows must be contiguous and must not overlap (strides {tuple(x2d.stride())})")
-    return max(x2d.stride(0), cols)
+    ld, inner = x2d.stride()
+    if (cols > 1 and inner != 1) or (rows > 1 and ld < cols):
+        raise RuntimeError(f"{what}: rows must be contiguous and must not overlap (strides {x2d.stride()})")
+    return ld if ld > cols else cols
 
 
-def _int8_weight(wq, w_scale, k, dev, what):
-    """(out, ctypes-ready checks) of an 8-bit weight [out, k rounded up to 16] with its scales."""
-    _cuda(wq, w_scale)
+def _int8_weight(wq, w_scale, bias, k, dtype, dev, what):
+    """Output channels of an 8-bit weight [out, k rounded up to 16] after checking it, its scales and the bias."""
     if wq.dtype != torch.int8 or w_scale.dtype != torch.float32 or wq.dim() != 2 or w_scale.shape != wq.shape[:1]:
         raise TypeError(f"{what}: weight int8 [out, pitch] and float32 scales [out] expected")
-    if wq.shape[1] != (k + 15) // 16 * 16:
-        raise ValueError(f"{what}: x has {k} features, weight rows of {wq.shape[1]} bytes (expected {(k + 15) // 16 * 16})")
-    if wq.device != dev or w_scale.device != dev:
+    if not (wq.is_contiguous() and w_scale.is_contiguous()):
+        _cuda(wq, w_scale)
+    out, pitch = wq.shape
+    if pitch != (k + 15) // 16 * 16:
+        raise ValueError(f"{what}: x has {k} features, weight rows of {pitch} bytes (expected {(k + 15) // 16 * 16})")
+    if wq.get_device() != dev or w_scale.get_device() != dev:
+        _cuda(wq, w_scale)
         raise ValueError(f"{what}: all tensors of a call must live on one device")
-    return wq.shape[0]
-
-
-def _int8_bias(bias, out, dtype, dev, what):
-    if bias is None:
-        return
-    _cuda(bias)
-    if bias.dtype != dtype or bias.shape != (out,) or bias.device != dev:
-        raise TypeError(f"{what}: bias must be {dtype} [{out}] on {dev}")
+    if bias is not None and (bias.dtype != dtype or bias.shape != w_scale.shape or bias.get_device() != dev
+                             or not bias.is_contiguous()):
+        _cuda(bias)
+        raise TypeError(f"{what}: bias must be {dtype} [{out}] on the operands' device")
+    return out
 
 
 def int8_quantize_rows(x2d):
@@ -755,12 +759,10 @@ def int8_gemm(xq, x_scale, wq, w_scale, bias=None, out_dtype=torch.bfloat16, sta
     if out_dtype not in _GRAD_DTYPES:
         raise TypeError("int8_gemm: out_dtype must be float32 or bfloat16")
     T, k = xq.shape
-    dev = xq.device
-    if x_scale.device != dev:
+    if x_scale.device != xq.device:
         raise ValueError("int8_gemm: all tensors of a call must live on one device")
-    out = _int8_weight(wq, w_scale, k, dev, "int8_gemm")
-    _int8_bias(bias, out, out_dtype, dev, "int8_gemm")
-    y = torch.empty((T, out), dtype=out_dtype, device=dev)
+    out = _int8_weight(wq, w_scale, bias, k, out_dtype, xq.get_device(), "int8_gemm")
+    y = torch.empty((T, out), dtype=out_dtype, device=xq.device)
     with _on_device_of(xq):
         check(lib().sf_int8_gemm(_p(xq), _p(x_scale), _p(wq), _p(w_scale), _p(bias), _p(y), _DT[out_dtype], T, k, out,
                                  _p(status), _stream()), "sf_int8_gemm")
@@ -772,17 +774,20 @@ def int8_linear(x2d, wq, w_scale, bias=None, status=None):
     (``int8_quantize_rows``) and multiplied in 8 bits (``int8_gemm``)."""
     ld = _int8_rows(x2d, "int8_linear")
     T, k = x2d.shape
-    dev = x2d.device
-    out = _int8_weight(wq, w_scale, k, dev, "int8_linear")
-    _int8_bias(bias, out, x2d.dtype, dev, "int8_linear")
-    y = torch.empty((T, out), dtype=x2d.dtype, device=dev)
+    dtype, dev = x2d.dtype, x2d.device
+    out = _int8_weight(wq, w_scale, bias, k, dtype, dev.index, "int8_linear")
+    y = torch.empty((T, out), dtype=dtype, device=dev)
     if T == 0:
         return y
+    h = lib()
     # a workspace of its own per call: calls on two streams, or in two captured graphs, never share one
-    ws = torch.empty(int(lib().sf_int8_linear_workspace_bytes(T, k)), dtype=torch.uint8, device=dev)
+    nbytes = h.sf_int8_linear_workspace_bytes(T, k)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on_device_of(x2d):
-        check(lib().sf_int8_linear(_p(x2d), ld, _p(wq), _p(w_scale), _p(bias), _p(y), _dt(x2d), T, k, out, _p(ws),
-                                   _p(status), _stream()), "sf_int8_linear")
+        rc = h.sf_int8_linear(x2d.data_ptr(), ld, wq.data_ptr(), w_scale.data_ptr(), _p(bias), y.data_ptr(), _DT[dtype],
+                              T, k, out, _p(ws), _p(status), _stream())
+    if rc:
+        check(rc, "sf_int8_linear")
     return y
 
 

@@ -93,6 +93,35 @@ def test_quantised_rows_near_and_on_halves(dtype):
     assert torch.equal(q[:, :x.shape[1]].double(), want)
 
 
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("exponent", [0, -60, 100])
+def test_every_bf16_quotient(exponent, sign):
+    """All significands of a row's largest value against all of an element's, the element up to ten powers of two smaller: every
+    quotient a bf16 row can hold that is not zero, on and beside every half. Through the quantiser and the single-row layer."""
+    sig = torch.arange(128, 256, dtype=torch.float64, device="cuda")
+    gaps = 2.0 ** -torch.arange(0, 11, dtype=torch.float64, device="cuda")
+    x = (sig[None, :, None] * gaps).reshape(1, -1).expand(128, -1).clone()
+    x = torch.where(x <= sig[:, None], x, torch.zeros_like(x))
+    x = (torch.cat([sig[:, None], x], 1) * 2.0 ** (exponent - 8) * sign).bfloat16()
+    ops = _ops()
+    q, _ = ops.int8_quantize_rows(x)
+    want, _ = _quantise64(x)
+    assert torch.equal(q[:, :x.shape[1]].double(), want)
+    # odd row length: the element-wise kernel
+    q, _ = ops.int8_quantize_rows(x[:, :1001])
+    assert torch.equal(q[:, :1001].double(), want[:, :1001])
+    # weight = identity scaled by one: the layer returns the integers times the scale
+    k = x.shape[1]
+    eye = torch.eye(k, device="cuda", dtype=torch.int8)
+    eye = torch.nn.functional.pad(eye, (0, -k % 16)) if k % 16 else eye
+    one = torch.ones(k, device="cuda")
+    for r in (0, 1, 63, 126, 127):
+        y = ops.int8_linear(x[r:r + 1].float(), eye, one)
+        assert torch.equal(torch.round(y.double() / (float(sig[r]) * 2.0 ** (exponent - 8) / 127.0)), want[r:r + 1])
+        yb = ops.int8_linear(x[r:r + 1], eye, one)
+        assert torch.equal(yb, y.bfloat16())
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_quantised_rows_at_the_ends_of_the_range(dtype):
     top = torch.finfo(DT[dtype]).max
@@ -233,7 +262,7 @@ def test_rows_behind_the_last_are_left_alone(T):
     wq, ws = ops.int8_quantize_rows(w)
     want = ops.int8_linear(x, wq, ws)
     y = torch.full((T + 2, n), 5.0, device="cuda", dtype=torch.bfloat16)
-    work = torch.empty(int(_lib.lib().sf_int8_linear_workspace_bytes(T, k)), dtype=torch.uint8, device="cuda")
+    work = torch.empty(int(_lib.lib().sf_int8_linear_workspace_bytes(T, k)) or 16, dtype=torch.uint8, device="cuda")
     rc = _lib.lib().sf_int8_linear(x.data_ptr(), k, wq.data_ptr(), ws.data_ptr(), None, y[1:].data_ptr(), _lib.SF_BF16, T, k, n,
                                    work.data_ptr(), None, torch.cuda.current_stream().cuda_stream)
     assert rc == 0
