@@ -551,24 +551,26 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// Few rows: D[128 output channels, BN tokens] = wq . xq^T, the reduction cut over the CTAs of a cluster.
+// Few rows: D[128 PAIR output channels, BN tokens] = wq . xq^T, the reduction cut over the CTAs of a cluster.
 //
 // The weight is what has to be read, so it is the 128-row operand and the tokens are the narrow one. A tile's K range
-// is cut over S CTAs (a cluster of S) so that about all SMs stream weights; each CTA leaves its partial sums (exact
-// integers) in its shared memory, and after a cluster barrier every CTA adds up BN / S of the token columns over all
-// S and writes them: one launch, no workspace, any order of arrival gives the same sum.
+// is cut into `split` parts so that about all SMs stream weights; the parts' CTAs form a cluster, each leaves its partial
+// sums (exact integers) in its shared memory, and after a cluster barrier every CTA adds up its share of the token
+// columns over all parts and writes them: one launch, no workspace, any order of arrival gives the same sum.
+// PAIR = 2 (more than 64 tokens): two CTAs share a 256-row tile (cta_group::2), each loads half of the tokens, 24 KiB per
+// stage instead of 32 for the same products: above 64 tokens the traffic into the SMs is what bounds the tile.
 // The weight loads of the first stages are issued before the kernel waits for the quantised rows.
 // ---------------------------------------------------------------------------------------------------------
-template <int BN>
+template <int BN, int PAIR>
 struct I8Few {
-    static constexpr int STAGES = BN >= 128 ? 6 : (BN >= 64 ? 4 : 5);  // two CTAs per SM up to 64 tokens
-    static constexpr int X_BYTES = BN * I8_BK;
-    static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_BYTES;
+    static constexpr int STAGES = BN * PAIR <= 32 ? 5 : 4;  // 94 to 104 KB: two CTAs per SM
+    static constexpr int X_ROWS = BN / PAIR;
+    static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_ROWS * I8_BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
     static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+    static constexpr int MAX_SPLIT = 8 / PAIR;              // clusters of at most eight CTAs
     static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "partial sums reuse the ring");
 };
-constexpr int I8_MAX_SPLIT = 8;
 
 template <int STAGES>
 struct I8FewTail {
@@ -579,12 +581,33 @@ struct I8FewTail {
     int abort_flag;
 };
 
-template <typename T, int BN>
-__global__ void __launch_bounds__(I8_THREADS, BN >= 128 ? 1 : 2)
+// Four consecutive output channels of one token.
+__device__ __forceinline__ void store4(__nv_bfloat16* dst, const float (&v)[4], int valid, bool vec) {
+    if (vec && valid >= 4) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < valid) dst[i] = __float2bfloat16_rn(v[i]);
+    }
+}
+__device__ __forceinline__ void store4(float* dst, const float (&v)[4], int valid, bool vec) {
+    if (vec && valid >= 4) {
+        *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < valid) dst[i] = v[i];
+    }
+}
+
+template <typename T, int BN, int PAIR>
+__global__ void __launch_bounds__(I8_THREADS, 2)
 int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                 const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
                 int rows, int out, int pitch, int split, int tiles_t, int32_t* status) {
-    using C = I8Few<BN>;
+    using C = I8Few<BN, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = ptx::smem_u32(smem_raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -593,11 +616,14 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     volatile int* abort_flag = &tail->abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int rank = split > 1 ? (int)ptx::cluster_ctarank() : 0;
-    const int tile = blockIdx.x / split;
-    const int n0 = tile / tiles_t * 128, t0 = tile % tiles_t * BN;
+    const bool clustered = PAIR * split > 1;
+    const int crank = clustered ? (int)ptx::cluster_ctarank() : 0;
+    const int half = PAIR == 2 ? crank & 1 : 0, part_no = crank / PAIR;
+    const uint32_t leader = (uint32_t)(part_no * PAIR);
+    const int tile = blockIdx.x / (PAIR * split);
+    const int n0 = (tile / tiles_t * PAIR + half) * 128, t0 = tile % tiles_t * BN;
     const int num_kb = (pitch + I8_BK - 1) / I8_BK;
-    const int kb0 = (int)((int64_t)num_kb * rank / split), kb1 = (int)((int64_t)num_kb * (rank + 1) / split);
+    const int kb0 = (int)((int64_t)num_kb * part_no / split), kb1 = (int)((int64_t)num_kb * (part_no + 1) / split);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
@@ -609,8 +635,13 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         ptx::fence_barrier_init();
     }
     if (warp == 1) {
-        ptx::tmem_alloc(ptx::smem_u32(&tail->tmem_base), C::TMEM_COLS);
-        ptx::tmem_relinquish();
+        if (PAIR == 2) {
+            ptx::tmem_alloc_pair(ptx::smem_u32(&tail->tmem_base), C::TMEM_COLS);
+            ptx::tmem_relinquish_pair();
+        } else {
+            ptx::tmem_alloc(ptx::smem_u32(&tail->tmem_base), C::TMEM_COLS);
+            ptx::tmem_relinquish();
+        }
     }
     if (warp == 0 && lane == 0) {
         ptx::prefetch_tensormap(&tmW);
@@ -618,22 +649,35 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     }
     ptx::tc_fence_before();
     __syncthreads();
+    if (PAIR == 2) ptx::cluster_sync_all();  // the other CTA's copies and commits arrive on this CTA's barriers
     ptx::tc_fence_after();
     const uint32_t tmem_base = tail->tmem_base;
 
     if (warp == 0) {
+        auto load = [&](int stage, int kb, bool weights, bool tokens) {
+            const uint32_t local = ptx::smem_u32(&tail->full[stage]);
+            const uint32_t sw = base + stage * C::STAGE_BYTES, sx = sw + I8_OPERAND_BYTES;
+            if (PAIR == 2) {
+                const uint32_t bar = ptx::map_to_cta(local, leader);
+                if (weights) {
+                    if (half == 0) ptx::mbar_arrive_expect_tx(local, 2 * C::STAGE_BYTES);
+                    ptx::tma_load_2d_pair(sw, &tmW, bar, kb * I8_BK, n0);
+                }
+                if (tokens) ptx::tma_load_2d_pair(sx, &tmX, bar, kb * I8_BK, t0 + half * C::X_ROWS);
+            } else {
+                if (weights) {
+                    ptx::mbar_arrive_expect_tx(local, C::STAGE_BYTES);
+                    ptx::tma_load_2d(sw, &tmW, local, kb * I8_BK, n0);
+                }
+                if (tokens) ptx::tma_load_2d(sx, &tmX, local, kb * I8_BK, t0);
+            }
+        };
         const int ahead = min(C::STAGES, kb1 - kb0);
         if (lane == 0)
-            for (int s = 0; s < ahead; ++s) {
-                const uint32_t bar = ptx::smem_u32(&tail->full[s]);
-                ptx::mbar_arrive_expect_tx(bar, C::STAGE_BYTES);
-                ptx::tma_load_2d(base + s * C::STAGE_BYTES, &tmW, bar, (kb0 + s) * I8_BK, n0);
-            }
+            for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
         ptx::dependency_wait();
         if (lane == 0)
-            for (int s = 0; s < ahead; ++s)
-                ptx::tma_load_2d(base + s * C::STAGE_BYTES + I8_OPERAND_BYTES, &tmX, ptx::smem_u32(&tail->full[s]),
-                                 (kb0 + s) * I8_BK, t0);
+            for (int s = 0; s < ahead; ++s) load(s, kb0 + s, false, true);
         __syncwarp();
         int stage = 0;
         uint32_t phase = 0;  // the first round of the ring is under way: wait for its release
@@ -641,19 +685,14 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         for (int kb = kb0 + ahead; kb < kb1; ++kb) {
             ok = ptx::mbar_wait(ptx::smem_u32(&tail->empty[stage]), phase, abort_flag, status, 51);
             if (!ok) break;
-            if (lane == 0) {
-                const uint32_t bar = ptx::smem_u32(&tail->full[stage]);
-                const uint32_t sw = base + stage * C::STAGE_BYTES;
-                ptx::mbar_arrive_expect_tx(bar, C::STAGE_BYTES);
-                ptx::tma_load_2d(sw, &tmW, bar, kb * I8_BK, n0);
-                ptx::tma_load_2d(sw + I8_OPERAND_BYTES, &tmX, bar, kb * I8_BK, t0);
-            }
+            if (lane == 0) load(stage, kb, true, true);
             __syncwarp();
             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) for (int i = 0; i < 1000; ++i) __nanosleep(1000);
-    } else if (warp == 1) {
-        constexpr uint32_t idesc = ptx::make_idesc_i8(128, BN);
+    } else if (warp == 1 && half == 0) {
+        constexpr uint32_t idesc = ptx::make_idesc_i8(128 * PAIR, BN);
+        const uint16_t both = (uint16_t)(3u << leader);
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -664,48 +703,43 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             if (lane == 0) {
                 const uint32_t sw = base + stage * C::STAGE_BYTES, sx = sw + I8_OPERAND_BYTES;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    ptx::mma_i8_ss(tmem_base, ptx::make_smem_desc(sw + k * 32, 16, 1024, 2),
-                                   ptx::make_smem_desc(sx + k * 32, 16, 1024, 2), idesc, (kb != kb0 || k != 0) ? 1u : 0u);
-                ptx::mma_commit(ptx::smem_u32(&tail->empty[stage]));
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t wd = ptx::make_smem_desc(sw + k * 32, 16, 1024, 2), xd = ptx::make_smem_desc(sx + k * 32, 16, 1024, 2);
+                    const uint32_t add = (kb != kb0 || k != 0) ? 1u : 0u;
+                    if (PAIR == 2) ptx::mma_i8_ss_pair(tmem_base, wd, xd, idesc, add);
+                    else ptx::mma_i8_ss(tmem_base, wd, xd, idesc, add);
+                }
+                if (PAIR == 2) ptx::mma_commit_pair(ptx::smem_u32(&tail->empty[stage]), both);
+                else ptx::mma_commit(ptx::smem_u32(&tail->empty[stage]));
             }
             __syncwarp();
             if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
         }
-        if (ok && lane == 0) ptx::mma_commit(ptx::smem_u32(&tail->tmem_full));
+        if (ok && lane == 0) {
+            if (PAIR == 2) ptx::mma_commit_pair(ptx::smem_u32(&tail->tmem_full), both);
+            else ptx::mma_commit(ptx::smem_u32(&tail->tmem_full));
+        }
         __syncwarp();
     }
-    // everything the MMAs read has been read once the accumulator is complete: the ring is free for partial sums
+    // everything the MMAs read has been read once the accumulator is complete: the ring is free for partial sums,
+    // laid out [token][128 channels]
     int* part = reinterpret_cast<int*>(base_ptr);
-    const int q = warp & 3;
-    const int n = n0 + q * 32 + lane;
     bool done = false;
-    float cs = 0.0f, cb = 0.0f;
     if (warp >= 2) {
         ptx::dependency_wait();
-        if (n < out) {
-            cs = ws[n];
-            if (bias != nullptr) cb = as_f32(bias[n]);
-        }
         done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {
             ptx::tc_fence_after();
+            const int q = warp & 3;
             const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16);
+            const int last = min(BN, rows - t0);
 #pragma unroll 1
-            for (int c = 0; c < BN; c += 16) {
+            for (int c = 0; c < last; c += 16) {
                 uint32_t r[16];
                 ptx::tmem_ld_32x32b_x16(taddr + (uint32_t)c, r);
                 ptx::tmem_ld_wait();
-                if (split == 1) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int t = t0 + c + j;
-                        if (t < rows && n < out) y[(int64_t)t * out + n] = (T)int8_out((int)r[j], xs[t], cs, cb);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) part[(c + j) * 128 + q * 32 + lane] = (int)r[j];
-                }
+                for (int j = 0; j < 16; ++j) part[(c + j) * 128 + q * 32 + lane] = (int)r[j];
             }
         }
     }
@@ -713,27 +747,58 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     if (split > 1) {
         __syncwarp();
         ptx::cluster_sync_all();
-        if (done) {
-            const uint32_t mine = ptx::smem_u32(part) + (uint32_t)(q * 32 + lane) * 4u;
-            uint32_t peer[I8_MAX_SPLIT];
+    } else {
+        __syncthreads();
+    }
+    if (done) {
+        // a warp takes whole token columns, a lane four channels of each; four columns' loads are in flight together
+        const int n = n0 + 4 * lane, valid = out - n;
+        const bool vec = out % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(T) - 1)) == 0;
+        float cs[4], cb[4];
 #pragma unroll
-            for (int s = 0; s < I8_MAX_SPLIT; ++s) peer[s] = ptx::map_to_cta(mine, (uint32_t)(s < split ? s : 0));
-            const int last = min(BN, rows - t0);
-            for (int c = rank; c < last; c += split) {
-                int sum = 0;
+        for (int i = 0; i < 4; ++i) {
+            cs[i] = i < valid ? ws[n + i] : 0.0f;
+            cb[i] = bias != nullptr && i < valid ? as_f32(bias[n + i]) : 0.0f;
+        }
+        const uint32_t mine = ptx::smem_u32(part) + (uint32_t)lane * 16u;
+        const int last = min(BN, rows - t0);
+        constexpr int GROUP = 4;
+        for (int c0 = part_no + split * (warp - 2); c0 < last; c0 += 4 * GROUP * split) {
+            int4 sum[GROUP];
 #pragma unroll
-                for (int s = 0; s < I8_MAX_SPLIT; ++s)
-                    if (s < split) sum += ptx::ld_shared_cluster_s32(peer[s] + (uint32_t)c * 512u);
-                if (n < out) y[(int64_t)(t0 + c) * out + n] = (T)int8_out(sum, xs[t0 + c], cs, cb);
+            for (int g = 0; g < GROUP; ++g) sum[g] = make_int4(0, 0, 0, 0);
+            for (int s = 0; s < split; ++s) {
+                const uint32_t peer = clustered ? ptx::map_to_cta(mine, (uint32_t)(s * PAIR + half)) : mine;
+                int4 v[GROUP];
+#pragma unroll
+                for (int g = 0; g < GROUP; ++g) {
+                    const int c = c0 + 4 * split * g;
+                    v[g] = c < last ? ptx::ld_shared_cluster_v4(peer + (uint32_t)c * 512u) : make_int4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int g = 0; g < GROUP; ++g) {
+                    sum[g].x += v[g].x; sum[g].y += v[g].y; sum[g].z += v[g].z; sum[g].w += v[g].w;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < GROUP; ++g) {
+                const int c = c0 + 4 * split * g;
+                if (c < last && valid > 0) {
+                    const float rs = xs[t0 + c];
+                    const float v[4] = {int8_out(sum[g].x, rs, cs[0], cb[0]), int8_out(sum[g].y, rs, cs[1], cb[1]),
+                                        int8_out(sum[g].z, rs, cs[2], cb[2]), int8_out(sum[g].w, rs, cs[3], cb[3])};
+                    store4(y + (int64_t)(t0 + c) * out + n, v, valid, vec);
+                }
             }
         }
-        __syncwarp();
-        ptx::cluster_sync_all();  // the partial sums of this CTA are read no more
     }
-    __syncthreads();
+    __syncwarp();
+    if (clustered) ptx::cluster_sync_all();  // the partial sums of this CTA are read no more, nor its tensor memory written
+    else __syncthreads();
     if (warp == 1) {
         ptx::tc_fence_after();
-        ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
+        if (PAIR == 2) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+        else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
 }
 
@@ -846,22 +911,23 @@ static int launch_pair(const int8_t* xq, const float* xs, const int8_t* wq, cons
     return SF_OK;
 }
 
-template <typename T, int BN>
+template <typename T, int BN, int PAIR>
 static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
                       int64_t rows, int pitch, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
+    using C = I8Few<BN, PAIR>;
     CUtensorMap tmW, tmX;
     if (int rc = make_byte_tensor_map(&tmW, wq, pitch, out, 128)) return rc;
-    if (int rc = make_byte_tensor_map(&tmX, xq, pitch, rows, BN)) return rc;
-    const int64_t tiles_t = (rows + BN - 1) / BN, tiles = (out + 127) / 128 * tiles_t;
-    if (tiles * I8_MAX_SPLIT > 0x7fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: too many tiles");
+    if (int rc = make_byte_tensor_map(&tmX, xq, pitch, rows, C::X_ROWS)) return rc;
+    const int64_t tiles_t = (rows + BN - 1) / BN, tiles = (out + 128 * PAIR - 1) / (128 * PAIR) * tiles_t;
+    if (tiles * 8 > 0x7fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: too many tiles");
     // doubled until most SMs stream weights, as long as every CTA keeps a block of K
     const int num_kb = (pitch + I8_BK - 1) / I8_BK;
     int split = 1;
-    while (split < I8_MAX_SPLIT && tiles * split * 4 < (int64_t)sm_count() * 3 && 2 * split <= num_kb) split *= 2;
-    auto kern = int8_few_kernel<T, BN>;
-    SF_I8_SMEM(kern, I8Few<BN>::SMEM);
-    SF_CHECK_CUDA(launch_dependent(kern, (int)(tiles * split), I8_THREADS, I8Few<BN>::SMEM, split, dependent, st, tmW, tmX, xs, ws,
-                                   (const T*)bias, (T*)y, (int)rows, (int)out, pitch, split, (int)tiles_t, status));
+    while (split < C::MAX_SPLIT && tiles * PAIR * split * 4 < (int64_t)sm_count() * 3 && 2 * split <= num_kb) split *= 2;
+    auto kern = int8_few_kernel<T, BN, PAIR>;
+    SF_I8_SMEM(kern, C::SMEM);
+    SF_CHECK_CUDA(launch_dependent(kern, (int)(tiles * PAIR * split), I8_THREADS, C::SMEM, PAIR * split, dependent, st, tmW, tmX,
+                                   xs, ws, (const T*)bias, (T*)y, (int)rows, (int)out, pitch, split, (int)tiles_t, status));
     return SF_OK;
 }
 
@@ -888,11 +954,12 @@ template <typename T>
 static int gemm_typed(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
                       int64_t rows, int64_t in, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
     const int pitch = (int)((in + 15) / 16 * 16);
-    if (rows <= 16) return launch_few<T, 16>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
-    if (rows <= 32) return launch_few<T, 32>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
-    if (rows <= 64) return launch_few<T, 64>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
-    const int64_t pair_tiles = ((rows + 255) / 256) * ((out + 255) / 256);
-    if (pair_tiles * 2 < sm_count() / 2) return launch_few<T, 128>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    if (rows <= 16) return launch_few<T, 16, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    if (rows <= 32) return launch_few<T, 32, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    if (rows <= 64) return launch_few<T, 64, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    // 256 channels x 128 tokens while such tiles fit the chip side by side, else the persistent 256 x 256 ones
+    const int64_t tiles = ((out + 255) / 256) * ((rows + 127) / 128);
+    if (rows <= 128 || 2 * tiles <= sm_count()) return launch_few<T, 128, 2>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     return launch_pair<T>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
 }
 

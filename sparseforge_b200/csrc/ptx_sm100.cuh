@@ -215,9 +215,10 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
 // kernel before this one is done and its results are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ int ld_shared_cluster_s32(uint32_t cluster_addr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(cluster_addr) : "memory");
+__device__ __forceinline__ int4 ld_shared_cluster_v4(uint32_t cluster_addr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr) : "memory");
     return v;
 }
 

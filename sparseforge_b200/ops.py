@@ -422,6 +422,8 @@ def kl_div_bwd(student2d, teacher2d, lse, row_scale, temperature=2.0, max_logit=
 # global gradient norm and clipping
 # ----------------------------------------------------------------------------------------
 _HERE = nullcontext()
+# stream handle of a device's current stream, without building a Stream object (3 us per call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
 def _on_device_of(t: torch.Tensor):
@@ -495,7 +497,7 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     with _on_device_of(grads[0]):
         norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
         scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=grads[0].device)
-        check(lib().sf_grad_norm(_addr(ptrs), _addr(sizes), _addr(codes), n, kind, _p(norm), _p(scratch), _stream()), "sf_grad_norm")
+        check(lib().sf_grad_norm(_addr(ptrs), _addr(sizes), _addr(codes), n, kind, _p(norm), _p(scratch), _raw_stream(grads[0].get_device())), "sf_grad_norm")
     return norm
 
 
@@ -512,7 +514,7 @@ def clip_grads(grads, norm, max_norm, out=None) -> None:
         raise TypeError("clip_grads: norm must be one float32 on the gradients' device")
     with _on_device_of(norm):
         check(lib().sf_clip_grads(_addr(ptrs), _addr(optrs), _addr(sizes), _addr(codes), _addr(ocodes), len(grads),
-                                  _p(norm), float(max_norm), _stream()), "sf_clip_grads")
+                                  _p(norm), float(max_norm), _raw_stream(grads[0].get_device())), "sf_clip_grads")
 
 
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
@@ -527,7 +529,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
         norm = torch.empty((), dtype=torch.float32, device=dev)
         scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=dev)
         check(lib().sf_clip_grad_norm(_addr(ptrs), _addr(optrs), _addr(sizes), _addr(codes), _addr(ocodes), n, kind,
-                                      float(max_norm), _p(norm), _p(scratch), _stream()), "sf_clip_grad_norm")
+                                      float(max_norm), _p(norm), _p(scratch), _raw_stream(grads[0].get_device())), "sf_clip_grad_norm")
     return norm
 
 
@@ -785,7 +787,7 @@ def int8_linear(x2d, wq, w_scale, bias=None, status=None):
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     with _on_device_of(x2d):
         rc = h.sf_int8_linear(x2d.data_ptr(), ld, wq.data_ptr(), w_scale.data_ptr(), _p(bias), y.data_ptr(), _DT[dtype],
-                              T, k, out, _p(ws), _p(status), _stream())
+                              T, k, out, _p(ws), _p(status), _raw_stream(dev.index))
     if rc:
         check(rc, "sf_int8_linear")
     return y
