@@ -150,7 +150,8 @@ __global__ void __launch_bounds__(THREADS)
 int8_quantize_vec_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
                          int cols, int pitch) {
     __shared__ uint32_t part[2][THREADS / 32];
-    ptx::launch_dependents();
+    ptx::dependency_wait();
+    ptx::launch_dependents();  // only now: what ran before this kernel is complete for the one behind it as well
     constexpr int PER_BLOCK = THREADS / TPR;
     const int lane = threadIdx.x % TPR, nv = cols >> 3;
     int row = blockIdx.x * PER_BLOCK + threadIdx.x / TPR;
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(kQThreads)
 int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int cols,
                      int pitch) {
     __shared__ uint32_t part[kQThreads / 32];
+    ptx::dependency_wait();
     ptx::launch_dependents();
     const T* row = x + (int64_t)blockIdx.x * ld;
     uint32_t top = 0;
@@ -464,6 +466,8 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
     extern __shared__ __align__(16) uint8_t xq[];  // [ROWS][pitch]
     __shared__ uint32_t part[ROWS][GV_WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    ptx::launch_dependents();
+    ptx::dependency_wait();
     const int step = GV_WARPS * gridDim.x;
     int n = warp * gridDim.x + blockIdx.x, at = lane * 16;
     int4 w[GV_LOADS];
@@ -567,7 +571,7 @@ struct I8Few {
     static constexpr int X_ROWS = BN / PAIR;
     static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_ROWS * I8_BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 512;
     static constexpr int MAX_SPLIT = 8 / PAIR;              // clusters of at most eight CTAs
     static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "partial sums reuse the ring");
 };
@@ -579,6 +583,7 @@ struct I8FewTail {
     uint64_t tmem_full;
     uint32_t tmem_base;
     int abort_flag;
+    float xs[128];  // scales of the tile's tokens
 };
 
 // Four consecutive output channels of one token.
@@ -725,8 +730,19 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     // laid out [token][128 channels]
     int* part = reinterpret_cast<int*>(base_ptr);
     bool done = false;
+    // output: a warp takes whole token columns, a lane four channels of each; their scales are fetched ahead
+    const int n = n0 + 4 * lane, valid = out - n;
+    float cs[4], cb[4];
+    ptx::launch_dependents();
     if (warp >= 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            cs[i] = i < valid ? ws[n + i] : 0.0f;
+            cb[i] = bias != nullptr && i < valid ? as_f32(bias[n + i]) : 0.0f;
+        }
         ptx::dependency_wait();
+        const int c = threadIdx.x - 64;
+        if (c < BN) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
         done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {
             ptx::tc_fence_after();
@@ -751,18 +767,10 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         __syncthreads();
     }
     if (done) {
-        // a warp takes whole token columns, a lane four channels of each; four columns' loads are in flight together
-        const int n = n0 + 4 * lane, valid = out - n;
         const bool vec = out % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(T) - 1)) == 0;
-        float cs[4], cb[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cs[i] = i < valid ? ws[n + i] : 0.0f;
-            cb[i] = bias != nullptr && i < valid ? as_f32(bias[n + i]) : 0.0f;
-        }
         const uint32_t mine = ptx::smem_u32(part) + (uint32_t)lane * 16u;
         const int last = min(BN, rows - t0);
-        constexpr int GROUP = 4;
+        constexpr int GROUP = 4;  // columns whose loads are in flight together
         for (int c0 = part_no + split * (warp - 2); c0 < last; c0 += 4 * GROUP * split) {
             int4 sum[GROUP];
 #pragma unroll
@@ -784,7 +792,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             for (int g = 0; g < GROUP; ++g) {
                 const int c = c0 + 4 * split * g;
                 if (c < last && valid > 0) {
-                    const float rs = xs[t0 + c];
+                    const float rs = tail->xs[c];
                     const float v[4] = {int8_out(sum[g].x, rs, cs[0], cb[0]), int8_out(sum[g].y, rs, cs[1], cb[1]),
                                         int8_out(sum[g].z, rs, cs[2], cb[2]), int8_out(sum[g].w, rs, cs[3], cb[3])};
                     store4(y + (int64_t)(t0 + c) * out + n, v, valid, vec);
@@ -814,49 +822,10 @@ static int check_int8(const char* who, int64_t rows, int64_t in, int64_t out) {
     return SF_OK;
 }
 
-// Rows that start on 16-byte boundaries and are a multiple of 8 long move in 16-byte accesses.
-static bool rows_vectorise(const void* x, int dtype, int64_t ld, int64_t rows, int64_t cols) {
-    const int64_t esize = dtype == SF_F32 ? 4 : 2;
-    return aligned16(x) && cols % 8 == 0 && (rows == 1 || ld * esize % 16 == 0);
-}
-
-template <typename T>
-static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
-                          cudaStream_t st) {
-    const int pitch = (int)((cols + 15) / 16 * 16);
-    // A warp per row up to 1024 elements, a block per row up to 16384, all of the row in registers. [8192, 4096] bf16: 17.7 us
-    // (5.7 TB/s) with 128 threads per row, 18.9 with 256, 21.5 with 512; [8192, 11008]: 44.3 us (6.1 TB/s).
-#define SF_I8_QUANT(THREADS, TPR, NV)                                                                                 \
-    do {                                                                                                              \
-        auto kern = int8_quantize_vec_kernel<T, THREADS, TPR, NV>;                                                    \
-        const int64_t need = (rows + THREADS / TPR - 1) / (THREADS / TPR);                                            \
-        const int grid = (int)std::min<int64_t>(need, (int64_t)sm_count() * (kQVecResident / THREADS));               \
-        kern<<<grid, THREADS, 0, st>>>(x, ld, q, scale, (int)rows, (int)cols, pitch);                                 \
-    } while (0)
-    if (vec && cols <= 1024) {
-        SF_I8_QUANT(256, 32, 4);
-    } else if (vec && cols <= 4096) {
-        SF_I8_QUANT(128, 128, 4);
-    } else if (vec && cols <= 12288) {
-        SF_I8_QUANT(256, 256, 6);
-    } else if (vec && cols <= 16384) {
-        SF_I8_QUANT(512, 512, 4);
-#undef SF_I8_QUANT
-    } else {
-        int8_quantize_kernel<T><<<(int)rows, kQThreads, 0, st>>>(x, ld, q, scale, (int)cols, pitch);
-    }
-    SF_CHECK_CUDA(cudaGetLastError());
-    return SF_OK;
-}
-static int quantize_impl(const void* x, int dtype, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
-                         cudaStream_t st) {
-    const bool vec = rows_vectorise(x, dtype, ld, rows, cols);
-    return dtype == SF_F32 ? quantize_typed((const float*)x, vec, ld, q, scale, rows, cols, st)
-                           : quantize_typed((const __nv_bfloat16*)x, vec, ld, q, scale, rows, cols, st);
-}
-
-// dependent: the launch may be set up, and load weights, while the kernel before it in the stream still runs. Only behind
-// this file's quantiser, which is itself an ordinary launch: whatever wrote the weights before it is complete then.
+// Launch that may be set up while the kernel before it in the stream still runs; every kernel launched this way waits for
+// that one's results (griddepcontrol.wait, in every block) before it touches any of them. The product behind the
+// quantiser loads weights before it waits: the quantiser lets it start only after its own wait, so whatever wrote the
+// weights is complete by then. Called on its own the product is an ordinary launch (dependent = false).
 template <typename... KArgs, typename... Args>
 static cudaError_t launch_dependent(void (*kern)(KArgs...), int grid, int threads, int smem, int cluster, bool dependent,
                                     cudaStream_t st, const Args&... args) {
@@ -880,6 +849,46 @@ static cudaError_t launch_dependent(void (*kern)(KArgs...), int grid, int thread
     cfg.numAttrs = (unsigned)n;
     cfg.attrs = attr;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
+// Rows that start on 16-byte boundaries and are a multiple of 8 long move in 16-byte accesses.
+static bool rows_vectorise(const void* x, int dtype, int64_t ld, int64_t rows, int64_t cols) {
+    const int64_t esize = dtype == SF_F32 ? 4 : 2;
+    return aligned16(x) && cols % 8 == 0 && (rows == 1 || ld * esize % 16 == 0);
+}
+
+template <typename T>
+static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                          cudaStream_t st) {
+    const int pitch = (int)((cols + 15) / 16 * 16);
+    // A warp per row up to 1024 elements, a block per row up to 16384, all of the row in registers. [8192, 4096] bf16: 17.7 us
+    // (5.7 TB/s) with 128 threads per row, 18.9 with 256, 21.5 with 512; [8192, 11008]: 44.3 us (6.1 TB/s).
+#define SF_I8_QUANT(THREADS, TPR, NV)                                                                                 \
+    do {                                                                                                              \
+        auto kern = int8_quantize_vec_kernel<T, THREADS, TPR, NV>;                                                    \
+        const int64_t need = (rows + THREADS / TPR - 1) / (THREADS / TPR);                                            \
+        const int grid = (int)std::min<int64_t>(need, (int64_t)sm_count() * (kQVecResident / THREADS));               \
+        SF_CHECK_CUDA(launch_dependent(kern, grid, THREADS, 0, 1, true, st, x, ld, q, scale, (int)rows, (int)cols, pitch)); \
+    } while (0)
+    if (vec && cols <= 1024) {
+        SF_I8_QUANT(256, 32, 4);
+    } else if (vec && cols <= 4096) {
+        SF_I8_QUANT(128, 128, 4);
+    } else if (vec && cols <= 12288) {
+        SF_I8_QUANT(256, 256, 6);
+    } else if (vec && cols <= 16384) {
+        SF_I8_QUANT(512, 512, 4);
+#undef SF_I8_QUANT
+    } else {
+        SF_CHECK_CUDA(launch_dependent(int8_quantize_kernel<T>, (int)rows, kQThreads, 0, 1, true, st, x, ld, q, scale, (int)cols, pitch));
+    }
+    return SF_OK;
+}
+static int quantize_impl(const void* x, int dtype, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
+                         cudaStream_t st) {
+    const bool vec = rows_vectorise(x, dtype, ld, rows, cols);
+    return dtype == SF_F32 ? quantize_typed((const float*)x, vec, ld, q, scale, rows, cols, st)
+                           : quantize_typed((const __nv_bfloat16*)x, vec, ld, q, scale, rows, cols, st);
 }
 
 // Raises a kernel's dynamic shared memory limit once per device and thread.
@@ -939,8 +948,8 @@ static int launch_stream(const void* x, int64_t ld, const int8_t* wq, const floa
     auto kern = int8_stream_kernel<T, ROWS>;
     SF_I8_SMEM(kern, GV_X_BYTES);
     const int grid = (int)std::min<int64_t>(sm_count(), (out + GV_WARPS - 1) / GV_WARPS);
-    kern<<<grid, GV_THREADS, smem, st>>>((const T*)x, ld, wq, ws, (const T*)bias, (T*)y, (int)in, (int)out, pitch, vec ? 1 : 0);
-    SF_CHECK_CUDA(cudaGetLastError());
+    SF_CHECK_CUDA(launch_dependent(kern, grid, GV_THREADS, smem, 1, true, st, (const T*)x, ld, wq, ws, (const T*)bias, (T*)y, (int)in,
+                                   (int)out, pitch, vec ? 1 : 0));
     return SF_OK;
 }
 template <typename T>
