@@ -560,7 +560,9 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
 // The weight is what has to be read, so it is the 128-row operand and the tokens are the narrow one. A tile's K range
 // is cut into `split` parts so that about all SMs stream weights; the parts' CTAs form a cluster, each leaves its partial
 // sums (exact integers) in its shared memory, and after a cluster barrier every CTA adds up its share of the token
-// columns over all parts and writes them: one launch, no workspace, any order of arrival gives the same sum.
+// columns (column c belongs to part c mod split) over all parts and writes them: one launch, no workspace, any order of
+// arrival gives the same sum. (Stores into the owner's shared memory instead save the second barrier but cost
+// more than it: [64, 4096] x [4096, 4096] 9.5 -> 15.9 us.)
 // PAIR = 2 (more than 64 tokens): two CTAs share a 256-row tile (cta_group::2), each loads half of the tokens, 24 KiB per
 // stage instead of 32 for the same products: above 64 tokens the traffic into the SMs is what bounds the tile.
 // The weight loads of the first stages are issued before the kernel waits for the quantised rows.
@@ -629,7 +631,26 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     const int n0 = (tile / tiles_t * PAIR + half) * 128, t0 = tile % tiles_t * BN;
     const int num_kb = (pitch + I8_BK - 1) / I8_BK;
     const int kb0 = (int)((int64_t)num_kb * part_no / split), kb1 = (int)((int64_t)num_kb * (part_no + 1) / split);
+    const int ahead = min(C::STAGES, kb1 - kb0);
 
+    auto load = [&](int stage, int kb, bool weights, bool tokens) {
+        const uint32_t local = ptx::smem_u32(&tail->full[stage]);
+        const uint32_t sw = base + stage * C::STAGE_BYTES, sx = sw + I8_OPERAND_BYTES;
+        if (PAIR == 2) {
+            const uint32_t bar = ptx::map_to_cta(local, leader);
+            if (weights) {
+                if (half == 0) ptx::mbar_arrive_expect_tx(local, 2 * C::STAGE_BYTES);
+                ptx::tma_load_2d_pair(sw, &tmW, bar, kb * I8_BK, n0);
+            }
+            if (tokens) ptx::tma_load_2d_pair(sx, &tmX, bar, kb * I8_BK, t0 + half * C::X_ROWS);
+        } else {
+            if (weights) {
+                ptx::mbar_arrive_expect_tx(local, C::STAGE_BYTES);
+                ptx::tma_load_2d(sw, &tmW, local, kb * I8_BK, n0);
+            }
+            if (tokens) ptx::tma_load_2d(sx, &tmX, local, kb * I8_BK, t0);
+        }
+    };
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; ++s) {
             ptx::mbar_init(ptx::smem_u32(&tail->full[s]), 1);
@@ -638,6 +659,8 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         ptx::mbar_init(ptx::smem_u32(&tail->tmem_full), 1);
         tail->abort_flag = 0;
         ptx::fence_barrier_init();
+        if (PAIR == 1)  // nobody else's barriers are involved: the weights are on their way before the block is set up
+            for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
     }
     if (warp == 1) {
         if (PAIR == 2) {
@@ -648,10 +671,6 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             ptx::tmem_relinquish();
         }
     }
-    if (warp == 0 && lane == 0) {
-        ptx::prefetch_tensormap(&tmW);
-        ptx::prefetch_tensormap(&tmX);
-    }
     ptx::tc_fence_before();
     __syncthreads();
     if (PAIR == 2) ptx::cluster_sync_all();  // the other CTA's copies and commits arrive on this CTA's barriers
@@ -659,26 +678,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     const uint32_t tmem_base = tail->tmem_base;
 
     if (warp == 0) {
-        auto load = [&](int stage, int kb, bool weights, bool tokens) {
-            const uint32_t local = ptx::smem_u32(&tail->full[stage]);
-            const uint32_t sw = base + stage * C::STAGE_BYTES, sx = sw + I8_OPERAND_BYTES;
-            if (PAIR == 2) {
-                const uint32_t bar = ptx::map_to_cta(local, leader);
-                if (weights) {
-                    if (half == 0) ptx::mbar_arrive_expect_tx(local, 2 * C::STAGE_BYTES);
-                    ptx::tma_load_2d_pair(sw, &tmW, bar, kb * I8_BK, n0);
-                }
-                if (tokens) ptx::tma_load_2d_pair(sx, &tmX, bar, kb * I8_BK, t0 + half * C::X_ROWS);
-            } else {
-                if (weights) {
-                    ptx::mbar_arrive_expect_tx(local, C::STAGE_BYTES);
-                    ptx::tma_load_2d(sw, &tmW, local, kb * I8_BK, n0);
-                }
-                if (tokens) ptx::tma_load_2d(sx, &tmX, local, kb * I8_BK, t0);
-            }
-        };
-        const int ahead = min(C::STAGES, kb1 - kb0);
-        if (lane == 0)
+        if (PAIR == 2 && lane == 0)
             for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
         ptx::dependency_wait();
         if (lane == 0)
@@ -729,21 +729,20 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     // everything the MMAs read has been read once the accumulator is complete: the ring is free for partial sums,
     // laid out [token][128 channels]
     int* part = reinterpret_cast<int*>(base_ptr);
-    bool done = false;
     // output: a warp takes whole token columns, a lane four channels of each; their scales are fetched ahead
     const int n = n0 + 4 * lane, valid = out - n;
     float cs[4], cb[4];
-    ptx::launch_dependents();
-    if (warp >= 2) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            cs[i] = i < valid ? ws[n + i] : 0.0f;
-            cb[i] = bias != nullptr && i < valid ? as_f32(bias[n + i]) : 0.0f;
-        }
-        ptx::dependency_wait();
+    for (int i = 0; i < 4; ++i) {
+        cs[i] = i < valid ? ws[n + i] : 0.0f;
+        cb[i] = bias != nullptr && i < valid ? as_f32(bias[n + i]) : 0.0f;
+    }
+    ptx::launch_dependents();
+    ptx::dependency_wait();
+    if (warp >= 2) {
         const int c = threadIdx.x - 64;
         if (c < BN) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
-        done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
+        const bool done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {
             ptx::tc_fence_after();
             const int q = warp & 3;
@@ -766,12 +765,12 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     } else {
         __syncthreads();
     }
-    if (done) {
+    if (*abort_flag == 0) {
         const bool vec = out % 4 == 0 && (reinterpret_cast<uintptr_t>(y) & (4 * sizeof(T) - 1)) == 0;
         const uint32_t mine = ptx::smem_u32(part) + (uint32_t)lane * 16u;
         const int last = min(BN, rows - t0);
-        constexpr int GROUP = 4;  // columns whose loads are in flight together
-        for (int c0 = part_no + split * (warp - 2); c0 < last; c0 += 4 * GROUP * split) {
+        constexpr int GROUP = 4, WARPS = I8_THREADS / 32;  // columns whose loads are in flight together; all warps take part
+        for (int c0 = part_no + split * warp; c0 < last; c0 += WARPS * GROUP * split) {
             int4 sum[GROUP];
 #pragma unroll
             for (int g = 0; g < GROUP; ++g) sum[g] = make_int4(0, 0, 0, 0);
@@ -780,8 +779,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 int4 v[GROUP];
 #pragma unroll
                 for (int g = 0; g < GROUP; ++g) {
-                    const int c = c0 + 4 * split * g;
-                    v[g] = c < last ? ptx::ld_shared_cluster_v4(peer + (uint32_t)c * 512u) : make_int4(0, 0, 0, 0);
+                    const int c = c0 + WARPS * split * g;
+                    v[g] = make_int4(0, 0, 0, 0);
+                    if (c < last) v[g] = ptx::ld_shared_cluster_v4(peer + (uint32_t)c * 512u);
                 }
 #pragma unroll
                 for (int g = 0; g < GROUP; ++g) {
@@ -790,7 +790,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             }
 #pragma unroll
             for (int g = 0; g < GROUP; ++g) {
-                const int c = c0 + 4 * split * g;
+                const int c = c0 + WARPS * split * g;
                 if (c < last && valid > 0) {
                     const float rs = tail->xs[c];
                     const float v[4] = {int8_out(sum[g].x, rs, cs[0], cb[0]), int8_out(sum[g].y, rs, cs[1], cb[1]),
@@ -801,7 +801,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         }
     }
     __syncwarp();
-    if (clustered) ptx::cluster_sync_all();  // the partial sums of this CTA are read no more, nor its tensor memory written
+    if (clustered) ptx::cluster_sync_all();  // this CTA's partial sums are read no more
     else __syncthreads();
     if (warp == 1) {
         ptx::tc_fence_after();

@@ -218,7 +218,7 @@ __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol
 __device__ __forceinline__ int4 ld_shared_cluster_v4(uint32_t cluster_addr) {
     int4 v;
     asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr) : "memory");
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(cluster_addr));
     return v;
 }
 
