@@ -569,12 +569,12 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
 // ---------------------------------------------------------------------------------------------------------
 template <int BN, int PAIR>
 struct I8Few {
-    static constexpr int STAGES = BN * PAIR <= 32 ? 5 : 4;  // 94 to 104 KB: two CTAs per SM
+    static constexpr int STAGES = BN > 128 ? 6 : (BN * PAIR <= 32 ? 5 : 4);  // up to 128 tokens 94 to 104 KB: two CTAs per SM
     static constexpr int X_ROWS = BN / PAIR;
     static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_ROWS * I8_BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 512;
-    static constexpr int MAX_SPLIT = 8 / PAIR;              // clusters of at most eight CTAs
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 1024;
+    static constexpr int MAX_SPLIT = PAIR == 2 ? 2 : 8;  // clusters of at most eight CTAs, of four where one fills an SM
     static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "partial sums reuse the ring");
 };
 
@@ -585,7 +585,7 @@ struct I8FewTail {
     uint64_t tmem_full;
     uint32_t tmem_base;
     int abort_flag;
-    float xs[128];  // scales of the tile's tokens
+    float xs[256];  // scales of the tile's tokens
 };
 
 // Four consecutive output channels of one token.
@@ -610,7 +610,7 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vali
 }
 
 template <typename T, int BN, int PAIR>
-__global__ void __launch_bounds__(I8_THREADS, 2)
+__global__ void __launch_bounds__(I8_THREADS, BN > 128 ? 1 : 2)
 int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                 const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
                 int rows, int out, int pitch, int split, int tiles_t, int32_t* status) {
@@ -675,6 +675,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     __syncthreads();
     if (PAIR == 2) ptx::cluster_sync_all();  // the other CTA's copies and commits arrive on this CTA's barriers
     ptx::tc_fence_after();
+    ptx::launch_dependents();
     const uint32_t tmem_base = tail->tmem_base;
 
     if (warp == 0) {
@@ -737,11 +738,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         cs[i] = i < valid ? ws[n + i] : 0.0f;
         cb[i] = bias != nullptr && i < valid ? as_f32(bias[n + i]) : 0.0f;
     }
-    ptx::launch_dependents();
     ptx::dependency_wait();
     if (warp >= 2) {
-        const int c = threadIdx.x - 64;
-        if (c < BN) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
+        for (int c = threadIdx.x - 64; c < BN; c += 128) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
         const bool done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {
             ptx::tc_fence_after();
@@ -880,7 +879,8 @@ static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* sc
         SF_I8_QUANT(512, 512, 4);
 #undef SF_I8_QUANT
     } else {
-        SF_CHECK_CUDA(launch_dependent(int8_quantize_kernel<T>, (int)rows, kQThreads, 0, 1, true, st, x, ld, q, scale, (int)cols, pitch));
+        SF_CHECK_CUDA(launch_dependent(int8_quantize_kernel<T>, (int)rows, kQThreads, 0, 1, true, st, x, ld, q, scale,
+                                       (int)cols, pitch));
     }
     return SF_OK;
 }
@@ -929,10 +929,19 @@ static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const
     if (int rc = make_byte_tensor_map(&tmX, xq, pitch, rows, C::X_ROWS)) return rc;
     const int64_t tiles_t = (rows + BN - 1) / BN, tiles = (out + 128 * PAIR - 1) / (128 * PAIR) * tiles_t;
     if (tiles * 8 > 0x7fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: too many tiles");
-    // doubled until most SMs stream weights, as long as every CTA keeps a block of K
+    // Doubled until most SMs stream weights, as long as every CTA keeps a block of K; and on to two CTAs per SM (tiles of up
+    // to 64 tokens), whose loads cover each other's latencies, while each keeps 16 blocks: shorter parts cost more in the join
+    // than they save ([64, 4096] x [4096, 4096]: 9.3 us with four parts of 8 blocks, 10.5 with eight of 4).
     const int num_kb = (pitch + I8_BK - 1) / I8_BK;
+    const int64_t sms = sm_count();
     int split = 1;
-    while (split < C::MAX_SPLIT && tiles * PAIR * split * 4 < (int64_t)sm_count() * 3 && 2 * split <= num_kb) split *= 2;
+    while (split < C::MAX_SPLIT && 2 * split <= num_kb) {
+        const int64_t ctas = tiles * PAIR * split;
+        const bool idle = ctas * 4 < sms * (BN > 128 ? 2 : 3);
+        const bool room = BN <= 64 && ctas <= sms && num_kb >= 32 * split;
+        if (!idle && !room) break;
+        split *= 2;
+    }
     auto kern = int8_few_kernel<T, BN, PAIR>;
     SF_I8_SMEM(kern, C::SMEM);
     SF_CHECK_CUDA(launch_dependent(kern, (int)(tiles * PAIR * split), I8_THREADS, C::SMEM, PAIR * split, dependent, st, tmW, tmX,
@@ -965,10 +974,14 @@ static int gemm_typed(const int8_t* xq, const float* xs, const int8_t* wq, const
     const int pitch = (int)((in + 15) / 16 * 16);
     if (rows <= 16) return launch_few<T, 16, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     if (rows <= 32) return launch_few<T, 32, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
-    if (rows <= 64) return launch_few<T, 64, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
-    // 256 channels x 128 tokens while such tiles fit the chip side by side, else the persistent 256 x 256 ones
-    const int64_t tiles = ((out + 255) / 256) * ((rows + 127) / 128);
-    if (rows <= 128 || 2 * tiles <= sm_count()) return launch_few<T, 128, 2>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    // More rows. While 128 x 64 tiles fit the chip at two per SM they are the fastest ([512, 4096] x [4096, 4096]: 16.0 us, 256 x
+    // 256 tiles cut in two 16.4, persistent 17.5; [128, 4096] x [11008, 4096]: 16.0, 18.4, 19.1), but their operands are
+    // loaded more often: past 256 rows a long reduction takes 256 x 256 tiles cut in two where those leave half of the SMs
+    // idle ([512, 11008] x [4096, 11008]: 25.4 us against 31.8 and 33.6). Beyond that, persistent tiles.
+    const int64_t small = ((out + 127) / 128) * ((rows + 63) / 64), large = ((out + 255) / 256) * ((rows + 255) / 256);
+    if (rows > 256 && pitch >= 8192 && large * 4 <= sm_count())
+        return launch_few<T, 256, 2>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
+    if (small <= 2 * (int64_t)sm_count()) return launch_few<T, 64, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     return launch_pair<T>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
 }
 
