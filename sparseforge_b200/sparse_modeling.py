@@ -368,6 +368,9 @@ class SparseLinear(nn.Linear):
             prm = getattr(self, n)
             if prm.dtype != torch.float32:
                 prm.data = old.to(device=prm.device, dtype=torch.float32)
+        for n in ("_i8_weight", "_i8_scale", "_i8_status"):  # 8-bit inference form: moved, never converted
+            if getattr(self, n, None) is not None:
+                setattr(self, n, getattr(self, n).to(self.weight.device))
         self.weight.mask = self.mask
         self.weight._sf_owner = weakref.ref(self)
         self._wm_key = None
@@ -692,10 +695,43 @@ class SparseLinear(nn.Linear):
         y = ops.sparse24_gemm(x2d.contiguous(), self._sp_values, self._sp_meta_tc, bias=self.bias, status=self._sp_status)
         return y.view(*x.shape[:-1], self.out_features).to(x.dtype)
 
+    # -- inference in 8-bit integers ------------------------------------------------------------
+    @torch.no_grad()
+    def quantize_for_inference(self, bake: bool = True):
+        """Stores weight * hard(mask) in 8-bit integers with one scale per output channel and switches ``mode`` to
+        ``"int8_forward"``: a call quantises its input rows on the fly, one scale per token, and multiplies in 8
+        bits with an exact 32-bit sum (``ops.int8_linear``). Any hard view; float32 or bfloat16 weights of any size.
+        ``bake=False`` takes the weight as it is (its zeros are already in place). No counterpart in the
+        reference, whose inference bake-in stays dense (legacy/eval_wiki_ppl.py:548-651). Forward only; the weight is kept."""
+        if self.weight.dtype not in (torch.float32, torch.bfloat16):
+            raise TypeError(f"quantize_for_inference: float32 or bfloat16 weights expected, got {self.weight.dtype}")
+        w = self.weight.data
+        if bake:
+            w = w * self._hard_mask_from_soft(self.mask.data).to(w.dtype)
+        self._i8_weight, self._i8_scale = ops.int8_quantize_rows(w.contiguous())
+        self._i8_status = torch.zeros(4, dtype=torch.int32, device=w.device)
+        self.mode = "int8_forward"
+        self._inference_optimized = True
+        return self
+
+    def _int8_forward(self, x):
+        if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad and self.training):
+            raise RuntimeError("mode 'int8_forward' is inference only; call it under torch.no_grad() / eval()")
+        if getattr(self, "_i8_weight", None) is None:
+            raise RuntimeError("mode 'int8_forward' without an 8-bit weight: call quantize_for_inference()")
+        x2d = x.reshape(-1, self.in_features)
+        if x2d.dtype not in (torch.float32, torch.bfloat16):
+            x2d = x2d.to(torch.float32)  # float16 values are exact in float32
+        if x2d.stride(1) != 1 or x2d.stride(0) < self.in_features:  # rows may be strided, not interleaved or repeated
+            x2d = x2d.contiguous()
+        bias = self.bias if self.bias is None or self.bias.dtype == x2d.dtype else self.bias.to(x2d.dtype)
+        y = ops.int8_linear(x2d, self._i8_weight, self._i8_scale, bias, status=self._i8_status)
+        return y.view(*x.shape[:-1], self.out_features).to(x.dtype)
+
     def forward(self, x):
         """legacy/sparse_modeling.py:737-796."""
-        if self.mode == "sparse24_forward":
-            out = self._sparse24_forward(x)
+        if self.mode in ("sparse24_forward", "int8_forward"):
+            out = self._sparse24_forward(x) if self.mode == "sparse24_forward" else self._int8_forward(x)
             if self.SLoRB and hasattr(self, "x_proj"):
                 # the low-rank bypass stays on at inference (legacy/eval_wiki_ppl.py:560-575, 623)
                 out = out + self._slorb(x)

@@ -493,13 +493,17 @@ def finalize_hard_masks(model):
 
 
 @torch.no_grad()
-def optimize_sparse_model_for_inference(model, use_slorb: bool = False, compressed: bool = False):
+def optimize_sparse_model_for_inference(model, use_slorb: bool = False, compressed: bool = False, int8: bool = False):
     """Inference bake-in (legacy/eval_wiki_ppl.py:548-651): every SparseLinear gets its HARD mask
     multiplied into the weight once and then runs ``dense_forward`` (a layer whose finalized
     weight already carries the zeros is not multiplied twice). With ``use_slorb`` the layer stays
     in ``sparse_forward`` and only its mask is made binary, as in the reference.
     ``compressed=True`` goes one step further than the reference: bf16 layers with a 2:4 hard view are stored in the
-    2:4 compressed form and run on the sparse tensor cores (``SparseLinear.compress_for_inference``)."""
+    2:4 compressed form and run on the sparse tensor cores (``SparseLinear.compress_for_inference``).
+    ``int8=True`` stores the baked weight of float32 and bfloat16 layers in 8-bit integers and quantises every call's input
+    rows (``SparseLinear.quantize_for_inference``). The two exclude each other; neither applies with ``use_slorb``."""
+    if compressed and int8:
+        raise ValueError("optimize_sparse_model_for_inference: choose one of compressed and int8")
     optimized = total = 0
     for m in _sparse_modules(get_raw_model(model)):
         total += 1
@@ -519,7 +523,9 @@ def optimize_sparse_model_for_inference(model, use_slorb: bool = False, compress
             else:
                 m.mask.data.copy_(hard.to(m.mask.dtype))
         if can_dense:
-            if compressed and m.weight.dtype == torch.bfloat16 and m.in_features % 16 == 0 and m._is_2to4_view():
+            if int8 and m.weight.dtype in (torch.float32, torch.bfloat16):
+                m.quantize_for_inference(bake=False)
+            elif compressed and m.weight.dtype == torch.bfloat16 and m.in_features % 16 == 0 and m._is_2to4_view():
                 m.mask.data.copy_(hard.to(m.mask.dtype))
                 m.compress_for_inference()
             else:

@@ -357,3 +357,38 @@ def test_gradient_clipping_refusals_without_a_gpu():
     p.grad = torch.zeros(8)
     with pytest.raises(RuntimeError, match="CUDA"):
         utils.clip_grad_norm_([p], 1.0)
+
+
+def test_int8_refusals_without_a_gpu():
+    """Bad 8-bit calls are refused on the host; no CPU path."""
+    from sparseforge_b200 import _lib, ops
+    import sparseforge_b200 as sf
+
+    lib = _lib.lib()
+    assert int(lib.sf_int8_pitch(1)) == 16 and int(lib.sf_int8_pitch(4096)) == 4096 and int(lib.sf_int8_pitch(1003)) == 1008
+    assert int(lib.sf_int8_linear_workspace_bytes(1, 4096)) == 0
+    assert int(lib.sf_int8_linear_workspace_bytes(16, 1003)) == 16 * 1008 + 64
+    A = 4096
+    assert lib.sf_int8_quantize_rows(A, _lib.SF_I8, 8, A, A, 1, 8, None) == -1
+    assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 4, A, A, 2, 8, None) == -1      # rows overlap
+    assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 8, A + 8, A, 2, 8, None) == -3  # q not 16-byte aligned
+    assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 1 << 20, A, A, 2, 131057, None) == -2
+    assert lib.sf_int8_quantize_rows(None, _lib.SF_F32, 8, None, None, 0, 8, None) == 0  # no rows: nothing to do
+    assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, -1, 8, 8, None, None) == -1
+    assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, 1, 8, 0, None, None) == -1
+    assert lib.sf_int8_gemm(A + 1, A, A, A, None, A, _lib.SF_BF16, 1, 8, 8, None, None) == -3
+    assert lib.sf_int8_gemm(A, None, A, A, None, A, _lib.SF_BF16, 1, 8, 8, None, None) == -1
+    assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_I8, 1, 8, 8, A, None, None) == -1
+    assert lib.sf_int8_linear(A, 4, A, A, None, A, _lib.SF_F32, 8, 8, 8, A, None, None) == -1
+    assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_F32, 8, 8, 8, None, None, None) == -1  # workspace missing
+    assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_F32, 8, 131057, 8, A, None, None) < 0
+    assert b"ld=8" in lib.sf_last_error_string() or b"overflow" in lib.sf_last_error_string()
+    x, q, s = torch.zeros(2, 8), torch.zeros(4, 16, dtype=torch.int8), torch.ones(4)
+    for call in (lambda: ops.int8_quantize_rows(x), lambda: ops.int8_linear(x, q, s), lambda: ops.int8_gemm(q, s, q, s)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    layer = sf.SparseLinear(16, 16, sparselinear_config=sf.SparseLinearConfig(), bias=False)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        layer.quantize_for_inference()
+    with pytest.raises(TypeError):
+        layer.half().quantize_for_inference()
