@@ -442,15 +442,21 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 }
 
 // ---------------------------------------------------------------------------------------------------------
-// One row or two: no tensor cores, one launch. A warp takes a whole weight row in pieces of 4 KiB, eight 16-byte loads
-// per lane straight into registers; 32 warps per SM keep 128 KiB in flight, as much as an SM's share of a [4096, 4096]
-// weight. The first piece is under way before the block quantises the tokens into shared memory: each block
-// repeats that small work, which saves a launch and a wait. A row's sum (dp4a) is added up over the warp.
+// One row or two: no tensor cores, one launch. A block owns consecutive output channels; its 32 warps take their weight rows
+// in pieces of 2 KiB, four 16-byte loads per lane straight into registers, the next piece under way while one is
+// multiplied (dp4a): 128 KiB in flight per SM, as much as an SM's share of a [4096, 4096] weight, and the last turn is
+// never more than one piece long. The first pieces are requested before the block quantises the tokens into shared
+// memory: each block repeats that small work, which saves a launch and a wait. Pieces' sums meet in shared memory (integer
+// additions: their order does not matter).
 // ---------------------------------------------------------------------------------------------------------
 constexpr int GV_WARPS = 32, GV_THREADS = 32 * GV_WARPS;
-constexpr int GV_LOADS = 8, GV_PIECE = GV_LOADS * 512;
+constexpr int GV_LOADS = 4, GV_PIECE = GV_LOADS * 512;
 constexpr int GV_X_BYTES = 128 * 1024;  // room for the quantised tokens
 constexpr int GV_MAX_ROWS = 2;
+constexpr int GV_CHANNELS = 2048;       // most output channels of a block
+// Called back to back: 0 / 64 / 128 / 512 KiB fetched ahead per block take [1, 4096] x [4096, 4096] 6.5 / 5.9 / 6.3 / 6.3 us
+// and x [11008, 4096] 11.3 / 10.2 / 10.0 / 11.5 us.
+constexpr int GV_AHEAD_BYTES = 64 * 1024;
 
 __device__ __forceinline__ int4 ld_weights(const int8_t* p) {
     int4 v;
@@ -465,18 +471,39 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
                    const T* __restrict__ bias, T* __restrict__ y, int in, int out, int pitch, int vec) {
     extern __shared__ __align__(16) uint8_t xq[];  // [ROWS][pitch]
     __shared__ uint32_t part[ROWS][GV_WARPS];
+    __shared__ int sums[ROWS][GV_CHANNELS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     ptx::launch_dependents();
+    const int first = (int)((int64_t)out * blockIdx.x / gridDim.x);
+    const int channels = (int)((int64_t)out * (blockIdx.x + 1) / gridDim.x) - first;
+    if (lane == 0) {
+        // while the kernel ahead finishes, the head of this block's weights comes as far as L2
+        const int64_t bytes = min((int64_t)channels * pitch, (int64_t)GV_AHEAD_BYTES), at = (int64_t)warp * (GV_AHEAD_BYTES / GV_WARPS);
+        if (at < bytes)
+            ptx::prefetch_l2(wq + (int64_t)first * pitch + at, (uint32_t)min(bytes - at, (int64_t)(GV_AHEAD_BYTES / GV_WARPS)));
+    }
     ptx::dependency_wait();
-    const int step = GV_WARPS * gridDim.x;
-    int n = warp * gridDim.x + blockIdx.x, at = lane * 16;
-    int4 w[GV_LOADS];
-    auto fetch = [&]() {
-        const int8_t* src = wq + (int64_t)n * pitch + at;
-#pragma unroll
-        for (int j = 0; j < GV_LOADS; ++j) w[j] = n < out && at + j * 512 < pitch ? ld_weights(src + j * 512) : make_int4(0, 0, 0, 0);
+    const int pieces = (pitch + GV_PIECE - 1) / GV_PIECE;
+    const int row_step = GV_WARPS / pieces, piece_step = GV_WARPS % pieces;
+    int4 w[2][GV_LOADS];
+    // the piece to fetch next, and the piece to multiply next: numbered row by row, every 32nd is this warp's
+    int fr = warp / pieces, fp = warp % pieces, mr = fr, mp = fp;
+    auto advance = [&](int& r, int& p) {
+        r += row_step;
+        p += piece_step;
+        if (p >= pieces) { p -= pieces; ++r; }
     };
-    fetch();
+    auto fetch = [&](int4 (&dst)[GV_LOADS]) {
+        const int at = fp * GV_PIECE + lane * 16;
+        const int8_t* src = wq + (int64_t)(first + fr) * pitch + at;
+#pragma unroll
+        for (int j = 0; j < GV_LOADS; ++j)
+            dst[j] = fr < channels && at + j * 512 < pitch ? ld_weights(src + j * 512) : make_int4(0, 0, 0, 0);
+        advance(fr, fp);
+    };
+    fetch(w[0]);
+    fetch(w[1]);
+    for (int i = threadIdx.x; i < ROWS * GV_CHANNELS; i += GV_THREADS) (&sums[0][0])[i] = 0;
 
     // the tokens, quantised
     uint32_t top[ROWS];
@@ -518,39 +545,42 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
     }
     __syncthreads();
 
-    int acc[ROWS];
+    auto multiply = [&](const int4 (&v)[GV_LOADS]) {
+        const int at = mp * GV_PIECE + lane * 16;
+        int acc[ROWS];
 #pragma unroll
-    for (int t = 0; t < ROWS; ++t) acc[t] = 0;
-    while (n < out) {
+        for (int t = 0; t < ROWS; ++t) acc[t] = 0;
 #pragma unroll
         for (int j = 0; j < GV_LOADS; ++j)
             if (at + j * 512 < pitch) {
 #pragma unroll
                 for (int t = 0; t < ROWS; ++t) {
-                    const int4 v = *reinterpret_cast<const int4*>(xq + t * pitch + at + j * 512);
-                    acc[t] = __dp4a(w[j].x, v.x, acc[t]);
-                    acc[t] = __dp4a(w[j].y, v.y, acc[t]);
-                    acc[t] = __dp4a(w[j].z, v.z, acc[t]);
-                    acc[t] = __dp4a(w[j].w, v.w, acc[t]);
+                    const int4 q = *reinterpret_cast<const int4*>(xq + t * pitch + at + j * 512);
+                    acc[t] = __dp4a(v[j].x, q.x, acc[t]);
+                    acc[t] = __dp4a(v[j].y, q.y, acc[t]);
+                    acc[t] = __dp4a(v[j].z, q.z, acc[t]);
+                    acc[t] = __dp4a(v[j].w, q.w, acc[t]);
                 }
             }
-        const int row = n;
-        at += GV_PIECE;
-        const bool whole = at - lane * 16 >= pitch;
-        if (whole) {
-            at = lane * 16;
-            n += step;
-        }
-        fetch();
-        if (whole) {
-            const float cs = ws[row], cb = bias != nullptr ? as_f32(bias[row]) : 0.0f;
 #pragma unroll
-            for (int t = 0; t < ROWS; ++t) {
-                const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
-                if (lane == t) y[(int64_t)t * out + row] = (T)int8_out(sum, xs[t], cs, cb);
-                acc[t] = 0;
-            }
+        for (int t = 0; t < ROWS; ++t) {
+            const int sum = __reduce_add_sync(0xffffffffu, acc[t]);
+            if (lane == 0) atomicAdd(&sums[t][mr], sum);
         }
+        advance(mr, mp);
+    };
+    while (mr < channels) {
+        multiply(w[0]);
+        fetch(w[0]);
+        if (mr >= channels) break;
+        multiply(w[1]);
+        fetch(w[1]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < channels; i += GV_THREADS) {
+        const float cs = ws[first + i], cb = bias != nullptr ? as_f32(bias[first + i]) : 0.0f;
+#pragma unroll
+        for (int t = 0; t < ROWS; ++t) y[(int64_t)t * out + first + i] = (T)int8_out(sums[t][i], xs[t], cs, cb);
     }
 }
 
@@ -956,7 +986,9 @@ static int launch_stream(const void* x, int64_t ld, const int8_t* wq, const floa
     const int smem = ROWS * pitch;
     auto kern = int8_stream_kernel<T, ROWS>;
     SF_I8_SMEM(kern, GV_X_BYTES);
-    const int grid = (int)std::min<int64_t>(sm_count(), (out + GV_WARPS - 1) / GV_WARPS);
+    // one block per SM; fewer where that leaves a warp less than a piece, more where a block's channels would not fit
+    const int64_t pieces = out * ((pitch + GV_PIECE - 1) / GV_PIECE);
+    const int grid = (int)std::max(std::min<int64_t>(sm_count(), (pieces + GV_WARPS - 1) / GV_WARPS), (out + GV_CHANNELS - 2) / (GV_CHANNELS - 1));
     SF_CHECK_CUDA(launch_dependent(kern, grid, GV_THREADS, smem, 1, true, st, (const T*)x, ld, wq, ws, (const T*)bias, (T*)y, (int)in,
                                    (int)out, pitch, vec ? 1 : 0));
     return SF_OK;

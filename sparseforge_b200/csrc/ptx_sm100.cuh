@@ -211,6 +211,11 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
                  ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar)
                  : "memory");
 }
+// Asks for `bytes` (a multiple of 16, from a 16-byte boundary) to be brought into L2. Nothing reaches the SM: harmless
+// whatever another kernel does to the bytes meanwhile.
+__device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 // Programmatic dependent launch: the next kernel of the stream may be set up from here on / wait until the
 // kernel before this one is done and its results are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

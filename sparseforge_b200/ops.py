@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from ._lib import SF_BF16, SF_F32, SF_I8, check, lib
 
-_GET_DTYPE, _GET_SHAPE = torch.Tensor.dtype.__get__, torch.Tensor.shape.__get__
+_GET_DTYPE = torch.Tensor.dtype.__get__
 _GRAD_DTYPES = {torch.float32, torch.bfloat16}
 _DT = {torch.float32: SF_F32, torch.bfloat16: SF_BF16, torch.int8: SF_I8}
 
@@ -463,12 +463,12 @@ def _clip_arrays(grads, out, what):
     out = list(out)
     if len(out) != len(grads):
         raise ValueError(f"{what}: {len(grads)} gradients, {len(out)} outputs")
-    optrs, _, ocodes, odense = _grad_arrays(out, what)
-    if out[0].device != grads[0].device:
+    optrs, osizes, ocodes, odense = _grad_arrays(out, what)
+    if out[0].get_device() != grads[0].get_device():
         raise ValueError(f"{what}: outputs must live on the gradients' device")
-    if list(map(_GET_SHAPE, out)) != list(map(_GET_SHAPE, grads)) or (
-            not (dense and odense) and any(o.stride() != g.stride() for g, o in zip(grads, out))):
-        raise ValueError(f"{what}: an output must have its gradient's shape and strides")
+    if osizes != sizes or (not (dense and odense) and any(o.shape != g.shape or o.stride() != g.stride()
+                                                          for g, o in zip(grads, out))):
+        raise ValueError(f"{what}: an output must have its gradient's size, and its shape and strides unless all are contiguous")
     return ptrs, optrs, sizes, codes, ocodes
 
 
@@ -497,14 +497,15 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
     with _on_device_of(grads[0]):
         norm = torch.empty((), dtype=torch.float32, device=grads[0].device)
         scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=grads[0].device)
-        check(lib().sf_grad_norm(_addr(ptrs), _addr(sizes), _addr(codes), n, kind, _p(norm), _p(scratch), _raw_stream(grads[0].get_device())), "sf_grad_norm")
+        check(lib().sf_grad_norm(_addr(ptrs), _addr(sizes), _addr(codes), n, kind, _p(norm), _p(scratch),
+                                 _raw_stream(grads[0].get_device())), "sf_grad_norm")
     return norm
 
 
 def clip_grads(grads, norm, max_norm, out=None) -> None:
     """``out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))`` with ``norm`` an fp32 scalar on the device (for
-    example ``grad_norm``'s, or one combined over ranks). In place without ``out``; an output may have the other
-    of the two dtypes (bf16 gradients from fp32 accumulators)."""
+    example ``grad_norm``'s, or one combined over ranks). In place without ``out``; an output has its gradient's
+    number of elements and may have the other of the two dtypes (bf16 gradients from fp32 accumulators)."""
     grads = list(grads)
     if not grads:
         return
