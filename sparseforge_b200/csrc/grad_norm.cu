@@ -335,10 +335,11 @@ struct GnSpan {
     int writes;
 };
 static int gn_check_overlap(const char* who, const void* const* grads, void* const* outs, const int64_t* sizes,
-                            const int32_t* in_dt, const int32_t* out_dt, int64_t count) {
+                            const int32_t* in_dt, const int32_t* out_dt, int64_t count, const float* norm, int norm_written) {
     GnSpan* sp = new (std::nothrow) GnSpan[2 * count + 1];
     if (!sp) return fail(SF_ERR_BAD_ARG, "%s: out of host memory", who);
     int64_t k = 0;
+    sp[k++] = GnSpan{reinterpret_cast<uintptr_t>(norm), reinterpret_cast<uintptr_t>(norm) + 4, norm_written};
     for (int64_t i = 0; i < count; ++i) {
         if (sizes[i] == 0) continue;
         const uintptr_t o = reinterpret_cast<uintptr_t>(outs[i]), g = reinterpret_cast<uintptr_t>(grads[i]);
@@ -354,7 +355,7 @@ static int gn_check_overlap(const char* who, const void* const* grads, void* con
         if (sp[i].writes) out_end = std::max(out_end, sp[i].end);
     }
     delete[] sp;
-    if (bad) return fail(SF_ERR_BAD_ARG, "%s: an output overlaps another tensor of the call (the same gradient twice?)", who);
+    if (bad) return fail(SF_ERR_BAD_ARG, "%s: an output overlaps another tensor of the call or the norm (the same gradient twice?)", who);
     return SF_OK;
 }
 
@@ -496,19 +497,19 @@ int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* 
     return SF_OK;
 }
 
-static int clip_impl(const char* who, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dt,
-                     const int32_t* out_dt, int64_t count, double max_norm) {
+static int clip_check(const char* who, const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dt,
+                     const int32_t* out_dt, int64_t count, double max_norm, const float* norm, int norm_written) {
     if (int rc = gn_check(who, grads, sizes, in_dt, count)) return rc;
+    if (!norm) return fail(SF_ERR_BAD_ARG, "%s: norm must be non-null", who);
     if (count > 0 && (!outs || !out_dt)) return fail(SF_ERR_BAD_ARG, "%s: outs and their dtypes must be non-null", who);
     if (int rc = gn_check(who, const_cast<const void* const*>(outs), sizes, out_dt, count)) return rc;
     if (!(max_norm >= 0.0)) return fail(SF_ERR_BAD_ARG, "%s: max_norm must not be negative or NaN", who);
-    return gn_check_overlap(who, grads, outs, sizes, in_dt, out_dt, count);
+    return gn_check_overlap(who, grads, outs, sizes, in_dt, out_dt, count, norm, norm_written);
 }
 
 int sf_clip_grads(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dtypes,
                   const int32_t* out_dtypes, int64_t count, const float* norm, double max_norm, void* stream) {
-    if (int rc = clip_impl("sf_clip_grads", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm)) return rc;
-    SF_CHECK_ARG(norm != nullptr, "sf_clip_grads: norm must be non-null");
+    if (int rc = clip_check("sf_clip_grads", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm, norm, 0)) return rc;
     if (count == 0) return SF_OK;
     return gn_scale(grads, outs, sizes, in_dtypes, out_dtypes, count, nullptr, 0, GN_L2, norm, nullptr, max_norm,
                     (cudaStream_t)stream);
@@ -517,9 +518,9 @@ int sf_clip_grads(const void* const* grads, void* const* outs, const int64_t* si
 int sf_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes, const int32_t* in_dtypes,
                       const int32_t* out_dtypes, int64_t count, int kind, double max_norm, float* norm, double* scratch,
                       void* stream) {
-    if (int rc = clip_impl("sf_clip_grad_norm", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm)) return rc;
+    if (int rc = clip_check("sf_clip_grad_norm", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm, norm, 1)) return rc;
     SF_CHECK_ARG(kind == GN_L2 || kind == GN_INF, "sf_clip_grad_norm: kind must be SF_NORM_L2 or SF_NORM_INF");
-    SF_CHECK_ARG(norm && scratch, "sf_clip_grad_norm: norm and scratch must be non-null");
+    SF_CHECK_ARG(scratch != nullptr, "sf_clip_grad_norm: scratch must be non-null");
     cudaStream_t st = (cudaStream_t)stream;
     int slots = 0;
     if (int rc = gn_partials(grads, sizes, in_dtypes, count, kind, scratch, &slots, st)) return rc;

@@ -844,7 +844,7 @@ static bool takes_stream(int64_t rows, int64_t in) { return rows <= GV_MAX_ROWS 
 
 static int check_int8(const char* who, int64_t rows, int64_t in, int64_t out) {
     if (rows < 0 || in <= 0 || out <= 0) return fail(SF_ERR_BAD_ARG, "%s: rows must not be negative, in and out positive", who);
-    if (rows > 0x7fffff00 || out > 0x7fffff00) return fail(SF_ERR_UNSUPPORTED, "%s: dimension beyond 2^31", who);
+    if (rows > (1 << 30) || out > (1 << 30)) return fail(SF_ERR_UNSUPPORTED, "%s: rows or out beyond 2^30", who);
     if (in > SF_INT8_MAX_IN)
         return fail(SF_ERR_UNSUPPORTED, "%s: in=%lld: beyond %lld the 32-bit sum of 8-bit products could overflow", who,
                     (long long)in, (long long)SF_INT8_MAX_IN);

@@ -197,6 +197,8 @@ def test_refusals():
         ops.clip_grad_norm([a, b], 1.0, out=[b, a])
     with pytest.raises(RuntimeError, match="overlaps"):
         ops.clip_grad_norm([a[:2048]], 1.0, out=[a.view(torch.bfloat16)[:2048]])
+    with pytest.raises(RuntimeError, match="norm"):
+        ops.clip_grads([a, b], a[7], 1.0)
     assert abs(float(ops.grad_norm([a, a])) - math.sqrt(2.0) * _exact([a])) <= 2 * NORM_TOL * _exact([a, a])  # reading twice is fine
     with pytest.raises(TypeError):
         ops.grad_norm([a.half()])

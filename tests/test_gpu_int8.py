@@ -199,6 +199,28 @@ def test_linear_at_real_sizes(T, k, n, dtype):
     assert torch.equal(ops.int8_linear(x[T - 1:], wq, ws, b), y[T - 1:])
 
 
+# every tile shape and every cut of the reduction that the sizes select, ragged in all three directions: tokens x channels
+# of 16, 32, 64 columns in 1, 2, 4, 8 parts, two tokens' worth of 64-token tiles, 256 x 256 tiles in 1 and 2 parts, persistent ones
+PATHS = [(3, 200, 100), (9, 300, 129), (13, 1000, 4100), (16, 2100, 1000), (20, 129, 40), (29, 5000, 2000), (33, 4200, 300),
+         (64, 9000, 500), (70, 4100, 4000), (130, 700, 3000), (190, 11008, 1100), (255, 4109, 1300), (256, 8300, 4111),
+         (258, 8200, 700), (300, 9001, 261), (400, 11008, 2500), (513, 8193, 4001), (600, 3001, 1700), (700, 640, 6001),
+         (1030, 1601, 5003), (2050, 777, 3001), (5000, 130, 300)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T,k,n", PATHS)
+def test_every_tile_shape(T, k, n, dtype):
+    ops = _ops()
+    x, w, b = _inputs(T, k, n, DT[dtype], True, seed=4)
+    wq, ws = ops.int8_quantize_rows(w)
+    want, mag = _exact(x, w, b)
+    xq, xs = ops.int8_quantize_rows(x)
+    for rep in range(3):  # parts join in whatever order they finish
+        y = ops.int8_linear(x, wq, ws, b)
+        _check(y, want, mag, DT[dtype])
+        assert torch.equal(y, ops.int8_gemm(xq, xs, wq, ws, b, out_dtype=DT[dtype]))
+
+
 @pytest.mark.parametrize("T", [1, 4, 9, 40, 300])
 def test_extreme_integers(T):
     """-128 and 127 everywhere, at the largest reduction: the 32-bit sum is exact to its end."""

@@ -343,6 +343,7 @@ def test_gradient_clipping_refusals_without_a_gpu():
     part = (ctypes.c_void_p * 2)(4096, 4096 + 32)
     assert lib.sf_clip_grads(part, part, S, D, D, 2, 16, 1.0, None) == -1  # 16 floats reach 64 bytes
     far = (ctypes.c_void_p * 2)(4096, 8192)
+    assert lib.sf_clip_grads(far, far, S, D, D, 2, 8192 + 60, 1.0, None) == -1  # the norm inside a gradient that is written
     swapped = (ctypes.c_void_p * 2)(8192, 4096)
     assert lib.sf_clip_grads(far, swapped, S, D, D, 2, 16, 1.0, None) == -1
     assert lib.sf_clip_grads(far, far, S, D, D, 2, 16, -1.0, None) == -1
@@ -378,6 +379,8 @@ def test_int8_refusals_without_a_gpu():
     assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, 1, 8, 0, None, None) == -1
     assert lib.sf_int8_gemm(A + 1, A, A, A, None, A, _lib.SF_BF16, 1, 8, 8, None, None) == -3
     assert lib.sf_int8_gemm(A, None, A, A, None, A, _lib.SF_BF16, 1, 8, 8, None, None) == -1
+    assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, (1 << 30) + 1, 8, 8, None, None) == -2
+    assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, 1, 8, (1 << 30) + 1, None, None) == -2
     assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_I8, 1, 8, 8, A, None, None) == -1
     assert lib.sf_int8_linear(A, 4, A, A, None, A, _lib.SF_F32, 8, 8, 8, A, None, None) == -1
     assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_F32, 8, 8, 8, None, None, None) == -1  # workspace missing
