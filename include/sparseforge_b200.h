@@ -544,7 +544,7 @@ SF_API int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const flo
  * at all gives norm 0. An infinite or NaN gradient makes the norm so; clipping by a NaN norm makes every output NaN, by
  * an infinite one 0 (NaN where the gradient is infinite), as the reference's does.
  * An output is its own input (clipping in place; with c = 1 it is left alone) or overlaps no other tensor of
- * the call; a call that breaks this, for example by naming a gradient twice, is refused.
+ * the call, nor the norm; a call that breaks this, for example by naming a gradient twice, is refused.
  * sf_clip_grads takes the norm from the device (for example combined over ranks first); sf_clip_grad_norm forms it
  * and clips in one call, with the coefficient taken from the unrounded norm.
  */
