@@ -777,18 +777,18 @@ def int8_linear(x2d, wq, w_scale, bias=None, status=None):
     (``int8_quantize_rows``) and multiplied in 8 bits (``int8_gemm``)."""
     ld = _int8_rows(x2d, "int8_linear")
     T, k = x2d.shape
-    dtype, dev = x2d.dtype, x2d.device
-    out = _int8_weight(wq, w_scale, bias, k, dtype, dev.index, "int8_linear")
-    y = torch.empty((T, out), dtype=dtype, device=dev)
+    dtype, dev = x2d.dtype, x2d.get_device()
+    out = _int8_weight(wq, w_scale, bias, k, dtype, dev, "int8_linear")
+    y = x2d.new_empty((T, out))
     if T == 0:
         return y
     h = lib()
     # a workspace of its own per call: calls on two streams, or in two captured graphs, never share one
     nbytes = h.sf_int8_linear_workspace_bytes(T, k)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    ws = wq.new_empty(nbytes) if nbytes else None
     with _on_device_of(x2d):
         rc = h.sf_int8_linear(x2d.data_ptr(), ld, wq.data_ptr(), w_scale.data_ptr(), _p(bias), y.data_ptr(), _DT[dtype],
-                              T, k, out, _p(ws), _p(status), _raw_stream(dev.index))
+                              T, k, out, _p(ws), _p(status), _raw_stream(dev))
     if rc:
         check(rc, "sf_int8_linear")
     return y
