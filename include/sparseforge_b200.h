@@ -516,7 +516,7 @@ SF_API int sf_kl_div_bwd(const void* student, const void* teacher, int dtype, co
  *     [out, pitch] with zero padding beyond `in`, bias (or NULL) and y [rows, out] of `dtype`. The sum is an exact
  *     32-bit integer (in <= SF_INT8_MAX_IN), the rest fp32 with one rounding to y: a row's values do not depend on the other rows.
  *   sf_int8_linear: both, for x of y's dtype (rows of stride ld); workspace of sf_int8_linear_workspace_bytes
- *     bytes (may be 0: few rows need none), 16-byte aligned, holds nothing between calls; calls that may run at
+ *     bytes (may be 0: one or two rows need none), 16-byte aligned, holds nothing between calls; calls that may run at
  *     the same time need one each.
  * Any rows >= 0, in and out >= 1. 8-bit operands are 16-byte aligned. status as in sf_masked_gemm_fwd.
  */
@@ -526,7 +526,7 @@ SF_API int sf_int8_quantize_rows(const void* x, int dtype, int64_t ld, int8_t* q
                           void* stream);
 SF_API int sf_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq, const float* w_scale, const void* bias,
                  void* y, int dtype, int64_t rows, int64_t in, int64_t out, int32_t* status, void* stream);
-SF_API int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out);
+SF_API int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in);
 SF_API int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_scale, const void* bias, void* y,
                    int dtype, int64_t rows, int64_t in, int64_t out, void* workspace, int32_t* status, void* stream);
 

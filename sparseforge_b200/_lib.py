@@ -69,7 +69,7 @@ _SIGNATURES = {
     "sf_int8_pitch": (c_int64, [c_int64]),
     "sf_int8_quantize_rows": (c_int, [_P, c_int, c_int64, _P, _P, c_int64, c_int64, _P]),
     "sf_int8_gemm": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P]),
-    "sf_int8_linear_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "sf_int8_linear_workspace_bytes": (c_int64, [c_int64, c_int64]),
     "sf_int8_linear": (c_int, [_P, c_int64, _P, _P, _P, _P, c_int, c_int64, c_int64, c_int64, _P, _P, _P]),
     "sf_grad_norm_scratch_doubles": (c_int64, [c_int64]),
     "sf_grad_norm": (c_int, [_P, _P, _P, c_int64, c_int, _P, _P, _P]),

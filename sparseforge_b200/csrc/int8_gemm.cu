@@ -68,15 +68,6 @@ struct Raw8;
 template <>
 struct Raw8<__nv_bfloat16> {
     uint4 v;
-    __device__ __forceinline__ void clear() { v = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void load_some(const __nv_bfloat16* p, int n) {  // the first n of eight, the rest zero
-        const unsigned short* u = reinterpret_cast<const unsigned short*>(p);
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = (2 * i < n ? (uint32_t)__ldg(u + 2 * i) : 0u) | (2 * i + 1 < n ? (uint32_t)__ldg(u + 2 * i + 1) << 16 : 0u);
-        v = make_uint4(w[0], w[1], w[2], w[3]);
-    }
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
     __device__ __forceinline__ void unpack(float (&x)[8]) const {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -90,11 +81,6 @@ struct Raw8<__nv_bfloat16> {
 template <>
 struct Raw8<float> {
     float4 a, b;
-    __device__ __forceinline__ void clear() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ __forceinline__ void load_some(const float* p, int n) {
-        a = make_float4(n > 0 ? __ldg(p) : 0.f, n > 1 ? __ldg(p + 1) : 0.f, n > 2 ? __ldg(p + 2) : 0.f, n > 3 ? __ldg(p + 3) : 0.f);
-        b = make_float4(n > 4 ? __ldg(p + 4) : 0.f, n > 5 ? __ldg(p + 5) : 0.f, n > 6 ? __ldg(p + 6) : 0.f, n > 7 ? __ldg(p + 7) : 0.f);
-    }
     __device__ __forceinline__ void load(const float* p) {
         a = __ldg(reinterpret_cast<const float4*>(p));
         b = __ldg(reinterpret_cast<const float4*>(p) + 1);
@@ -610,20 +596,15 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
 // PAIR = 2 (more than 64 tokens): two CTAs share a 256-row tile (cta_group::2), each loads half of the tokens, 24 KiB per
 // stage instead of 32 for the same products: above 64 tokens the traffic into the SMs is what bounds the tile.
 // The weight loads of the first stages are issued before the kernel waits for the quantised rows.
-// FUSED (up to 32 tokens, no quantiser before the kernel): a CTA reads its K range of the tokens themselves, finds each
-// token's largest magnitude over the range, the cluster exchanges them, and the CTA writes its quantised range into
-// shared memory in the layout of a swizzled load. One launch instead of two: called back to back, the product's wait
-// for the quantiser alone took 1.9 us and the quantiser 1.1. The weights come as far as L2 while the kernel waits
-// for the one ahead of it, whatever that is.
 // ---------------------------------------------------------------------------------------------------------
-constexpr int I8_TAIL_BYTES = 2048;  // barriers and scales; keeps what follows on a 1024-byte boundary
-template <int BN, int PAIR, bool FUSED>
+template <int BN, int PAIR>
 struct I8Few {
-    static constexpr int STAGES = BN > 128 ? 6 : (BN * PAIR <= 32 && !FUSED ? 5 : 4);  // up to 64 tokens two CTAs per SM
+    static constexpr int STAGES = BN > 128 ? 6 : (BN * PAIR <= 32 ? 5 : 4);  // up to 128 tokens 94 to 104 KB: two CTAs per SM
     static constexpr int X_ROWS = BN / PAIR;
-    static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + (FUSED ? 0 : X_ROWS * I8_BK);
+    static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_ROWS * I8_BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + I8_TAIL_BYTES;  // FUSED: and the quantised tokens
+    static constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256 + 1024;
+    static constexpr int MAX_SPLIT = PAIR == 2 ? 2 : 8;  // clusters of at most eight CTAs, of four where one fills an SM
     static_assert(128 * BN * 4 <= STAGES * STAGE_BYTES, "partial sums reuse the ring");
 };
 
@@ -635,8 +616,6 @@ struct I8FewTail {
     uint32_t tmem_base;
     int abort_flag;
     float xs[256];  // scales of the tile's tokens
-    uint32_t top[32];     // FUSED: largest magnitudes over this CTA's range of K, as bit patterns
-    uint32_t all_top[32]; // ... over all of it
 };
 
 // Four consecutive output channels of one token.
@@ -660,31 +639,17 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vali
     }
 }
 
-// The tokens as the user has them (FUSED).
-template <typename T>
-struct RawTokens {
-    const T* x;
-    int64_t ld;
-    int in;
-    int vec;
-};
-constexpr int I8_AHEAD_BOXES = 8;  // 16 KiB boxes of weights a CTA brings into L2 while it waits
-
-template <typename T, int BN, int PAIR, bool FUSED>
+template <typename T, int BN, int PAIR>
 __global__ void __launch_bounds__(I8_THREADS, BN > 128 ? 1 : 2)
-int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const RawTokens<T> raw,
+int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                 const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
                 int rows, int out, int pitch, int split, int tiles_t, int32_t* status) {
-    static_assert(!FUSED || (PAIR == 1 && BN <= 32), "quantising in place: up to 32 tokens, single CTAs");
-    using C = I8Few<BN, PAIR, FUSED>;
+    using C = I8Few<BN, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = ptx::smem_u32(smem_raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw_addr);
     auto* tail = reinterpret_cast<I8FewTail<C::STAGES>*>(base_ptr + C::STAGES * C::STAGE_BYTES);
-    // FUSED: [blocks of K][BN][128 bytes], behind the tail
-    uint8_t* xtile = base_ptr + C::STAGES * C::STAGE_BYTES + I8_TAIL_BYTES;
-    static_assert(sizeof(I8FewTail<C::STAGES>) <= I8_TAIL_BYTES, "the tail fits its room");
     volatile int* abort_flag = &tail->abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -713,7 +678,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                 ptx::mbar_arrive_expect_tx(local, C::STAGE_BYTES);
                 ptx::tma_load_2d(sw, &tmW, local, kb * I8_BK, n0);
             }
-            if (tokens && !FUSED) ptx::tma_load_2d(sx, &tmX, local, kb * I8_BK, t0);
+            if (tokens) ptx::tma_load_2d(sx, &tmX, local, kb * I8_BK, t0);
         }
     };
     if (threadIdx.x == 0) {
@@ -724,12 +689,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         ptx::mbar_init(ptx::smem_u32(&tail->tmem_full), 1);
         tail->abort_flag = 0;
         ptx::fence_barrier_init();
-        if (FUSED)
-            for (int kb = kb0; kb < min(kb1, kb0 + I8_AHEAD_BOXES); ++kb) ptx::tma_prefetch_2d(&tmW, kb * I8_BK, n0);
-        else if (PAIR == 1)  // nobody else's barriers are involved: the weights are on their way before the block is set up
+        if (PAIR == 1)  // nobody else's barriers are involved: the weights are on their way before the block is set up
             for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
     }
-    if (FUSED && threadIdx.x >= 32 && threadIdx.x < 64) tail->top[threadIdx.x - 32] = 0;
     if (warp == 1) {
         if (PAIR == 2) {
             ptx::tmem_alloc_pair(ptx::smem_u32(&tail->tmem_base), C::TMEM_COLS);
@@ -746,69 +708,11 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     ptx::launch_dependents();
     const uint32_t tmem_base = tail->tmem_base;
 
-    if (FUSED) {
-        ptx::dependency_wait();
-        if (threadIdx.x == 0)
-            for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
-        __syncwarp();
-        // groups of eight elements, numbered token by token; 16 (one 128-byte row of a block) always share a token
-        const int groups = (kb1 - kb0) * (I8_BK / 8), tokens = min(BN, rows - t0), total = tokens * groups;
-        const T* x0 = raw.x + (int64_t)t0 * raw.ld + kb0 * I8_BK;
-        const int left = raw.in - kb0 * I8_BK;  // elements from this range's start to the row's end
-        constexpr int BATCH = 4;                // groups whose loads are in flight together
-        auto each = [&](auto&& use) {
-            for (int i0 = threadIdx.x; i0 - lane < total; i0 += BATCH * I8_THREADS) {
-                Raw8<T> r[BATCH];
-#pragma unroll
-                for (int b = 0; b < BATCH; ++b) {
-                    const int i = i0 + b * I8_THREADS, t = i / groups, k = (i - t * groups) * 8;
-                    const T* src = x0 + t * raw.ld + k;
-                    r[b].clear();
-                    if (i < total) {
-                        if (raw.vec && k + 8 <= left) r[b].load(src);
-                        else r[b].load_some(src, left - k);
-                    }
-                }
-#pragma unroll
-                for (int b = 0; b < BATCH; ++b) {
-                    const int i = i0 + b * I8_THREADS, t = i / groups;
-                    use(r[b], i, t, i - t * groups);
-                }
-            }
-        };
-        each([&](const Raw8<T>& r, int i, int t, int) {
-            uint32_t m = top_bits(T(), top8(r, 0u));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            if ((lane & 15) == 0 && i < total) atomicMax(&tail->top[t], m);
-        });
-        __syncthreads();
-        if (split > 1) ptx::cluster_sync_all();
-        if (threadIdx.x < tokens) {
-            const uint32_t mine = ptx::smem_u32(&tail->top[threadIdx.x]);
-            uint32_t m = 0;
-            for (int s = 0; s < split; ++s) m = max(m, ptx::ld_shared_cluster_u32(clustered ? ptx::map_to_cta(mine, (uint32_t)s) : mine));
-            tail->all_top[threadIdx.x] = m;
-            tail->xs[threadIdx.x] = m < 0x7f800000u ? __fdiv_rn(__uint_as_float(m), 127.0f) : nan_f32();
-        }
-        __syncthreads();
-        each([&](const Raw8<T>& r, int i, int t, int g) {
-            if (i >= total) return;
-            const uint32_t m = tail->all_top[t];
-            const uint2 q = m < 0x7f800000u && m != 0 ? quantise8(r, row_scale<T>(__uint_as_float(m))) : make_uint2(0u, 0u);
-            // 128-byte swizzle: the 16-byte piece p of row t lies where piece p ^ (t mod 8) would
-            const int kb = g >> 4, piece = (g >> 1) & 7;
-            *reinterpret_cast<uint2*>(xtile + kb * (BN * I8_BK) + t * I8_BK + ((piece ^ (t & 7)) << 4) + (g & 1) * 8) = q;
-        });
-        ptx::fence_proxy_async();  // the tensor cores read what these stores wrote
-        __syncthreads();
-    }
-
     if (warp == 0) {
         if (PAIR == 2 && lane == 0)
             for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
         ptx::dependency_wait();
-        if (!FUSED && lane == 0)
+        if (lane == 0)
             for (int s = 0; s < ahead; ++s) load(s, kb0 + s, false, true);
         __syncwarp();
         int stage = 0;
@@ -833,8 +737,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             if (!ok) break;
             ptx::tc_fence_after();
             if (lane == 0) {
-                const uint32_t sw = base + stage * C::STAGE_BYTES;
-                const uint32_t sx = FUSED ? ptx::smem_u32(xtile) + (uint32_t)((kb - kb0) * (BN * I8_BK)) : sw + I8_OPERAND_BYTES;
+                const uint32_t sw = base + stage * C::STAGE_BYTES, sx = sw + I8_OPERAND_BYTES;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const uint64_t wd = ptx::make_smem_desc(sw + k * 32, 16, 1024, 2), xd = ptx::make_smem_desc(sx + k * 32, 16, 1024, 2);
@@ -867,8 +770,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     }
     ptx::dependency_wait();
     if (warp >= 2) {
-        if (!FUSED)
-            for (int c = threadIdx.x - 64; c < BN; c += 128) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
+        for (int c = threadIdx.x - 64; c < BN; c += 128) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
         const bool done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {
             ptx::tc_fence_after();
@@ -935,40 +837,6 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         if (PAIR == 2) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
         else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
     }
-}
-
-// Host side of the kernels for few rows: tiles, and how many parts their reduction is cut into.
-static int64_t few_tiles(int64_t rows, int64_t out, int bn, int pair) {
-    return (out + 128 * pair - 1) / (128 * pair) * ((rows + bn - 1) / bn);
-}
-// Doubled until most SMs stream weights, as long as every CTA keeps a block of K; and on to two CTAs per SM (tiles of up
-// to 64 tokens), whose loads cover each other's latencies, while each keeps 16 blocks: shorter parts cost more in the join
-// than they save ([64, 4096] x [4096, 4096]: 9.3 us with four parts of 8 blocks, 10.5 with eight of 4).
-static int few_split(int64_t tiles, int bn, int pair, int pitch) {
-    // clusters of at most eight CTAs; of four where one CTA fills an SM, since more would not all find their SMs at once
-    const int num_kb = (pitch + I8_BK - 1) / I8_BK, most = pair == 2 ? 2 : 8;
-    const int64_t sms = sm_count();
-    int split = 1;
-    while (split < most && 2 * split <= num_kb) {
-        const int64_t ctas = tiles * pair * split;
-        const bool idle = ctas * 4 < sms * (bn > 128 ? 2 : 3);
-        const bool room = bn <= 64 && ctas <= sms && num_kb >= 32 * split;
-        if (!idle && !room) break;
-        split *= 2;
-    }
-    return split;
-}
-// Shared memory a CTA needs for its quantised range of the tokens, and the most that leaves two CTAs per SM.
-static int few_token_bytes(int bn, int split, int pitch) {
-    const int num_kb = (pitch + I8_BK - 1) / I8_BK;
-    return (num_kb + split - 1) / split * bn * I8_BK;
-}
-constexpr int I8_FUSED_X_BYTES = 44 * 1024;
-// Up to 32 rows quantise their tokens in the product's own launch where a CTA's range of them fits.
-static bool takes_fused(int64_t rows, int64_t in, int64_t out) {
-    if (rows > 32) return false;
-    const int pitch = (int)((in + 15) / 16 * 16), bn = rows <= 16 ? 16 : 32;
-    return few_token_bytes(bn, few_split(few_tiles(rows, out, bn, 1), bn, 1, pitch), pitch) <= I8_FUSED_X_BYTES;
 }
 
 // One row or two, whose quantised form fits into shared memory, take the kernel without a workspace.
@@ -1085,38 +953,29 @@ static int launch_pair(const int8_t* xq, const float* xs, const int8_t* wq, cons
 template <typename T, int BN, int PAIR>
 static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const float* ws, const void* bias, void* y,
                       int64_t rows, int pitch, int64_t out, int32_t* status, bool dependent, cudaStream_t st) {
-    using C = I8Few<BN, PAIR, false>;
+    using C = I8Few<BN, PAIR>;
     CUtensorMap tmW, tmX;
     if (int rc = make_byte_tensor_map(&tmW, wq, pitch, out, 128)) return rc;
     if (int rc = make_byte_tensor_map(&tmX, xq, pitch, rows, C::X_ROWS)) return rc;
-    const int64_t tiles = few_tiles(rows, out, BN, PAIR);
+    const int64_t tiles_t = (rows + BN - 1) / BN, tiles = (out + 128 * PAIR - 1) / (128 * PAIR) * tiles_t;
     if (tiles * 8 > 0x7fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: too many tiles");
-    const int split = few_split(tiles, BN, PAIR, pitch);
-    auto kern = int8_few_kernel<T, BN, PAIR, false>;
+    // Doubled until most SMs stream weights, as long as every CTA keeps a block of K; and on to two CTAs per SM (tiles of up
+    // to 64 tokens), whose loads cover each other's latencies, while each keeps 16 blocks: shorter parts cost more in the join
+    // than they save ([64, 4096] x [4096, 4096]: 9.3 us with four parts of 8 blocks, 10.5 with eight of 4).
+    const int num_kb = (pitch + I8_BK - 1) / I8_BK;
+    const int64_t sms = sm_count();
+    int split = 1;
+    while (split < C::MAX_SPLIT && 2 * split <= num_kb) {
+        const int64_t ctas = tiles * PAIR * split;
+        const bool idle = ctas * 4 < sms * (BN > 128 ? 2 : 3);
+        const bool room = BN <= 64 && ctas <= sms && num_kb >= 32 * split;
+        if (!idle && !room) break;
+        split *= 2;
+    }
+    auto kern = int8_few_kernel<T, BN, PAIR>;
     SF_I8_SMEM(kern, C::SMEM);
-    const RawTokens<T> none = {};
     SF_CHECK_CUDA(launch_dependent(kern, (int)(tiles * PAIR * split), I8_THREADS, C::SMEM, PAIR * split, dependent, st, tmW, tmX,
-                                   none, xs, ws, (const T*)bias, (T*)y, (int)rows, (int)out, pitch, split,
-                                   (int)((rows + BN - 1) / BN), status));
-    return SF_OK;
-}
-
-template <typename T, int BN>
-static int launch_fused(const void* x, int64_t ld, const int8_t* wq, const float* ws, const void* bias, void* y, int64_t rows,
-                        int64_t in, int64_t out, bool vec, int32_t* status, cudaStream_t st) {
-    using C = I8Few<BN, 1, true>;
-    const int pitch = (int)((in + 15) / 16 * 16);
-    CUtensorMap tmW;
-    if (int rc = make_byte_tensor_map(&tmW, wq, pitch, out, 128)) return rc;
-    const int64_t tiles = few_tiles(rows, out, BN, 1);
-    if (tiles * 8 > 0x7fffffff) return fail(SF_ERR_UNSUPPORTED, "8-bit product: too many tiles");
-    const int split = few_split(tiles, BN, 1, pitch);
-    auto kern = int8_few_kernel<T, BN, 1, true>;
-    SF_I8_SMEM(kern, C::SMEM + I8_FUSED_X_BYTES);
-    const RawTokens<T> raw = {(const T*)x, ld, (int)in, vec ? 1 : 0};
-    SF_CHECK_CUDA(launch_dependent(kern, (int)(tiles * split), I8_THREADS, C::SMEM + few_token_bytes(BN, split, pitch), split, true, st,
-                                   tmW, tmW, raw, (const float*)nullptr, ws, (const T*)bias, (T*)y, (int)rows, (int)out, pitch,
-                                   split, 1, status));
+                                   xs, ws, (const T*)bias, (T*)y, (int)rows, (int)out, pitch, split, (int)tiles_t, status));
     return SF_OK;
 }
 
@@ -1202,8 +1061,8 @@ int sf_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq, const
     return gemm_impl(xq, x_scale, wq, w_scale, bias, y, dtype, rows, in, out, status, false, (cudaStream_t)stream);
 }
 
-int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in, int64_t out) {
-    if (rows <= 0 || in <= 0 || out <= 0 || in > SF_INT8_MAX_IN || takes_stream(rows, in) || takes_fused(rows, in, out)) return 0;
+int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in) {
+    if (rows <= 0 || in <= 0 || takes_stream(rows, in)) return 0;
     return rows * sf_int8_pitch(in) + rows * 4;
 }
 
@@ -1211,27 +1070,19 @@ int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_s
                    int64_t rows, int64_t in, int64_t out, void* workspace, int32_t* status, void* stream) {
     if (int rc = check_product("sf_int8_linear", wq, w_scale, y, dtype, rows, in, out)) return rc;
     if (rows == 0) return SF_OK;
-    const bool stream_rows = takes_stream(rows, in), fused = !stream_rows && takes_fused(rows, in, out);
-    SF_CHECK_ARG(x && (workspace || stream_rows || fused), "sf_int8_linear: x and workspace must be non-null");
+    const bool stream_rows = takes_stream(rows, in);
+    SF_CHECK_ARG(x && (workspace || stream_rows), "sf_int8_linear: x and workspace must be non-null");
     SF_CHECK_ARG(ld >= in || rows == 1, "sf_int8_linear: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(workspace)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: workspace must be 16-byte aligned");
-    const bool vec = rows_vectorise(x, dtype, ld, rows, in);
-    cudaStream_t st = (cudaStream_t)stream;
-    if (fused) {
-        if (rows <= 16)
-            return dtype == SF_F32 ? launch_fused<float, 16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, st)
-                                   : launch_fused<__nv_bfloat16, 16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, st);
-        return dtype == SF_F32 ? launch_fused<float, 32>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, st)
-                               : launch_fused<__nv_bfloat16, 32>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, status, st);
-    }
     if (stream_rows) {
-        return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, st)
-                               : stream_typed<__nv_bfloat16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, st);
+        const bool vec = rows_vectorise(x, dtype, ld, rows, in);
+        return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream)
+                               : stream_typed<__nv_bfloat16>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream);
     }
     int8_t* xq = static_cast<int8_t*>(workspace);
     float* xs = reinterpret_cast<float*>(xq + rows * sf_int8_pitch(in));
-    if (int rc = quantize_impl(x, dtype, ld, xq, xs, rows, in, st)) return rc;
-    return gemm_impl(xq, xs, wq, w_scale, bias, y, dtype, rows, in, out, status, true, st);
+    if (int rc = quantize_impl(x, dtype, ld, xq, xs, rows, in, (cudaStream_t)stream)) return rc;
+    return gemm_impl(xq, xs, wq, w_scale, bias, y, dtype, rows, in, out, status, true, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -79,10 +79,6 @@ __device__ __forceinline__ void tma_load_2d(uint32_t smem_dst, const CUtensorMap
         ::"r"(smem_dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
         : "memory");
 }
-// Brings the box that tma_load_2d would load as far as L2.
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int c0, int c1) {
-    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(c0), "r"(c1) : "memory");
-}
 __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
@@ -224,11 +220,6 @@ __device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
 // kernel before this one is done and its results are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ uint32_t ld_shared_cluster_u32(uint32_t cluster_addr) {
-    uint32_t v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(cluster_addr));
-    return v;
-}
 __device__ __forceinline__ int4 ld_shared_cluster_v4(uint32_t cluster_addr) {
     int4 v;
     asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];"

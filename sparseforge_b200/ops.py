@@ -784,7 +784,7 @@ def int8_linear(x2d, wq, w_scale, bias=None, status=None):
         return y
     h = lib()
     # a workspace of its own per call: calls on two streams, or in two captured graphs, never share one
-    nbytes = h.sf_int8_linear_workspace_bytes(T, k, out)
+    nbytes = h.sf_int8_linear_workspace_bytes(T, k)
     ws = wq.new_empty(nbytes) if nbytes else None
     with _on_device_of(x2d):
         rc = h.sf_int8_linear(x2d.data_ptr(), ld, wq.data_ptr(), w_scale.data_ptr(), _p(bias), y.data_ptr(), _DT[dtype],

@@ -284,7 +284,7 @@ def test_rows_behind_the_last_are_left_alone(T):
     wq, ws = ops.int8_quantize_rows(w)
     want = ops.int8_linear(x, wq, ws)
     y = torch.full((T + 2, n), 5.0, device="cuda", dtype=torch.bfloat16)
-    work = torch.empty(int(_lib.lib().sf_int8_linear_workspace_bytes(T, k, n)) or 16, dtype=torch.uint8, device="cuda")
+    work = torch.empty(int(_lib.lib().sf_int8_linear_workspace_bytes(T, k)) or 16, dtype=torch.uint8, device="cuda")
     rc = _lib.lib().sf_int8_linear(x.data_ptr(), k, wq.data_ptr(), ws.data_ptr(), None, y[1:].data_ptr(), _lib.SF_BF16, T, k, n,
                                    work.data_ptr(), None, torch.cuda.current_stream().cuda_stream)
     assert rc == 0

@@ -367,8 +367,8 @@ def test_int8_refusals_without_a_gpu():
 
     lib = _lib.lib()
     assert int(lib.sf_int8_pitch(1)) == 16 and int(lib.sf_int8_pitch(4096)) == 4096 and int(lib.sf_int8_pitch(1003)) == 1008
-    assert int(lib.sf_int8_linear_workspace_bytes(1, 4096, 4096)) == 0
-    assert int(lib.sf_int8_linear_workspace_bytes(100, 1003, 64)) == 100 * 1008 + 400
+    assert int(lib.sf_int8_linear_workspace_bytes(1, 4096)) == 0
+    assert int(lib.sf_int8_linear_workspace_bytes(16, 1003)) == 16 * 1008 + 64
     A = 4096
     assert lib.sf_int8_quantize_rows(A, _lib.SF_I8, 8, A, A, 1, 8, None) == -1
     assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 4, A, A, 2, 8, None) == -1      # rows overlap
@@ -383,7 +383,7 @@ def test_int8_refusals_without_a_gpu():
     assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, 1, 8, (1 << 30) + 1, None, None) == -2
     assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_I8, 1, 8, 8, A, None, None) == -1
     assert lib.sf_int8_linear(A, 4, A, A, None, A, _lib.SF_F32, 8, 8, 8, A, None, None) == -1
-    assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_F32, 80, 8, 8, None, None, None) == -1  # workspace missing
+    assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_F32, 8, 8, 8, None, None, None) == -1  # workspace missing
     assert lib.sf_int8_linear(A, 8, A, A, None, A, _lib.SF_F32, 8, 131057, 8, A, None, None) < 0
     assert b"ld=8" in lib.sf_last_error_string() or b"overflow" in lib.sf_last_error_string()
     x, q, s = torch.zeros(2, 8), torch.zeros(4, 16, dtype=torch.int8), torch.ones(4)
