@@ -39,8 +39,8 @@ struct GnTensor {
     void* out;
     int64_t n;
 };
-// kind bits of a table entry
-enum { GN_IN_BF16 = 1, GN_OUT_BF16 = 2, GN_VEC = 4, GN_IN_PLACE = 8 };
+// kind bits of a table entry; from bit 4 on: elements before the first one that is on a 16-byte boundary on both sides
+enum { GN_IN_BF16 = 1, GN_OUT_BF16 = 2, GN_VEC = 4, GN_IN_PLACE = 8, GN_HEAD_SHIFT = 4 };
 template <int CAP>
 struct GnTable {
     GnTensor t[CAP];
@@ -150,11 +150,13 @@ grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __res
         const int64_t at = (int64_t)(c - tab.first[ti]) * tab.chunk;
         const int len = (int)min((int64_t)tab.chunk, tab.t[ti].n - at);
         const int kind = tab.kind[ti];
-        const int nv = (kind & GN_VEC) ? len / kGnVec : 0;
+        // a chunk is a multiple of eight long, so every chunk of a tensor starts as far from a boundary as the first
+        const int head = min(len, kind >> GN_HEAD_SHIFT), nv = (kind & GN_VEC) ? (len - head) / kGnVec : 0;
         const bool keep = c >= tab.keep_from;
         if (kind & GN_IN_BF16) {
             const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(tab.t[ti].in) + at;
-            const uint4* q = reinterpret_cast<const uint4*>(p);
+            const uint4* q = reinterpret_cast<const uint4*>(p + head);
+#pragma unroll 1
             for (int v = threadIdx.x; v < nv; v += kGnNormBatch * kGnThreads) {
                 uint4 r[kGnNormBatch];  // loads of a batch are in flight together
 #pragma unroll
@@ -168,10 +170,13 @@ grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __res
                         acc8<MAXNORM>(acc, x);
                     }
             }
-            for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) acc1<MAXNORM>(acc, __bfloat162float(p[i]));
+#pragma unroll 1
+            for (int i = threadIdx.x; i < len - nv * kGnVec; i += kGnThreads)
+                acc1<MAXNORM>(acc, __bfloat162float(p[i < head ? i : i + nv * kGnVec]));
         } else {
             const float* p = static_cast<const float*>(tab.t[ti].in) + at;
-            const uint4* q = reinterpret_cast<const uint4*>(p);
+            const uint4* q = reinterpret_cast<const uint4*>(p + head);
+#pragma unroll 1
             for (int v = threadIdx.x; v < nv; v += kGnNormBatch / 2 * kGnThreads) {
                 uint4 r[kGnNormBatch];
 #pragma unroll
@@ -188,7 +193,8 @@ grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __res
                         acc8<MAXNORM>(acc, x);
                     }
             }
-            for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) acc1<MAXNORM>(acc, p[i]);
+#pragma unroll 1
+            for (int i = threadIdx.x; i < len - nv * kGnVec; i += kGnThreads) acc1<MAXNORM>(acc, p[i < head ? i : i + nv * kGnVec]);
         }
     }
     // the kernel behind this one may be set up meanwhile; it waits for these slots
@@ -247,12 +253,14 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
         if ((ent & GN_IN_PLACE) && c == 1.0f) continue;
         const int64_t at = (int64_t)(ch - tab.first[ti]) * tab.chunk;
         const int len = (int)min((int64_t)tab.chunk, tab.t[ti].n - at);
-        const int nv = (ent & GN_VEC) ? len / kGnVec : 0;
+        const int head = min(len, ent >> GN_HEAD_SHIFT), nv = (ent & GN_VEC) ? (len - head) / kGnVec : 0;
         const bool ib = ent & GN_IN_BF16, ob = ent & GN_OUT_BF16;
         const char* ip = static_cast<const char*>(tab.t[ti].in) + at * (ib ? 2 : 4);
         char* op = static_cast<char*>(tab.t[ti].out) + at * (ob ? 2 : 4);
+        const char* iv = ip + head * (ib ? 2 : 4);
+        char* ov = op + head * (ob ? 2 : 4);
         if (ib && ob) {
-            const uint4* q = reinterpret_cast<const uint4*>(ip);
+            const uint4* q = reinterpret_cast<const uint4*>(iv);
             for (int v = threadIdx.x; v < nv; v += kGnClipBatch * kGnThreads) {
                 uint4 r[kGnClipBatch];
 #pragma unroll
@@ -265,7 +273,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
                         unpack_bf16(r[u], x);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) x[i] *= c;
-                        Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(op) + (v + u * kGnThreads) * kGnVec, x);
+                        Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(ov) + (v + u * kGnThreads) * kGnVec, x);
                     }
             }
         } else {
@@ -275,7 +283,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
 #pragma unroll
                 for (int u = 0; u < U; ++u)
                     if (v + u * kGnThreads < nv) {
-                        const uint4* q = reinterpret_cast<const uint4*>(ip) + (ib ? 1 : 2) * (v + u * kGnThreads);
+                        const uint4* q = reinterpret_cast<const uint4*>(iv) + (ib ? 1 : 2) * (v + u * kGnThreads);
                         r[u][0] = ld_stream16(q);
                         if (!ib) r[u][1] = ld_stream16(q + 1);
                     }
@@ -288,12 +296,13 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restr
                         else unpack_f32(r[u][0], r[u][1], x);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) x[i] *= c;
-                        if (ob) Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(op) + at, x);
-                        else Vec8<float>::store(reinterpret_cast<float*>(op) + at, x);
+                        if (ob) Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(ov) + at, x);
+                        else Vec8<float>::store(reinterpret_cast<float*>(ov) + at, x);
                     }
             }
         }
-        for (int i = nv * kGnVec + threadIdx.x; i < len; i += kGnThreads) {
+        for (int j = threadIdx.x; j < len - nv * kGnVec; j += kGnThreads) {
+            const int i = j < head ? j : j + nv * kGnVec;
             const float x = (ib ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(ip)[i])
                                 : reinterpret_cast<const float*>(ip)[i]) * c;
             if (ob) reinterpret_cast<__nv_bfloat16*>(op)[i] = __float2bfloat16_rn(x);
@@ -385,9 +394,14 @@ static int64_t gn_fill(GnTable<CAP>& tab, const void* const* grads, void* const*
         void* o = outs ? outs[i] : nullptr;
         tab.t[k] = GnTensor{grads[i], o, sizes[i]};
         const int odt = out_dt ? out_dt[i] : in_dt[i];
-        tab.kind[k] = (uint8_t)((in_dt[i] == SF_BF16 ? GN_IN_BF16 : 0) | (odt == SF_BF16 ? GN_OUT_BF16 : 0) |
-                                (aligned16(grads[i]) && aligned16(o) ? GN_VEC : 0) |
-                                (o == grads[i] && odt == in_dt[i] ? GN_IN_PLACE : 0));
+        const int is = in_dt[i] == SF_BF16 ? 2 : 4, os = odt == SF_BF16 ? 2 : 4;
+        int head = 0;  // the first element that is on a 16-byte boundary on both sides, if there is one
+        while (head < 8 && ((reinterpret_cast<uintptr_t>(grads[i]) + head * is) % 16 ||
+                            (o && (reinterpret_cast<uintptr_t>(o) + head * os) % 16)))
+            ++head;
+        tab.kind[k] = (uint8_t)((is == 2 ? GN_IN_BF16 : 0) | (os == 2 ? GN_OUT_BF16 : 0) |
+                                (o == grads[i] && is == os ? GN_IN_PLACE : 0) |
+                                (head < 8 ? GN_VEC | head << GN_HEAD_SHIFT : 0));
         tab.all_in_place &= (tab.kind[k] & GN_IN_PLACE) != 0;
         tab.first[k] = c;
         c += (uint32_t)((sizes[i] + chunk - 1) / chunk);

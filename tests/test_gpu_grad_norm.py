@@ -62,7 +62,7 @@ def _set(name, **kw):
 
 
 @pytest.mark.parametrize("p", [2.0, math.inf])
-@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("offset", [0, 1, 6])
 @pytest.mark.parametrize("name", list(SETS))
 def test_norm(name, offset, p):
     grads = _set(name, seed=3, offset=offset)
@@ -113,7 +113,7 @@ def test_infinite_and_nan_gradients(bad, at, p):
 
 
 @pytest.mark.parametrize("p", [2.0, math.inf])
-@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("offset", [0, 3, 4])
 @pytest.mark.parametrize("mode", ["in_place", "same", "other"])
 @pytest.mark.parametrize("name", list(SETS))
 def test_clip(name, mode, offset, p):
@@ -299,3 +299,35 @@ def test_codes_of_the_c_entry_points():
     assert float(n) == 4.0
     assert lib.sf_grad_norm(None, None, None, 0, 0, n.data_ptr(), sc.data_ptr(), st) == 0
     assert float(n) == 0.0
+
+
+def test_a_tensor_of_more_than_2_to_the_31_elements():
+    ops = _ops()
+    n = (1 << 31) + 12345
+    g = torch.zeros(n, device="cuda", dtype=torch.bfloat16)
+    g[::1 << 20] = 1.0
+    g[-1] = 2.0
+    want = math.sqrt(float(len(range(0, n, 1 << 20))) + 4.0 - (1.0 if (n - 1) % (1 << 20) == 0 else 0.0))
+    norm = ops.clip_grad_norm([g], want / 4)
+    assert abs(float(norm) - want) <= NORM_TOL * want
+    assert float(g[-1]) == 0.5 and float(g[0]) == 0.25 and float(g[1 << 20]) == 0.25
+    assert float(ops.grad_norm([g[-5:], g], math.inf)) == 0.5
+
+
+@pytest.mark.parametrize("dt,odt", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
+def test_every_alignment(dt, odt):
+    """Gradients and outputs at every element offset from a 16-byte boundary, and lengths around the access sizes."""
+    ops = _ops()
+    src = torch.randn(9000, device="cuda").to(DT[dt])
+    for go in range(9):
+        for oo in (go, 0, 1, 3, 4, 7):
+            for n in (1, 2, 7, 8, 9, 15, 17, 4096, 8200):
+                g = src[go:go + n]
+                buf = torch.full((n + oo + 9,), 7.0, device="cuda", dtype=DT[odt])
+                o = buf[oo:oo + n]
+                norm = ops.clip_grad_norm([g], 0.5, out=[o])
+                w = _exact([g])
+                assert abs(float(norm) - w) <= NORM_TOL * w
+                ref = g.double() * min(1.0, 0.5 / (w + 1e-6))
+                assert ((o.double() - ref).abs() <= _value_tol(o.dtype) * ref.abs() + 1e-40).all(), (go, oo, n)
+                assert (buf[:oo] == 7.0).all() and (buf[oo + n:] == 7.0).all()

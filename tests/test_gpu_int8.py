@@ -325,3 +325,21 @@ def test_streams_and_graph_replay():
         torch.cuda.synchronize()
         for (x, wq, ws, b, _), (_, y) in zip(cases, graphs):
             assert torch.equal(y, ops.int8_linear(x, wq, ws, b))
+
+
+@pytest.mark.parametrize("T,k,n", [(280000, 40, 8000), (270000, 8200, 33), (1, 8192, 270000), (2, 8192, 270000), (20, 8192, 270000),
+                                   (64, 8192, 270000)])
+def test_offsets_beyond_32_bits(T, k, n):
+    """Outputs, inputs or weights of more than 2^31 bytes and elements: the last rows and channels are right."""
+    ops = _ops()
+    x = torch.randn(T, k, device="cuda", dtype=torch.bfloat16)
+    wq = torch.randint(-127, 128, (n, (k + 15) // 16 * 16), device="cuda", dtype=torch.int8)
+    wq[:, k:] = 0
+    ws = torch.rand(n, device="cuda") * 1e-2
+    y = ops.int8_linear(x, wq, ws)
+    q, s = _quantise64(x[-3:])
+    last = slice(max(0, n - 300), n)
+    raw = (q @ wq[last, :k].double().t()) * s[:, None] * ws[last].double()
+    _check(y[-3:, last].contiguous(), raw, raw.abs(), torch.bfloat16)
+    first = (q[:1] @ wq[:64, :k].double().t()) * s[:1, None] * ws[:64].double()
+    _check(y[-3 if T > 2 else -T:, :64][:1].contiguous(), first, first.abs(), torch.bfloat16)
