@@ -12,6 +12,9 @@
 // eight in fp64. Where the fp32 sum of eight leaves [2^-100, 2^120] its elements are squared in fp64 instead, so
 // neither large nor tiny gradients (whose squares leave fp32) change the norm. Partial sums have one slot per block and
 // are added in one fixed order: the result does not depend on timing.
+//
+// Both passes are bound by HBM. One decoder layer in bf16 (202 M elements): norm 64 us (6.3 TB/s), norm and clipping into
+// other buffers 193 us (three passes over 405 MB, 6.3 TB/s); 150 tensors of 1.9 M elements in all: 6 and 10 us.
 #include <cstdlib>
 
 #include <algorithm>

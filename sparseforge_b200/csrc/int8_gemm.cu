@@ -228,6 +228,8 @@ __device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bia
 // kernel (128 bytes of K = 128 integers instead of 64 bf16; 16 KiB of A and 16 KiB of B per CTA, six stages), an
 // instruction covers 32 of K at the bf16 instruction's cycle count. Two accumulators of 256 columns fill the tensor memory:
 // the epilogue (integer -> float, two scales, bias, store) of a tile runs under the next tile's products.
+// [8192, 4096] x [4096, 4096]: 88 us = 3120 TOP/s, the tensor pipe busy in 83 % of its cycles (operand delivery takes the
+// rest, as in the bf16 kernel); [8192, 4096] x [11008, 4096]: 219 us = 3370 TOP/s in a burst, 240 us under the power cap.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int I8_BK = 128;                      // bytes = integers of K per stage: one 128-byte swizzled row
 constexpr int I8_THREADS = 192;

@@ -43,6 +43,47 @@ def combine_score_sums(sums: torch.Tensor, n_local: int, group=None) -> Tuple[to
     return sums, n_local * world
 
 
+@torch.no_grad()
+def clip_grad_norm_(model: nn.Module, max_norm, norm_type=2.0) -> torch.Tensor:
+    """``utils.clip_grad_norm_`` for a model with row-sharded layers: the norm is that of the whole model's gradients.
+
+    Gradients inside ``RowShardedLinear`` / ``PeerShardedLinear`` are this rank's rows, so their norm is combined over
+    the layers' process group (one group per model); all other gradients are the same on every rank and
+    counted once. Every rank calls this, and every rank scales by the same coefficient. One all-reduce of two
+    numbers; nothing is read back to the host. Without a process group this is ``utils.clip_grad_norm_``."""
+    from . import ops
+
+    local, groups = set(), set()
+    for m in model.modules():
+        if isinstance(m, (RowShardedLinear, PeerShardedLinear)):
+            local.update(id(p) for p in m.shard.parameters())
+            groups.add(m.group)
+    if len(groups) > 1:
+        raise ValueError("clip_grad_norm_: the model's sharded layers must share one process group")
+    grads = [(p.grad, id(p) in local) for p in model.parameters() if p.grad is not None]
+    group = next(iter(groups), None)
+    world = dist.get_world_size(group) if (groups and dist.is_available() and dist.is_initialized()) else 1
+    if world == 1:
+        every = [g for g, _ in grads]
+        return ops.clip_grad_norm(every, max_norm, norm_type) if every else torch.tensor(0.0)
+    mine, common = [g for g, s in grads if s], [g for g, s in grads if not s]
+    device = grads[0][0].device if grads else next(model.parameters()).device
+    zero = torch.zeros((), dtype=torch.float32, device=device)
+    a = ops.grad_norm(mine, norm_type) if mine else zero
+    b = ops.grad_norm(common, norm_type) if common else zero
+    if float(norm_type) == 2.0:
+        sq = a.double().square()  # fp64: the square of an fp32 norm stays in range
+        dist.all_reduce(sq, op=dist.ReduceOp.SUM, group=group)
+        norm = (sq + b.double().square()).sqrt().float()
+    else:
+        # a maximum over ranks may drop a NaN: it travels as a flag of its own
+        pair = torch.stack([torch.nan_to_num(a, nan=0.0, posinf=float("inf")), torch.isnan(a).float()])
+        dist.all_reduce(pair, op=dist.ReduceOp.MAX, group=group)
+        norm = torch.maximum(torch.where(pair[1] > 0, torch.full_like(pair[0], float("nan")), pair[0]), b)
+    ops.clip_grads([g for g, _ in grads], norm, max_norm)
+    return norm
+
+
 class _GatherColumns(torch.autograd.Function):
     """[T, rows] per rank -> [T, rows * world]; backward keeps the rank's own column block."""
 

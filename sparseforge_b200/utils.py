@@ -165,8 +165,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     Two launches for up to 448 gradients. The norm is one fp32 scalar on the device that was never rounded to the
     gradients' dtype; gradients that need no scaling are read once and not written. ``norm_type``: 2 or ``inf``.
     ``error_if_nonfinite`` reads the norm back. ``foreach`` is accepted and ignored. A parameter named twice is
-    counted and scaled once. With row shards the norm is this rank's: combine ``ops.grad_norm`` over the ranks and
-    call ``ops.clip_grads`` instead."""
+    counted and scaled once. A model with row-sharded layers takes ``sharding.clip_grad_norm_``."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads, seen = [], set()

@@ -286,6 +286,22 @@ def test_utils_clip_matches_torch():
     assert float(utils.clip_grad_norm_(p, 10.0, norm_type=math.inf, error_if_nonfinite=True)) == 4.0
 
 
+def test_clip_of_a_model_with_a_sharded_layer_in_one_process():
+    from sparseforge_b200 import sharding, utils
+
+    torch.manual_seed(1)
+    model = torch.nn.Sequential(sharding.RowShardedLinear(torch.nn.Linear(16, 8)), torch.nn.LayerNorm(8)).cuda()
+    for q in model.parameters():
+        q.grad = torch.randn_like(q)
+    raw = [q.grad.clone() for q in model.parameters()]
+    norm = sharding.clip_grad_norm_(model, 0.25)
+    clipped = [q.grad.clone() for q in model.parameters()]
+    for q, r in zip(model.parameters(), raw):
+        q.grad = r
+    assert torch.equal(norm, utils.clip_grad_norm_(model.parameters(), 0.25))
+    assert all(torch.equal(q.grad, c) for q, c in zip(model.parameters(), clipped))
+
+
 def test_codes_of_the_c_entry_points():
     from sparseforge_b200 import _lib
 

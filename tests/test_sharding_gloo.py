@@ -179,3 +179,59 @@ def test_single_process_is_a_no_op():
 
     x = torch.randn(3, 4)
     assert gather_columns(x) is x and sum_input_grad(x) is x
+
+
+def _plain_norm(grads, p=2.0):
+    flat = torch.cat([g.double().flatten() for g in grads])
+    return (flat.abs().max() if p == float("inf") else flat.square().sum().sqrt()).float()
+
+
+def _plain_clip(grads, norm, max_norm, out=None):
+    c = torch.clamp(max_norm / (norm.double() + 1e-6), max=1.0)
+    for g in grads:
+        g.mul_(c.to(g.dtype))
+
+
+def _clip_worker(rank, world, port, out_q):
+    """Host logic of clipping with row shards; the two kernels are stood in for by plain sums (there is no CPU path)."""
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        from sparseforge_b200 import ops, sharding
+
+        ops.grad_norm, ops.clip_grads = _plain_norm, _plain_clip
+        ok = True
+        for p in (2.0, float("inf")):
+            for poison in (None, float("nan"), float("inf")):
+                g = torch.Generator().manual_seed(3)  # the whole model's gradients, alike on every rank
+                full, common = torch.randn(32, 8, generator=g), torch.randn(11, generator=g)
+                if poison is not None:
+                    full[20, 3] = poison  # a row of rank 1
+                lo, hi = sharding.shard_bounds(32, world, rank)
+                model = torch.nn.Sequential(sharding.RowShardedLinear(torch.nn.Linear(8, hi - lo, bias=False)),
+                                            torch.nn.LayerNorm(11, bias=False))
+                model[0].shard.weight.grad, model[1].weight.grad = full[lo:hi].clone(), common.clone()
+                norm = sharding.clip_grad_norm_(model, 0.5, p)
+                want = _plain_norm([full, common], p)
+                both = torch.cat([full[lo:hi].flatten(), common])
+                _plain_clip([both], want, 0.5)
+                got = torch.cat([model[0].shard.weight.grad.flatten(), model[1].weight.grad])
+                ok = ok and torch.allclose(norm, want, rtol=1e-6, equal_nan=True)
+                ok = ok and torch.allclose(got, both, rtol=1e-5, equal_nan=True)
+        out_q.put((rank, bool(ok)))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_clipping_with_row_shards_uses_the_whole_models_norm():
+    world, port = 2, _free_port()
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_clip_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    for p in procs:
+        p.join(timeout=180)
+    assert all(p.exitcode == 0 for p in procs), [p.exitcode for p in procs]
+    results = dict(q.get(timeout=10) for _ in range(world))
+    assert results == {0: True, 1: True}
