@@ -68,7 +68,15 @@ struct Raw8;
 template <>
 struct Raw8<__nv_bfloat16> {
     uint4 v;
+    __device__ __forceinline__ void clear() { v = make_uint4(0u, 0u, 0u, 0u); }
     __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void load_edge(const __nv_bfloat16* row, int first, int cols) {  // zero outside the row
+        const unsigned short* u = reinterpret_cast<const unsigned short*>(row);
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = first + i >= 0 && first + i < cols ? (uint32_t)__ldg(u + first + i) : 0u;
+        v = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+    }
     __device__ __forceinline__ void unpack(float (&x)[8]) const {
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -81,9 +89,17 @@ struct Raw8<__nv_bfloat16> {
 template <>
 struct Raw8<float> {
     float4 a, b;
+    __device__ __forceinline__ void clear() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
     __device__ __forceinline__ void load(const float* p) {
         a = __ldg(reinterpret_cast<const float4*>(p));
         b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    }
+    __device__ __forceinline__ void load_edge(const float* row, int first, int cols) {  // zero outside the row
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = first + i >= 0 && first + i < cols ? __ldg(row + first + i) : 0.0f;
+        a = make_float4(w[0], w[1], w[2], w[3]);
+        b = make_float4(w[4], w[5], w[6], w[7]);
     }
     __device__ __forceinline__ void unpack(float (&x)[8]) const {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
@@ -190,30 +206,83 @@ int8_quantize_vec_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict
     }
 }
 
-// Any other row: one block per row, read twice (the second time from a cache), element by element.
+// Any other row (any length, any element alignment): TPR threads per row. Loads are the 16-byte granules the row lies in;
+// the two granules at its ends that it only partly fills are read element by element. A granule's eight results
+// belong to two neighbouring 8-byte pieces of the output: the second part comes from the next lane, so a warp takes 32
+// granules and writes 31 pieces. NV > 0: all of a row's granules stay in registers, NV per thread (rows of up to NV * 31 *
+// TPR / 32 pieces); NV = 0: longer rows are read twice, the second time from a cache.
 template <typename T>
+__device__ __forceinline__ void load_granule(Raw8<T>& r, const T* row, int first, int cols) {  // elements first ... first + 7
+    if (first >= 0 && first + 8 <= cols) r.load(row + first);
+    else r.load_edge(row, first, cols);
+}
+template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(kQThreads)
-int8_quantize_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int cols,
-                     int pitch) {
+int8_quantize_any_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
+                         int cols, int pitch) {
     __shared__ uint32_t part[kQThreads / 32];
     ptx::dependency_wait();
     ptx::launch_dependents();
-    const T* row = x + (int64_t)blockIdx.x * ld;
+    constexpr int STEP = TPR / 32 * 31;
+    const int wanted = blockIdx.x * (kQThreads / TPR) + threadIdx.x / TPR;
+    const bool live = wanted < rows;
+    const int r = live ? wanted : rows - 1;  // threads without a row follow the last one, for the barrier, and write nothing
+    const T* row = x + (int64_t)r * ld;
+    const int lead = (int)(reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T);  // elements of the first granule before the row
+    const int granules = (cols + lead + 7) / 8, pieces = pitch / 8, me = threadIdx.x % TPR, lane = threadIdx.x & 31;
+    const int first = me / 32 * 31;  // first piece of this warp
+    Raw8<T> kept[NV ? NV : 1];
     uint32_t top = 0;
-#pragma unroll 4
-    for (int k = threadIdx.x; k < cols; k += kQThreads) top = max(top, magnitude_bits(as_f32(row[k])));
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-    __syncthreads();
+    if (NV) {
 #pragma unroll
-    for (int w = 0; w < kQThreads / 32; ++w) top = max(top, part[w]);
+        for (int u = 0; u < NV; ++u) {
+            const int v = first + u * STEP + lane;
+            kept[u].clear();
+            if (v < granules) load_granule(kept[u], row, 8 * v - lead, cols);
+        }
+#pragma unroll
+        for (int u = 0; u < NV; ++u) top = top8(kept[u], top);
+    } else {
+#pragma unroll 4
+        for (int v = me; v < granules; v += TPR) {
+            Raw8<T> g;
+            load_granule(g, row, 8 * v - lead, cols);
+            top = top8(g, top);
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top_bits(T(), top));
+    if (TPR > 32) {
+        const int w0 = threadIdx.x / TPR * (TPR / 32);
+        if (lane == 0) part[threadIdx.x >> 5] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < TPR / 32; ++w) top = max(top, part[w0 + w]);
+    }
     const bool usable = top < 0x7f800000u && top != 0;
     const RowScale rs = row_scale<T>(__uint_as_float(top));
-    if (threadIdx.x == 0) scale[blockIdx.x] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
-    int8_t* out = q + (int64_t)blockIdx.x * pitch;
-#pragma unroll 4
-    for (int k = threadIdx.x; k < pitch; k += kQThreads)
-        out[k] = (int8_t)(k < cols && usable ? quantise(T(), as_f32(row[k]), rs) : 0);
+    if (live && me == 0) scale[r] = top < 0x7f800000u ? __fdiv_rn(rs.a, 127.0f) : nan_f32();
+    unsigned long long* dst = reinterpret_cast<unsigned long long*>(q + (int64_t)r * pitch);
+    auto put = [&](const Raw8<T>& g, int v) {
+        unsigned long long bytes = 0;
+        if (usable && v < granules) {
+            const uint2 b = quantise8(g, rs);
+            bytes = (unsigned long long)b.y << 32 | b.x;
+        }
+        const unsigned long long next = __shfl_down_sync(0xffffffffu, bytes, 1);
+        if (live && lane < 31 && v < pieces) dst[v] = lead ? bytes >> (8 * lead) | next << (64 - 8 * lead) : bytes;
+    };
+    if (NV) {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) put(kept[u], first + u * STEP + lane);
+    } else {
+#pragma unroll 2
+        for (int base = first; base < pieces; base += STEP) {
+            Raw8<T> g;
+            g.clear();
+            if (base + lane < granules) load_granule(g, row, 8 * (base + lane) - lead, cols);
+            put(g, base + lane);
+        }
+    }
 }
 
 // One place for the arithmetic behind the sum, so that every kernel rounds alike (bias 0 where there is none).
@@ -892,7 +961,7 @@ template <typename T>
 static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
                           cudaStream_t st) {
     const int pitch = (int)((cols + 15) / 16 * 16);
-    // A warp per row up to 1024 elements, a block per row up to 16384, all of the row in registers. [8192, 4096] bf16: 17.7 us
+    // A warp per row up to 1024 elements, a block per row up to 32768, all of the row in registers. [8192, 4096] bf16: 17.7 us
     // (5.7 TB/s) with 128 threads per row, 18.9 with 256, 21.5 with 512; [8192, 11008]: 44.3 us (6.1 TB/s).
 #define SF_I8_QUANT(THREADS, TPR, NV)                                                                                 \
     do {                                                                                                              \
@@ -909,11 +978,23 @@ static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* sc
         SF_I8_QUANT(256, 256, 6);
     } else if (vec && cols <= 16384) {
         SF_I8_QUANT(512, 512, 4);
+    } else if (vec && cols <= 32768) {
+        SF_I8_QUANT(1024, 1024, 4);
 #undef SF_I8_QUANT
+    // unaligned rows; a warp per row where there are many short ones
+#define SF_I8_QUANT_ANY(TPR, NV)                                                                                      \
+    SF_CHECK_CUDA(launch_dependent(int8_quantize_any_kernel<T, TPR, NV>, (int)((rows + kQThreads / TPR - 1) / (kQThreads / TPR)), \
+                                   kQThreads, 0, 1, true, st, x, ld, q, scale, (int)rows, (int)cols, pitch))
+    } else if (pitch <= 8 * 31 * 4 && rows >= 16 * (int64_t)sm_count()) {
+        SF_I8_QUANT_ANY(32, 4);
+    } else if (pitch <= 8 * 31 * 4 * 5) {
+        SF_I8_QUANT_ANY(128, 5);
+    } else if (pitch <= 8 * 31 * 8 * 6) {
+        SF_I8_QUANT_ANY(256, 6);
     } else {
-        SF_CHECK_CUDA(launch_dependent(int8_quantize_kernel<T>, (int)rows, kQThreads, 0, 1, true, st, x, ld, q, scale,
-                                       (int)cols, pitch));
+        SF_I8_QUANT_ANY(256, 0);
     }
+#undef SF_I8_QUANT_ANY
     return SF_OK;
 }
 static int quantize_impl(const void* x, int dtype, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
@@ -1041,6 +1122,8 @@ int sf_int8_quantize_rows(const void* x, int dtype, int64_t ld, int8_t* q, float
     SF_CHECK_ARG(x && q && scale, "sf_int8_quantize_rows: x, q and scale must be non-null");
     SF_CHECK_ARG(ld >= cols || rows == 1, "sf_int8_quantize_rows: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(q)) return fail(SF_ERR_ALIGNMENT, "sf_int8_quantize_rows: q must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(x) % (dtype == SF_F32 ? 4 : 2))
+        return fail(SF_ERR_ALIGNMENT, "sf_int8_quantize_rows: x must be aligned to its elements");
     return quantize_impl(x, dtype, ld, q, scale, rows, cols, (cudaStream_t)stream);
 }
 
@@ -1076,6 +1159,8 @@ int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_s
     SF_CHECK_ARG(x && (workspace || stream_rows), "sf_int8_linear: x and workspace must be non-null");
     SF_CHECK_ARG(ld >= in || rows == 1, "sf_int8_linear: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(workspace)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: workspace must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(x) % (dtype == SF_F32 ? 4 : 2))
+        return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: x must be aligned to its elements");
     if (stream_rows) {
         const bool vec = rows_vectorise(x, dtype, ld, rows, in);
         return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream)

@@ -76,6 +76,23 @@ def test_quantised_rows(cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols", [1, 2, 7, 8, 9, 23, 247, 248, 249, 1000, 1024, 1025, 2047, 4104, 20000, 32769])
+def test_quantised_rows_at_every_alignment(cols, dtype):
+    """Rows starting at every element offset from a 16-byte boundary, with guard elements around them; strided so that the
+    offset changes from row to row, and in a constant one."""
+    ops = _ops()
+    for off in range(9):
+        for ld in (cols + 3, (cols + 15) // 8 * 8):
+            buf = torch.full((off + 11 * ld + 16,), 1e4, device="cuda", dtype=DT[dtype])  # a guard that is read would win the maximum
+            x = torch.as_strided(buf, (11, cols), (ld, 1), off)
+            x.copy_(torch.randn(11, cols, device="cuda"))
+            q, s = ops.int8_quantize_rows(x)
+            want, scale = _quantise64(x)
+            assert torch.equal(q[:, :cols].double(), want) and not q[:, cols:].any(), (off, ld)
+            assert ((s.double() - scale).abs() <= U * scale).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_quantised_rows_near_and_on_halves(dtype):
     """Quotients exactly half-way go to the even integer; the neighbours of such values go to their own side."""
     rows = []

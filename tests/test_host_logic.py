@@ -373,6 +373,8 @@ def test_int8_refusals_without_a_gpu():
     assert lib.sf_int8_quantize_rows(A, _lib.SF_I8, 8, A, A, 1, 8, None) == -1
     assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 4, A, A, 2, 8, None) == -1      # rows overlap
     assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 8, A + 8, A, 2, 8, None) == -3  # q not 16-byte aligned
+    assert lib.sf_int8_quantize_rows(A + 2, _lib.SF_F32, 8, A, A, 2, 8, None) == -3  # x not on an element
+    assert lib.sf_int8_linear(A + 1, 8, A, A, None, A, _lib.SF_BF16, 1, 8, 8, A, None, None) == -3
     assert lib.sf_int8_quantize_rows(A, _lib.SF_F32, 1 << 20, A, A, 2, 131057, None) == -2
     assert lib.sf_int8_quantize_rows(None, _lib.SF_F32, 8, None, None, 0, 8, None) == 0  # no rows: nothing to do
     assert lib.sf_int8_gemm(A, A, A, A, None, A, _lib.SF_BF16, -1, 8, 8, None, None) == -1
