@@ -518,7 +518,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 // multiplied (dp4a): 128 KiB in flight per SM, as much as an SM's share of a [4096, 4096] weight, and the last turn is
 // never more than one piece long. The first pieces are requested before the block quantises the tokens into shared
 // memory: each block repeats that small work, which saves a launch and a wait. Pieces' sums meet in shared memory (integer
-// additions: their order does not matter).
+// additions: their order does not matter). [1, 4096] x [4096, 4096]: 5.9 us, x [11008, 4096]: 10.2 us, [1, 11008] x [4096,
+// 11008]: 11.0 us back to back; from the end of the kernel ahead the weights are in within 5.8 us of the 10.2.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int GV_WARPS = 32, GV_THREADS = 32 * GV_WARPS;
 constexpr int GV_LOADS = 4, GV_PIECE = GV_LOADS * 512;
@@ -664,13 +665,15 @@ int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict
 // columns (column c belongs to part c mod split) over all parts and writes them: one launch, no workspace, any order of
 // arrival gives the same sum. (Stores into the owner's shared memory instead save the second barrier but cost
 // more than it: [64, 4096] x [4096, 4096] 9.5 -> 15.9 us.)
-// PAIR = 2 (more than 64 tokens): two CTAs share a 256-row tile (cta_group::2), each loads half of the tokens, 24 KiB per
-// stage instead of 32 for the same products: above 64 tokens the traffic into the SMs is what bounds the tile.
+// PAIR = 2 (256 tokens): two CTAs share a 256 x 256 tile (cta_group::2) and each loads half of the tokens, for long
+// reductions over some hundred rows, where the traffic into the SMs is what bounds the tile.
 // The weight loads of the first stages are issued before the kernel waits for the quantised rows.
+// [16, 4096] x [11008, 4096]: 13.3 us back to back, of which 8.1 the stream of weights (5.5 TB/s), 0.6 setting up, 1.6 joining
+// and writing, the rest handing over between launches; [16, 4096] x [4096, 4096]: 7.9 us, [64, 4096] x [4096, 4096]: 9.6 us.
 // ---------------------------------------------------------------------------------------------------------
 template <int BN, int PAIR>
 struct I8Few {
-    static constexpr int STAGES = BN > 128 ? 6 : (BN * PAIR <= 32 ? 5 : 4);  // up to 128 tokens 94 to 104 KB: two CTAs per SM
+    static constexpr int STAGES = BN > 64 ? 6 : (BN <= 32 ? 5 : 4);  // up to 64 tokens 93 to 103 KB: two CTAs per SM
     static constexpr int X_ROWS = BN / PAIR;
     static constexpr int STAGE_BYTES = I8_OPERAND_BYTES + X_ROWS * I8_BK;
     static constexpr int TMEM_COLS = BN < 32 ? 32 : BN;
@@ -711,7 +714,7 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vali
 }
 
 template <typename T, int BN, int PAIR>
-__global__ void __launch_bounds__(I8_THREADS, BN > 128 ? 1 : 2)
+__global__ void __launch_bounds__(I8_THREADS, BN > 64 ? 1 : 2)
 int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                 const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
                 int rows, int out, int pitch, int split, int tiles_t, int32_t* status) {
@@ -1050,7 +1053,7 @@ static int launch_few(const int8_t* xq, const float* xs, const int8_t* wq, const
     int split = 1;
     while (split < C::MAX_SPLIT && 2 * split <= num_kb) {
         const int64_t ctas = tiles * PAIR * split;
-        const bool idle = ctas * 4 < sms * (BN > 128 ? 2 : 3);
+        const bool idle = ctas * 4 < sms * (BN > 64 ? 2 : 3);
         const bool room = BN <= 64 && ctas <= sms && num_kb >= 32 * split;
         if (!idle && !room) break;
         split *= 2;
