@@ -297,8 +297,8 @@ __device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bia
 // kernel (128 bytes of K = 128 integers instead of 64 bf16; 16 KiB of A and 16 KiB of B per CTA, six stages), an
 // instruction covers 32 of K at the bf16 instruction's cycle count. Two accumulators of 256 columns fill the tensor memory:
 // the epilogue (integer -> float, two scales, bias, store) of a tile runs under the next tile's products.
-// [8192, 4096] x [4096, 4096]: 88 us = 3120 TOP/s, the tensor pipe busy in 83 % of its cycles (operand delivery takes the
-// rest, as in the bf16 kernel); [8192, 4096] x [11008, 4096]: 219 us = 3370 TOP/s in a burst, 240 us under the power cap.
+// [8192, 4096] x [4096, 4096]: 84 us = 3260 TOP/s, the tensor pipe busy in 83 % of its cycles and more (operand delivery takes
+// the rest, as in the bf16 kernel); [8192, 4096] x [11008, 4096]: 230 us = 3210 TOP/s under the power cap.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int I8_BK = 128;                      // bytes = integers of K per stage: one 128-byte swizzled row
 constexpr int I8_THREADS = 192;
@@ -306,7 +306,7 @@ constexpr int I8_STAGES = 6;
 constexpr int I8_OPERAND_BYTES = 128 * I8_BK;   // 16 KiB: this CTA's 128 rows of A, and its half of B's 256 rows
 constexpr int I8_STAGE_BYTES = 2 * I8_OPERAND_BYTES;
 constexpr int I8_EPI_BYTES = 2 * 256 * 4;       // per epilogue warp: scales and bias of the tile's columns
-constexpr int I8_PAIR_SMEM = I8_STAGES * I8_STAGE_BYTES + 4 * I8_EPI_BYTES + 1024 + 256;
+constexpr int I8_PAIR_SMEM = I8_STAGES * I8_STAGE_BYTES + 4 * (I8_EPI_BYTES + 32 * 144) + 1024 + 256;  // and four turn buffers
 constexpr int I8_RASTER_M = 16;                 // tile rows per raster group: panels are shared in L2
 
 struct I8PairTail {
@@ -326,34 +326,51 @@ __device__ __forceinline__ void i8_tile_coords(int tile, int tiles_m, int tiles_
     tn = r / gm;
 }
 
-// Stores 32 consecutive columns of one row. vec: the row starts on a 16-byte boundary and all 32 columns exist.
-__device__ __forceinline__ void store_cols32(__nv_bfloat16* dst, const float (&v)[32], int valid, bool vec) {
-    if (vec && valid >= 32) {
+// Results leave through a turn buffer in shared memory, 128 bytes of 32 rows at a time (64 bf16 or 32 fp32 columns): a
+// thread holds one row, a store instruction then covers whole rows: four rows x 128 bytes in 16-byte pieces, or, where
+// rows are not on 16-byte boundaries, 32 consecutive elements of one row. Stored straight from the threads that hold a row
+// each, an odd number of channels cost [8192, 4096] x [4095, 4096] 348 us instead of 88.
+constexpr int I8_TURN_ROW = 128 + 16;  // padding against bank conflicts
+constexpr int I8_TURN_BYTES = 32 * I8_TURN_ROW;
+
+__device__ __forceinline__ void turn_in(uint8_t* row, const float (&v)[32], int part, __nv_bfloat16) {  // part: left or right half
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
+    for (int j = 0; j < 4; ++j) {
+        uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
-                w[i] = *reinterpret_cast<const uint32_t*>(&h);
-            }
-            *reinterpret_cast<uint4*>(dst + 8 * j) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(v[8 * j + 2 * i], v[8 * j + 2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
-    } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < valid) dst[j] = __float2bfloat16_rn(v[j]);
+        *reinterpret_cast<uint4*>(row + part * 64 + j * 16) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
-__device__ __forceinline__ void store_cols32(float* dst, const float (&v)[32], int valid, bool vec) {
-    if (vec && valid >= 32) {
+__device__ __forceinline__ void turn_in(uint8_t* row, const float (&v)[32], int, float) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            *reinterpret_cast<float4*>(dst + 4 * j) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    for (int j = 0; j < 8; ++j)
+        *reinterpret_cast<float4*>(row + j * 16) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+}
+// 32 rows of the turn buffer to y: dst is row 0's first column of the chunk, `rows` rows and `cols` columns of it exist.
+template <typename T>
+__device__ __forceinline__ void turn_out(const uint8_t* buf, T* dst, int64_t ld, int rows, int cols, bool vec, int lane) {
+    constexpr int PIECE = 16 / sizeof(T), COLS = 128 / sizeof(T);
+    if (vec) {
+        const int piece = lane & 7;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (r < rows && piece * PIECE < cols)  // ld is a multiple of PIECE, so a piece exists wholly or not at all
+                *reinterpret_cast<uint4*>(dst + r * ld + piece * PIECE) = *reinterpret_cast<const uint4*>(buf + r * I8_TURN_ROW + piece * 16);
+        }
     } else {
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) {
+            if (r >= rows) break;
+            const T* src = reinterpret_cast<const T*>(buf + r * I8_TURN_ROW);
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < valid) dst[j] = v[j];
+            for (int c = 0; c < COLS; c += 32)
+                if (c + lane < cols) dst[r * ld + c + lane] = src[c + lane];
+        }
     }
 }
 
@@ -367,7 +384,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw_addr);
     float* epi = reinterpret_cast<float*>(base_ptr + I8_STAGES * I8_STAGE_BYTES);
-    I8PairTail* tail = reinterpret_cast<I8PairTail*>(base_ptr + I8_STAGES * I8_STAGE_BYTES + 4 * I8_EPI_BYTES);
+    uint8_t* turns = base_ptr + I8_STAGES * I8_STAGE_BYTES + 4 * I8_EPI_BYTES;
+    I8PairTail* tail = reinterpret_cast<I8PairTail*>(turns + 4 * I8_TURN_BYTES);
     volatile int* abort_flag = &tail->abort_flag;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -466,6 +484,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const uint32_t leader_empty0 = ptx::map_to_cta(ptx::smem_u32(&tail->tmem_empty[0]), 0);
         const uint32_t leader_empty1 = ptx::map_to_cta(ptx::smem_u32(&tail->tmem_empty[1]), 0);
         float* cs = epi + (warp - 2) * 512;  // scales of the tile's 256 columns, then their bias
+        uint8_t* turn = turns + (warp - 2) * I8_TURN_BYTES;
         const bool vec = ((int64_t)out * sizeof(T)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
         bool ok = true;
         int t = 0;
@@ -485,21 +504,33 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             ok = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full[acc]), (uint32_t)(t >> 1) & 1u, abort_flag, status, 44);
             if (!ok) break;
             ptx::tc_fence_after();
-            T* drow = y + (int64_t)row * out + n0;
             const uint32_t taddr = tmem_base + (uint32_t)(acc * 256) + ((uint32_t)(q * 32) << 16);
+            constexpr int PARTS = 4 / (int)sizeof(T);  // accumulator reads of 32 columns per 128 bytes of a row
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-                uint32_t r[32];
-                ptx::tmem_ld_32x32b_x32(taddr + (uint32_t)(c * 32), r);
-                ptx::tmem_ld_wait();
-                float v[32];
+            for (int c = 0; c < 8; c += PARTS) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = int8_out((int)r[j], rs, cs[c * 32 + j], cs[256 + c * 32 + j]);
-                if (row < rows) store_cols32(drow + c * 32, v, out - n0 - c * 32, vec);
+                for (int part = 0; part < PARTS; ++part) {
+                    const int col = (c + part) * 32;
+                    uint32_t r[32];
+                    ptx::tmem_ld_32x32b_x32(taddr + (uint32_t)col, r);
+                    ptx::tmem_ld_wait();
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = int8_out((int)r[j], rs, cs[col + j], cs[256 + col + j]);
+                    turn_in(turn + lane * I8_TURN_ROW, v, part, T());
+                }
+                if (c + PARTS == 8) {  // the last of the accumulator has been read: the MMA warp may have it back
+                    ptx::tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+                } else {
+                    __syncwarp();
+                }
+                const int col = c * 32, row0 = row - lane;
+                if (row0 < rows && n0 + col < out)
+                    turn_out(turn, y + (int64_t)row0 * out + n0 + col, (int64_t)out, rows - row0, out - n0 - col, vec, lane);
+                __syncwarp();  // the turn buffer and, after the last chunk, the column scales may be overwritten
             }
-            ptx::tc_fence_before();
-            __syncwarp();  // also: the column scales may be overwritten
-            if (lane == 0) ptx::mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
         }
     }
 
