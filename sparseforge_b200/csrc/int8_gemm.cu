@@ -516,7 +516,14 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                     ptx::tmem_ld_wait();
                     float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = int8_out((int)r[j], rs, cs[col + j], cs[256 + col + j]);
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 s4 = *reinterpret_cast<const float4*>(cs + col + j);
+                        const float4 b4 = *reinterpret_cast<const float4*>(cs + 256 + col + j);
+                        v[j] = int8_out((int)r[j], rs, s4.x, b4.x);
+                        v[j + 1] = int8_out((int)r[j + 1], rs, s4.y, b4.y);
+                        v[j + 2] = int8_out((int)r[j + 2], rs, s4.z, b4.z);
+                        v[j + 3] = int8_out((int)r[j + 3], rs, s4.w, b4.w);
+                    }
                     turn_in(turn + lane * I8_TURN_ROW, v, part, T());
                 }
                 if (c + PARTS == 8) {  // the last of the accumulator has been read: the MMA warp may have it back
@@ -1125,10 +1132,10 @@ static int gemm_typed(const int8_t* xq, const float* xs, const int8_t* wq, const
     if (rows <= 32) return launch_few<T, 32, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     // More rows. While 128 x 64 tiles fit the chip at two per SM they are the fastest ([512, 4096] x [4096, 4096]: 16.0 us, 256 x
     // 256 tiles cut in two 16.4, persistent 17.5; [128, 4096] x [11008, 4096]: 16.0, 18.4, 19.1), but their operands are
-    // loaded more often: past 256 rows a long reduction takes 256 x 256 tiles cut in two where those leave half of the SMs
-    // idle ([512, 11008] x [4096, 11008]: 25.4 us against 31.8 and 33.6). Beyond that, persistent tiles.
+    // loaded more often: past 256 rows a long reduction takes 256 x 256 tiles cut in two where those fill half of the SMs and
+    // fit all ([512, 11008] x [4096, 11008]: 25.4 us against 31.8 and 33.6). Beyond that, persistent tiles.
     const int64_t small = ((out + 127) / 128) * ((rows + 63) / 64), large = ((out + 255) / 256) * ((rows + 255) / 256);
-    if (rows > 256 && pitch >= 8192 && large * 4 <= sm_count())
+    if (rows > 256 && pitch >= 8192 && large * 4 <= sm_count() && large * 8 >= sm_count())
         return launch_few<T, 256, 2>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     if (small <= 2 * (int64_t)sm_count()) return launch_few<T, 64, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     return launch_pair<T>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
