@@ -360,3 +360,82 @@ def test_offsets_beyond_32_bits(T, k, n):
     _check(y[-3:, last].contiguous(), raw, raw.abs(), torch.bfloat16)
     first = (q[:1] @ wq[:64, :k].double().t()) * s[:1, None] * ws[:64].double()
     _check(y[-3 if T > 2 else -T:, :64][:1].contiguous(), first, first.abs(), torch.bfloat16)
+
+
+@pytest.mark.parametrize("T", [1, 2, 9, 40, 200, 600])
+@pytest.mark.parametrize("captured", [False, True])
+def test_operands_written_just_before_the_call(T, captured):
+    """Inputs, weights, scales and bias that the work right ahead in the stream (a copy, a fill, a kernel, the
+    quantiser, another 8-bit call) has just written are what the call uses, eagerly and in a graph with a fork."""
+    ops = _ops()
+    k, n = 1024, 1500
+    g = torch.Generator(device="cuda").manual_seed(T)
+    xs = [torch.randn(T, k, device="cuda", generator=g).bfloat16() for _ in range(4)]
+    ws = [ops.int8_quantize_rows(torch.randn(n, k, device="cuda", generator=g).bfloat16()) for _ in range(3)]
+    raw = [torch.randn(n, k, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    bs = [torch.randn(n, device="cuda", generator=g).bfloat16() for _ in range(2)]
+    want = []
+    for i in range(4):
+        for w in ws + [ops.int8_quantize_rows(r) for r in raw]:
+            want.append(ops.int8_linear(xs[i], w[0], w[1], bs[i % 2]))
+    torch.cuda.synchronize()
+    x, wq, sc, b = torch.empty_like(xs[0]), torch.empty_like(ws[0][0]), torch.empty_like(ws[0][1]), torch.empty_like(bs[0])
+    got = [torch.empty_like(want[0]) for _ in want]
+    side = torch.cuda.Stream()
+
+    def run():
+        j = 0
+        for i in range(4):
+            for w in ws:
+                wq.zero_()
+                x.fill_(float("nan"))
+                sc.copy_(w[1])
+                b.copy_(bs[i % 2])
+                x.copy_(xs[i])
+                wq.copy_(w[0])
+                got[j].copy_(ops.int8_linear(x, wq, sc, b))
+                j += 1
+            for r in raw:  # the weight comes from the quantiser right ahead, the input from a kernel on another stream
+                now = torch.cuda.current_stream()
+                side.wait_stream(now)
+                with torch.cuda.stream(side):
+                    torch.add(xs[i], 0.0, out=x)
+                    y_side = ops.int8_linear(x, wq, sc, b)
+                q, s = ops.int8_quantize_rows(r)
+                now.wait_stream(side)
+                got[j].copy_(ops.int8_linear(x, q, s, b))
+                assert y_side.shape == got[j].shape
+                j += 1
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        for _ in range(3):
+            for t in got:
+                t.zero_()
+            graph.replay()
+    else:
+        for _ in range(3):
+            run()
+    torch.cuda.synchronize()
+    for a, w in zip(got, want):
+        assert torch.equal(a, w)
+
+
+def test_clipping_sees_gradients_written_just_before():
+    """Gradients written by the call right ahead (and norms read by the one behind), over and over on one stream."""
+    from sparseforge_b200 import ops
+
+    src = [torch.randn(1 << 20, device="cuda").bfloat16() * s for s in (1e-3, 1.0, 30.0)]
+    want = []
+    for s in src:
+        o = torch.empty_like(s)
+        want.append((ops.clip_grad_norm([s], 0.5, out=[o]), o))
+    g = torch.empty_like(src[0])
+    for rep in range(20):
+        s, (n, o) = src[rep % 3], want[rep % 3]
+        g.copy_(s)
+        norm = ops.clip_grad_norm([g], 0.5)
+        again = ops.grad_norm([g])
+        assert torch.equal(norm, n) and torch.equal(g, o) and torch.equal(again, ops.grad_norm([o]))
