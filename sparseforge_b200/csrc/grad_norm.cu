@@ -207,7 +207,7 @@ grad_norm_partial_kernel(const __grid_constant__ GnTable<CAP> tab, double* __res
 }
 
 // The norm from all slots, by every thread block that needs it: each computes the same value. Valid in every thread.
-__device__ __forceinline__ double norm_of_slots(const double* __restrict__ slots, int count, bool maxnorm, NormAcc* part,
+__device__ __forceinline__ double norm_of_slots(const double* slots, int count, bool maxnorm, NormAcc* part,
                                                 double* shared_norm) {
     NormAcc a{0.0, 0u};
     for (int i = threadIdx.x; i < count; i += kGnThreads) {
@@ -221,7 +221,7 @@ __device__ __forceinline__ double norm_of_slots(const double* __restrict__ slots
 }
 
 __global__ void __launch_bounds__(kGnThreads)
-grad_norm_final_kernel(const double* __restrict__ slots, int count, int kind, float* __restrict__ norm) {
+grad_norm_final_kernel(const double* slots, int count, int kind, float* norm) {
     __shared__ NormAcc part[kGnThreads / 32];
     __shared__ double value;
     ptx::dependency_wait();
@@ -233,7 +233,7 @@ grad_norm_final_kernel(const double* __restrict__ slots, int count, int kind, fl
 // value); or, with slots = NULL, the norm is read from norm_in.
 template <int CAP>
 __global__ void __launch_bounds__(kGnThreads, kGnClipBlocks)
-grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* __restrict__ slots, int slot_count, int kind,
+grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, int slot_count, int kind,
                  const float* norm_in, float* norm_out, double max_norm) {
     __shared__ NormAcc part[kGnThreads / 32];
     __shared__ double value;

@@ -69,12 +69,12 @@ template <>
 struct Raw8<__nv_bfloat16> {
     uint4 v;
     __device__ __forceinline__ void clear() { v = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ptx::ld_global_v4(p); }
     __device__ __forceinline__ void load_edge(const __nv_bfloat16* row, int first, int cols) {  // zero outside the row
         const unsigned short* u = reinterpret_cast<const unsigned short*>(row);
         uint32_t w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = first + i >= 0 && first + i < cols ? (uint32_t)__ldg(u + first + i) : 0u;
+        for (int i = 0; i < 8; ++i) w[i] = first + i >= 0 && first + i < cols ? ptx::ld_global_u16(u + first + i) : 0u;
         v = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
     }
     __device__ __forceinline__ void unpack(float (&x)[8]) const {
@@ -91,13 +91,14 @@ struct Raw8<float> {
     float4 a, b;
     __device__ __forceinline__ void clear() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
     __device__ __forceinline__ void load(const float* p) {
-        a = __ldg(reinterpret_cast<const float4*>(p));
-        b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+        const uint4 u = ptx::ld_global_v4(p), w = ptx::ld_global_v4(p + 4);
+        a = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
+        b = make_float4(__uint_as_float(w.x), __uint_as_float(w.y), __uint_as_float(w.z), __uint_as_float(w.w));
     }
     __device__ __forceinline__ void load_edge(const float* row, int first, int cols) {  // zero outside the row
         float w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = first + i >= 0 && first + i < cols ? __ldg(row + first + i) : 0.0f;
+        for (int i = 0; i < 8; ++i) w[i] = first + i >= 0 && first + i < cols ? ptx::ld_global_f32(row + first + i) : 0.0f;
         a = make_float4(w[0], w[1], w[2], w[3]);
         b = make_float4(w[4], w[5], w[6], w[7]);
     }
@@ -163,7 +164,7 @@ __device__ __forceinline__ uint2 quantise8(const Raw8<T>& r, const RowScale& rs)
 // loads of the next are issued before the present one is reduced, so that the memory system is never left idle.
 template <typename T, int THREADS, int TPR, int NV>
 __global__ void __launch_bounds__(THREADS)
-int8_quantize_vec_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
+int8_quantize_vec_kernel(const T* x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
                          int cols, int pitch) {
     __shared__ uint32_t part[2][THREADS / 32];
     ptx::dependency_wait();
@@ -218,7 +219,7 @@ __device__ __forceinline__ void load_granule(Raw8<T>& r, const T* row, int first
 }
 template <typename T, int TPR, int NV>
 __global__ void __launch_bounds__(kQThreads)
-int8_quantize_any_kernel(const T* __restrict__ x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
+int8_quantize_any_kernel(const T* x, int64_t ld, int8_t* __restrict__ q, float* __restrict__ scale, int rows,
                          int cols, int pitch) {
     __shared__ uint32_t part[kQThreads / 32];
     ptx::dependency_wait();
@@ -377,8 +378,8 @@ __device__ __forceinline__ void turn_out(const uint8_t* buf, T* dst, int64_t ld,
 template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                 const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
-                 int rows, int out, int pitch, int32_t* status) {
+                 const float* xs, const float* __restrict__ ws, const T* __restrict__ bias, T* y, int rows, int out,
+                 int pitch, int32_t* status) {
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = ptx::smem_u32(smem_raw);
     const uint32_t base = (raw_addr + 1023u) & ~1023u;
@@ -570,15 +571,15 @@ constexpr int GV_AHEAD_BYTES = 64 * 1024;
 
 __device__ __forceinline__ int4 ld_weights(const int8_t* p) {
     int4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    asm volatile("ld.global.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
 
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(GV_THREADS, 1)
-int8_stream_kernel(const T* __restrict__ x, int64_t ld, const int8_t* __restrict__ wq, const float* __restrict__ ws,
-                   const T* __restrict__ bias, T* __restrict__ y, int in, int out, int pitch, int vec) {
+int8_stream_kernel(const T* x, int64_t ld, const int8_t* wq, const float* ws, const T* bias, T* y, int in, int out,
+                   int pitch, int vec) {
     extern __shared__ __align__(16) uint8_t xq[];  // [ROWS][pitch]
     __shared__ uint32_t part[ROWS][GV_WARPS];
     __shared__ int sums[ROWS][GV_CHANNELS];
@@ -754,8 +755,8 @@ __device__ __forceinline__ void store4(float* dst, const float (&v)[4], int vali
 template <typename T, int BN, int PAIR>
 __global__ void __launch_bounds__(I8_THREADS, BN > 64 ? 1 : 2)
 int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
-                const float* __restrict__ xs, const float* __restrict__ ws, const T* __restrict__ bias, T* __restrict__ y,
-                int rows, int out, int pitch, int split, int tiles_t, int32_t* status) {
+                const float* xs, const float* __restrict__ ws, const T* __restrict__ bias, T* y, int rows, int out,
+                int pitch, int split, int tiles_t, int32_t* status) {
     using C = I8Few<BN, PAIR>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw_addr = ptx::smem_u32(smem_raw);

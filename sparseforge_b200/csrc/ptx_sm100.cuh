@@ -216,6 +216,24 @@ __device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, ui
 __device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
+// Ordinary (coherent) loads that stay behind the volatile statements before them. A kernel that is set up while the one
+// ahead of it runs must read that one's results this way: read-only loads (ld.global.nc, which the compiler also uses for
+// const __restrict__ pointers) assume data that does not change while the kernel lives.
+__device__ __forceinline__ uint4 ld_global_v4(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_global_u16(const void* p) {
+    unsigned short v;
+    asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_global_f32(const void* p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
 // Programmatic dependent launch: the next kernel of the stream may be set up from here on / wait until the
 // kernel before this one is done and its results are visible.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
