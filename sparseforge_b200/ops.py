@@ -754,14 +754,16 @@ def int8_quantize_rows(x2d):
 
 
 def int8_gemm(xq, x_scale, wq, w_scale, bias=None, out_dtype=torch.bfloat16, status=None):
-    """y[T, out] = (xq @ wq^T) * x_scale[:, None] * w_scale (+ bias) for operands of ``int8_quantize_rows``; the
-    sum is an exact 32-bit integer."""
-    _cuda(xq, x_scale, status)
+    """y[T, out] = (xq @ wq^T) * x_scale[:, None] * w_scale (+ bias) for operands of ``int8_quantize_rows`` (rows of a
+    multiple of 16 bytes, zero behind the last feature); the sum is an exact 32-bit integer."""
     if xq.dtype != torch.int8 or x_scale.dtype != torch.float32 or xq.dim() != 2 or x_scale.shape != xq.shape[:1]:
         raise TypeError("int8_gemm: xq int8 [rows, pitch] and float32 scales [rows] expected")
     if out_dtype not in _GRAD_DTYPES:
         raise TypeError("int8_gemm: out_dtype must be float32 or bfloat16")
     T, k = xq.shape
+    if k % 16:
+        raise ValueError(f"int8_gemm: rows of {k} bytes; operands have rows of a multiple of 16, as int8_quantize_rows makes them")
+    _cuda(xq, x_scale, status)
     if x_scale.device != xq.device:
         raise ValueError("int8_gemm: all tensors of a call must live on one device")
     out = _int8_weight(wq, w_scale, bias, k, out_dtype, xq.get_device(), "int8_gemm")

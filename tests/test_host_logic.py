@@ -397,3 +397,14 @@ def test_int8_refusals_without_a_gpu():
         layer.quantize_for_inference()
     with pytest.raises(TypeError):
         layer.half().quantize_for_inference()
+
+
+def test_int8_product_refuses_rows_that_are_no_multiple_of_16_bytes():
+    """The product reads rows of a multiple of 16 bytes: narrower operands would be read at the wrong place and past
+    their end. Refused before anything else is looked at, so the refusal is the same without a GPU."""
+    from sparseforge_b200 import ops
+
+    for k in (1, 15, 17, 20, 31):
+        xq, wq = torch.zeros(3, k, dtype=torch.int8), torch.zeros(7, (k + 15) // 16 * 16, dtype=torch.int8)
+        with pytest.raises(ValueError, match="multiple of 16"):
+            ops.int8_gemm(xq, torch.ones(3), wq, torch.ones(7))
