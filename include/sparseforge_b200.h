@@ -518,7 +518,8 @@ SF_API int sf_kl_div_bwd(const void* student, const void* teacher, int dtype, co
  *   sf_int8_linear: both, for x of y's dtype (rows of stride ld); workspace of sf_int8_linear_workspace_bytes
  *     bytes (may be 0: one or two rows need none), 16-byte aligned, holds nothing between calls; calls that may run at
  *     the same time need one each.
- * Any rows >= 0, in and out >= 1. 8-bit operands are 16-byte aligned. status as in sf_masked_gemm_fwd.
+ * Any rows >= 0, in and out >= 1. 8-bit operands are 16-byte aligned, everything else to its elements. No output
+ * overlaps an input. status as in sf_masked_gemm_fwd.
  */
 #define SF_INT8_MAX_IN ((int64_t)131056)
 SF_API int64_t sf_int8_pitch(int64_t cols);

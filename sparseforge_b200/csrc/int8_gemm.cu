@@ -952,6 +952,9 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     }
 }
 
+// An address that elements of the type may start at (4 bytes for SF_F32 and 32-bit integers, 2 for SF_BF16).
+static bool on_elements(const void* p, int dtype) { return reinterpret_cast<uintptr_t>(p) % (dtype == SF_F32 ? 4 : 2) == 0; }
+
 // One row or two, whose quantised form fits into shared memory, take the kernel without a workspace.
 static bool takes_stream(int64_t rows, int64_t in) { return rows <= GV_MAX_ROWS && rows * ((in + 15) / 16 * 16) <= GV_X_BYTES; }
 
@@ -1164,27 +1167,30 @@ int sf_int8_quantize_rows(const void* x, int dtype, int64_t ld, int8_t* q, float
     SF_CHECK_ARG(x && q && scale, "sf_int8_quantize_rows: x, q and scale must be non-null");
     SF_CHECK_ARG(ld >= cols || rows == 1, "sf_int8_quantize_rows: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(q)) return fail(SF_ERR_ALIGNMENT, "sf_int8_quantize_rows: q must be 16-byte aligned");
-    if (reinterpret_cast<uintptr_t>(x) % (dtype == SF_F32 ? 4 : 2))
-        return fail(SF_ERR_ALIGNMENT, "sf_int8_quantize_rows: x must be aligned to its elements");
+    if (!on_elements(x, dtype) || !on_elements(scale, SF_F32))
+        return fail(SF_ERR_ALIGNMENT, "sf_int8_quantize_rows: x and scale must be aligned to their elements");
     return quantize_impl(x, dtype, ld, q, scale, rows, cols, (cudaStream_t)stream);
 }
 
-static int check_product(const char* who, const void* wq, const float* ws, const void* y, int dtype, int64_t rows, int64_t in,
-                         int64_t out) {
+static int check_product(const char* who, const void* wq, const float* ws, const void* bias, const void* y, int dtype,
+                         int64_t rows, int64_t in, int64_t out, const int32_t* status) {
     if (int rc = check_int8(who, rows, in, out)) return rc;
     if (dtype != SF_F32 && dtype != SF_BF16) return fail(SF_ERR_BAD_ARG, "%s: dtype must be SF_F32 or SF_BF16", who);
     if (rows == 0) return SF_OK;
     if (!wq || !ws || !y) return fail(SF_ERR_BAD_ARG, "%s: weight, scales and y must be non-null", who);
     if (!aligned16(wq)) return fail(SF_ERR_ALIGNMENT, "%s: 8-bit operands must be 16-byte aligned", who);
+    if (!on_elements(ws, SF_F32) || !on_elements(bias, dtype) || !on_elements(y, dtype) || !on_elements(status, SF_F32))
+        return fail(SF_ERR_ALIGNMENT, "%s: scales, bias, y and status must be aligned to their elements", who);
     return SF_OK;
 }
 
 int sf_int8_gemm(const int8_t* xq, const float* x_scale, const int8_t* wq, const float* w_scale, const void* bias, void* y,
                  int dtype, int64_t rows, int64_t in, int64_t out, int32_t* status, void* stream) {
-    if (int rc = check_product("sf_int8_gemm", wq, w_scale, y, dtype, rows, in, out)) return rc;
+    if (int rc = check_product("sf_int8_gemm", wq, w_scale, bias, y, dtype, rows, in, out, status)) return rc;
     if (rows == 0) return SF_OK;
     SF_CHECK_ARG(xq && x_scale, "sf_int8_gemm: xq and x_scale must be non-null");
     if (!aligned16(xq)) return fail(SF_ERR_ALIGNMENT, "sf_int8_gemm: 8-bit operands must be 16-byte aligned");
+    if (!on_elements(x_scale, SF_F32)) return fail(SF_ERR_ALIGNMENT, "sf_int8_gemm: x_scale must be aligned to its elements");
     return gemm_impl(xq, x_scale, wq, w_scale, bias, y, dtype, rows, in, out, status, false, (cudaStream_t)stream);
 }
 
@@ -1195,14 +1201,13 @@ int64_t sf_int8_linear_workspace_bytes(int64_t rows, int64_t in) {
 
 int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const float* w_scale, const void* bias, void* y, int dtype,
                    int64_t rows, int64_t in, int64_t out, void* workspace, int32_t* status, void* stream) {
-    if (int rc = check_product("sf_int8_linear", wq, w_scale, y, dtype, rows, in, out)) return rc;
+    if (int rc = check_product("sf_int8_linear", wq, w_scale, bias, y, dtype, rows, in, out, status)) return rc;
     if (rows == 0) return SF_OK;
     const bool stream_rows = takes_stream(rows, in);
     SF_CHECK_ARG(x && (workspace || stream_rows), "sf_int8_linear: x and workspace must be non-null");
     SF_CHECK_ARG(ld >= in || rows == 1, "sf_int8_linear: ld=%lld is smaller than a row", (long long)ld);
     if (!aligned16(workspace)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: workspace must be 16-byte aligned");
-    if (reinterpret_cast<uintptr_t>(x) % (dtype == SF_F32 ? 4 : 2))
-        return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: x must be aligned to its elements");
+    if (!on_elements(x, dtype)) return fail(SF_ERR_ALIGNMENT, "sf_int8_linear: x must be aligned to its elements");
     if (stream_rows) {
         const bool vec = rows_vectorise(x, dtype, ld, rows, in);
         return dtype == SF_F32 ? stream_typed<float>(x, ld, wq, w_scale, bias, y, rows, in, out, vec, (cudaStream_t)stream)

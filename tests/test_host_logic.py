@@ -408,3 +408,32 @@ def test_int8_product_refuses_rows_that_are_no_multiple_of_16_bytes():
         xq, wq = torch.zeros(3, k, dtype=torch.int8), torch.zeros(7, (k + 15) // 16 * 16, dtype=torch.int8)
         with pytest.raises(ValueError, match="multiple of 16"):
             ops.int8_gemm(xq, torch.ones(3), wq, torch.ones(7))
+
+
+@pytest.mark.parametrize("entry", ["quantize", "gemm", "linear_one_row", "linear"])
+def test_int8_addresses_off_their_elements_are_refused(entry):
+    """Every address a kernel would load or store through is checked on the host: a misaligned one would be a device
+    fault. The addresses are invented; a call that passed all checks would fail later here, for want of a device."""
+    from sparseforge_b200 import _lib
+
+    lib, A = _lib.lib(), 4096
+    f32, bf16, bad = _lib.SF_F32, _lib.SF_BF16, -3
+
+    def product(name, dtype, **off):
+        a = {k: A + off.get(k, 0) for k in ("x", "xs", "wq", "ws", "bias", "y", "work", "status")}
+        if name == "gemm":
+            return lib.sf_int8_gemm(a["x"], a["xs"], a["wq"], a["ws"], a["bias"], a["y"], dtype, 4, 16, 8, a["status"], None)
+        rows = 1 if name == "linear_one_row" else 4
+        return lib.sf_int8_linear(a["x"], 16, a["wq"], a["ws"], a["bias"], a["y"], dtype, rows, 16, 8, a["work"], a["status"], None)
+
+    if entry == "quantize":
+        assert lib.sf_int8_quantize_rows(A, f32, 16, A, A + 2, 4, 16, None) == bad
+        assert b"scale" in lib.sf_last_error_string()
+        return
+    for dtype, step in ((f32, 2), (bf16, 1)):
+        for name in ("bias", "y"):
+            assert product(entry, dtype, **{name: step}) == bad, (name, dtype)
+    for name in ("ws", "status") + (("xs",) if entry == "gemm" else ()):
+        for step in (1, 2):
+            assert product(entry, bf16, **{name: step}) == bad, name
+    assert b"aligned" in lib.sf_last_error_string()
