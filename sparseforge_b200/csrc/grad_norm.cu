@@ -340,6 +340,12 @@ static int gn_check(const char* who, const void* const* grads, const int64_t* si
     return SF_OK;
 }
 
+static int gn_check_results(const char* who, const float* norm, const double* scratch) {
+    if (reinterpret_cast<uintptr_t>(norm) % sizeof(float) || reinterpret_cast<uintptr_t>(scratch) % sizeof(double))
+        return fail(SF_ERR_ALIGNMENT, "%s: norm and scratch must be aligned to their elements", who);
+    return SF_OK;
+}
+
 // Every output is either its own input (same address, same type) or overlaps no other tensor of the call: blocks work
 // on the tensors in any order.
 struct GnSpan {
@@ -505,6 +511,7 @@ int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* 
     if (int rc = gn_check("sf_grad_norm", grads, sizes, dtypes, count)) return rc;
     SF_CHECK_ARG(kind == GN_L2 || kind == GN_INF, "sf_grad_norm: kind must be SF_NORM_L2 or SF_NORM_INF");
     SF_CHECK_ARG(norm && scratch, "sf_grad_norm: norm and scratch must be non-null");
+    if (int rc = gn_check_results("sf_grad_norm", norm, scratch)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     int slots = 0;
     if (int rc = gn_partials(grads, sizes, dtypes, count, kind, scratch, &slots, st)) return rc;
@@ -518,6 +525,7 @@ static int clip_check(const char* who, const void* const* grads, void* const* ou
                      const int32_t* out_dt, int64_t count, double max_norm, const float* norm, int norm_written) {
     if (int rc = gn_check(who, grads, sizes, in_dt, count)) return rc;
     if (!norm) return fail(SF_ERR_BAD_ARG, "%s: norm must be non-null", who);
+    if (int rc = gn_check_results(who, norm, nullptr)) return rc;
     if (count > 0 && (!outs || !out_dt)) return fail(SF_ERR_BAD_ARG, "%s: outs and their dtypes must be non-null", who);
     if (int rc = gn_check(who, const_cast<const void* const*>(outs), sizes, out_dt, count)) return rc;
     if (!(max_norm >= 0.0)) return fail(SF_ERR_BAD_ARG, "%s: max_norm must not be negative or NaN", who);
@@ -538,6 +546,7 @@ int sf_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t
     if (int rc = clip_check("sf_clip_grad_norm", grads, outs, sizes, in_dtypes, out_dtypes, count, max_norm, norm, 1)) return rc;
     SF_CHECK_ARG(kind == GN_L2 || kind == GN_INF, "sf_clip_grad_norm: kind must be SF_NORM_L2 or SF_NORM_INF");
     SF_CHECK_ARG(scratch != nullptr, "sf_clip_grad_norm: scratch must be non-null");
+    if (int rc = gn_check_results("sf_clip_grad_norm", norm, scratch)) return rc;
     cudaStream_t st = (cudaStream_t)stream;
     int slots = 0;
     if (int rc = gn_partials(grads, sizes, in_dtypes, count, kind, scratch, &slots, st)) return rc;

@@ -437,3 +437,17 @@ def test_int8_addresses_off_their_elements_are_refused(entry):
         for step in (1, 2):
             assert product(entry, bf16, **{name: step}) == bad, name
     assert b"aligned" in lib.sf_last_error_string()
+
+
+def test_gradient_norm_results_off_their_elements_are_refused():
+    """The norm is one float, the scratch holds doubles; the addresses are invented, nothing is launched."""
+    import ctypes
+
+    from sparseforge_b200 import _lib
+
+    lib = _lib.lib()
+    P, S, D = (ctypes.c_void_p * 1)(4096), (ctypes.c_int64 * 1)(16), (ctypes.c_int32 * 1)(_lib.SF_F32)
+    for norm, scratch in ((18, 64), (17, 64), (16, 68), (16, 65)):
+        assert lib.sf_grad_norm(P, S, D, 1, 0, norm, scratch, None) == -3, (norm, scratch)
+        assert lib.sf_clip_grad_norm(P, P, S, D, D, 1, 0, 1.0, norm, scratch, None) == -3, (norm, scratch)
+    assert lib.sf_clip_grads(P, P, S, D, D, 1, 18, 1.0, None) == -3
