@@ -740,6 +740,12 @@ def _int8_weight(wq, w_scale, bias, k, dtype, dev, what):
     return out
 
 
+def _int8_status(status, dev, what):
+    """The word that a wait which ran out leaves its code in; the kernels write it from the device."""
+    if status is not None and (status.dtype != torch.int32 or status.get_device() != dev or status.numel() < 1):
+        raise TypeError(f"{what}: status must be int32 on the operands' device")
+
+
 def int8_quantize_rows(x2d):
     """(q int8 [rows, cols rounded up to 16], scale float32 [rows]): every row divided by its largest magnitude over
     127 and rounded (half to even). Rows may be strided. See ``sf_int8_quantize_rows``."""
@@ -767,6 +773,7 @@ def int8_gemm(xq, x_scale, wq, w_scale, bias=None, out_dtype=torch.bfloat16, sta
     if x_scale.device != xq.device:
         raise ValueError("int8_gemm: all tensors of a call must live on one device")
     out = _int8_weight(wq, w_scale, bias, k, out_dtype, xq.get_device(), "int8_gemm")
+    _int8_status(status, xq.get_device(), "int8_gemm")
     y = torch.empty((T, out), dtype=out_dtype, device=xq.device)
     with _on_device_of(xq):
         check(lib().sf_int8_gemm(_p(xq), _p(x_scale), _p(wq), _p(w_scale), _p(bias), _p(y), _DT[out_dtype], T, k, out,
@@ -781,6 +788,7 @@ def int8_linear(x2d, wq, w_scale, bias=None, status=None):
     T, k = x2d.shape
     dtype, dev = x2d.dtype, x2d.get_device()
     out = _int8_weight(wq, w_scale, bias, k, dtype, dev, "int8_linear")
+    _int8_status(status, dev, "int8_linear")
     y = x2d.new_empty((T, out))
     if T == 0:
         return y

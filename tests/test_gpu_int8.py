@@ -439,3 +439,17 @@ def test_clipping_sees_gradients_written_just_before():
         norm = ops.clip_grad_norm([g], 0.5)
         again = ops.grad_norm([g])
         assert torch.equal(norm, n) and torch.equal(g, o) and torch.equal(again, ops.grad_norm([o]))
+
+
+def test_status_words_the_device_cannot_write_are_refused():
+    ops = _ops()
+    x, w, _ = _inputs(4, 64, 32, torch.bfloat16)
+    xq, xs = ops.int8_quantize_rows(x)
+    wq, ws = ops.int8_quantize_rows(w)
+    good = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for bad in (good.cpu(), good.float(), good[:0]):
+        with pytest.raises((TypeError, RuntimeError)):
+            ops.int8_linear(x, wq, ws, status=bad)
+        with pytest.raises((TypeError, RuntimeError)):
+            ops.int8_gemm(xq, xs, wq, ws, status=bad)
+    assert torch.equal(ops.int8_linear(x, wq, ws, status=good), ops.int8_linear(x, wq, ws)) and not good.any()
