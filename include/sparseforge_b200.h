@@ -514,7 +514,9 @@ SF_API int sf_kl_div_bwd(const void* student, const void* teacher, int dtype, co
  *     sf_int8_pitch(cols) bytes (cols rounded up to 16), the padding zero.
  *   sf_int8_gemm: y[t, n] = float(sum_k xq[t, k] wq[n, k]) * x_scale[t] * w_scale[n] + bias[n]; xq [rows, pitch], wq
  *     [out, pitch] with zero padding beyond `in`, bias (or NULL) and y [rows, out] of `dtype`. The sum is an exact
- *     32-bit integer (in <= SF_INT8_MAX_IN), the rest fp32 with one rounding to y: a row's values do not depend on the other rows.
+ *     32-bit integer (in <= SF_INT8_MAX_IN), the rest fp32 with one rounding to y: a row's values do not depend on the other
+ *     rows. What fits y's type is not lost on the way: no product of the sum and one scale leaves fp32. Scales below 2^-126 (rows
+ *     whose largest value is below 1.5e-36) are multiples of 2^-149 and lose bits accordingly.
  *   sf_int8_linear: both, for x of y's dtype (rows of stride ld); workspace of sf_int8_linear_workspace_bytes
  *     bytes (may be 0: one or two rows need none), 16-byte aligned, holds nothing between calls; calls that may run at
  *     the same time need one each.

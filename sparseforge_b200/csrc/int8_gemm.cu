@@ -286,9 +286,20 @@ int8_quantize_any_kernel(const T* x, int64_t ld, int8_t* __restrict__ q, float* 
     }
 }
 
-// One place for the arithmetic behind the sum, so that every kernel rounds alike (bias 0 where there is none).
-__device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bias) {
+// One place for the arithmetic behind the sum, so that every kernel rounds alike (bias 0 where there is none). The sum times
+// the token's scale is formed first: rounded once, and exact where it is subnormal (an integer times a multiple of 2^-149). From
+// a scale of 2^96 on it could leave fp32 (the sum is below 2^31) though the result, after the channel's scale, does not: it
+// is formed 2^32 lower there, with the same significand, and the rest in fp64.
+constexpr float kHugeScale = 0x1p96f;
+__device__ __noinline__ float int8_out_huge(int acc, float xs, float ws, float bias) {
+    const float low = __fmul_rn(__int2float_rn(acc), xs * 0x1p-32f);
+    return __double2float_rn(__fma_rn((double)low, (double)ws * 0x1p32, (double)bias));
+}
+__device__ __forceinline__ float int8_out_usual(int acc, float xs, float ws, float bias) {
     return __fmaf_rn(__fmul_rn(__int2float_rn(acc), xs), ws, bias);
+}
+__device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bias) {
+    return xs >= kHugeScale ? int8_out_huge(acc, xs, ws, bias) : int8_out_usual(acc, xs, ws, bias);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -507,38 +518,43 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
             ptx::tc_fence_after();
             const uint32_t taddr = tmem_base + (uint32_t)(acc * 256) + ((uint32_t)(q * 32) << 16);
             constexpr int PARTS = 4 / (int)sizeof(T);  // accumulator reads of 32 columns per 128 bytes of a row
+            auto put = [&](auto out_of) {
 #pragma unroll 1
-            for (int c = 0; c < 8; c += PARTS) {
+                for (int c = 0; c < 8; c += PARTS) {
 #pragma unroll
-                for (int part = 0; part < PARTS; ++part) {
-                    const int col = (c + part) * 32;
-                    uint32_t r[32];
-                    ptx::tmem_ld_32x32b_x32(taddr + (uint32_t)col, r);
-                    ptx::tmem_ld_wait();
-                    float v[32];
+                    for (int part = 0; part < PARTS; ++part) {
+                        const int col = (c + part) * 32;
+                        uint32_t r[32];
+                        ptx::tmem_ld_32x32b_x32(taddr + (uint32_t)col, r);
+                        ptx::tmem_ld_wait();
+                        float v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        const float4 s4 = *reinterpret_cast<const float4*>(cs + col + j);
-                        const float4 b4 = *reinterpret_cast<const float4*>(cs + 256 + col + j);
-                        v[j] = int8_out((int)r[j], rs, s4.x, b4.x);
-                        v[j + 1] = int8_out((int)r[j + 1], rs, s4.y, b4.y);
-                        v[j + 2] = int8_out((int)r[j + 2], rs, s4.z, b4.z);
-                        v[j + 3] = int8_out((int)r[j + 3], rs, s4.w, b4.w);
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 s4 = *reinterpret_cast<const float4*>(cs + col + j);
+                            const float4 b4 = *reinterpret_cast<const float4*>(cs + 256 + col + j);
+                            v[j] = out_of((int)r[j], rs, s4.x, b4.x);
+                            v[j + 1] = out_of((int)r[j + 1], rs, s4.y, b4.y);
+                            v[j + 2] = out_of((int)r[j + 2], rs, s4.z, b4.z);
+                            v[j + 3] = out_of((int)r[j + 3], rs, s4.w, b4.w);
+                        }
+                        turn_in(turn + lane * I8_TURN_ROW, v, part, T());
                     }
-                    turn_in(turn + lane * I8_TURN_ROW, v, part, T());
+                    if (c + PARTS == 8) {  // the last of the accumulator has been read: the MMA warp may have it back
+                        ptx::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
+                    } else {
+                        __syncwarp();
+                    }
+                    const int col = c * 32, row0 = row - lane;
+                    if (row0 < rows && n0 + col < out)
+                        turn_out(turn, y + (int64_t)row0 * out + n0 + col, (int64_t)out, rows - row0, out - n0 - col, vec, lane);
+                    __syncwarp();  // the turn buffer and, after the last chunk, the column scales may be overwritten
                 }
-                if (c + PARTS == 8) {  // the last of the accumulator has been read: the MMA warp may have it back
-                    ptx::tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive_cluster(acc ? leader_empty1 : leader_empty0);
-                } else {
-                    __syncwarp();
-                }
-                const int col = c * 32, row0 = row - lane;
-                if (row0 < rows && n0 + col < out)
-                    turn_out(turn, y + (int64_t)row0 * out + n0 + col, (int64_t)out, rows - row0, out - n0 - col, vec, lane);
-                __syncwarp();  // the turn buffer and, after the last chunk, the column scales may be overwritten
-            }
+            };
+            // a loop of its own for huge rows: a test inside one loop took [8192, 64] x [12288, 64] from 89 to 99 us
+            if (__any_sync(0xffffffffu, rs >= kHugeScale)) put([](int a, float x, float w, float b) { return int8_out(a, x, w, b); });
+            else put([](int a, float x, float w, float b) { return int8_out_usual(a, x, w, b); });
         }
     }
 
@@ -728,6 +744,7 @@ struct I8FewTail {
     uint64_t tmem_full;
     uint32_t tmem_base;
     int abort_flag;
+    int any_huge;   // one of the scales is beyond kHugeScale
     float xs[256];  // scales of the tile's tokens
 };
 
@@ -800,7 +817,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
             ptx::mbar_init(ptx::smem_u32(&tail->empty[s]), 1);
         }
         ptx::mbar_init(ptx::smem_u32(&tail->tmem_full), 1);
-        tail->abort_flag = 0;
+        tail->abort_flag = tail->any_huge = 0;
         ptx::fence_barrier_init();
         if (PAIR == 1)  // nobody else's barriers are involved: the weights are on their way before the block is set up
             for (int s = 0; s < ahead; ++s) load(s, kb0 + s, true, false);
@@ -883,7 +900,11 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
     }
     ptx::dependency_wait();
     if (warp >= 2) {
-        for (int c = threadIdx.x - 64; c < BN; c += 128) tail->xs[c] = t0 + c < rows ? xs[t0 + c] : 0.0f;
+        for (int c = threadIdx.x - 64; c < BN; c += 128) {
+            const float scale = t0 + c < rows ? xs[t0 + c] : 0.0f;
+            tail->xs[c] = scale;
+            if (scale >= kHugeScale) tail->any_huge = 1;
+        }
         const bool done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {
             ptx::tc_fence_after();
@@ -930,16 +951,21 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
                     sum[g].x += v[g].x; sum[g].y += v[g].y; sum[g].z += v[g].z; sum[g].w += v[g].w;
                 }
             }
+            auto put = [&](auto out_of) {
 #pragma unroll
-            for (int g = 0; g < GROUP; ++g) {
-                const int c = c0 + WARPS * split * g;
-                if (c < last && valid > 0) {
-                    const float rs = tail->xs[c];
-                    const float v[4] = {int8_out(sum[g].x, rs, cs[0], cb[0]), int8_out(sum[g].y, rs, cs[1], cb[1]),
-                                        int8_out(sum[g].z, rs, cs[2], cb[2]), int8_out(sum[g].w, rs, cs[3], cb[3])};
-                    store4(y + (int64_t)(t0 + c) * out + n, v, valid, vec);
+                for (int g = 0; g < GROUP; ++g) {
+                    const int c = c0 + WARPS * split * g;
+                    if (c < last && valid > 0) {
+                        const float rs = tail->xs[c];
+                        const float v[4] = {out_of(sum[g].x, rs, cs[0], cb[0]), out_of(sum[g].y, rs, cs[1], cb[1]),
+                                            out_of(sum[g].z, rs, cs[2], cb[2]), out_of(sum[g].w, rs, cs[3], cb[3])};
+                        store4(y + (int64_t)(t0 + c) * out + n, v, valid, vec);
+                    }
                 }
-            }
+            };
+            // one test for the tile, not one per column: the columns' loads, products and stores stay interleaved
+            if (tail->any_huge) put([](int a, float xs, float ws, float b) { return int8_out(a, xs, ws, b); });
+            else put([](int a, float xs, float ws, float b) { return int8_out_usual(a, xs, ws, b); });
         }
     }
     __syncwarp();

@@ -453,3 +453,54 @@ def test_status_words_the_device_cannot_write_are_refused():
         with pytest.raises((TypeError, RuntimeError)):
             ops.int8_gemm(xq, xs, wq, ws, status=bad)
     assert torch.equal(ops.int8_linear(x, wq, ws, status=good), ops.int8_linear(x, wq, ws)) and not good.any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T,k,n", [(1, 1000, 70), (2, 1003, 64), (3, 4096, 70), (20, 500, 130), (60, 2000, 130), (300, 640, 200),
+                                   (513, 8193, 1700), (2048, 256, 1303)])
+def test_rows_at_the_ends_of_the_range_through_the_product(T, k, n, dtype):
+    """Finite rows of huge and of tiny values, against channels of all sizes: what fits the result's type comes out right even
+    where the sum times one of the scales would not fit fp32.
+
+    Tolerance: that of ``_check`` without its constant, and what the subnormal range adds. A scale below 2^-126 is a
+    multiple of 2^-149 (half a step: 2^-150, times the sum and the other scale), and so is a result (2^-150 in fp32, before
+    the bias 2^-150 again where the product alone is that small; 2^-134 in bf16)."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(7)
+    dt = DT[dtype]
+    x = torch.randn(T, k, device="cuda", generator=g).clamp_(-3, 3)
+    x[:, 1] = x[:, 0]
+    w = torch.randn(n, k, device="cuda", generator=g).clamp_(-3, 3)
+    wscale = torch.tensor([1e-3, 1e-30, 1e30, 1e-38, 1e-20, 1e34, 0.0, 1.0], device="cuda")[torch.arange(n, device="cuda") % 8]
+    w *= wscale[:, None]
+    for j, b in ((9, 1e37), (17, 1.0)):  # channels whose sum is zero for every row
+        w[j] = 0.0
+        w[j, 0], w[j, 1] = b, -b
+    w = w.to(dt)
+    bias = torch.randn(n, device="cuda", generator=g).to(dt)
+    wq, ws = ops.int8_quantize_rows(w)
+    wi, wsc = _quantise64(w)
+    top = torch.finfo(dt).max
+    # 127 * 2^96 = 1.006e31 is where the scale reaches 2^96
+    sizes = [1e36, 1e38, 1e31 / 3, 1.1e31 / 3, 1e20, 1e-37, 1e-40, 1e-20, 1e-3]
+    for first in range(0, len(sizes), 1 if T < 9 else len(sizes)):
+        rows = torch.tensor([sizes[(first + t) % len(sizes)] for t in range(T)], device="cuda")
+        xt = (x.double() * rows.double()[:, None]).clamp(-top, top).to(dt)
+        xi, xsc = _quantise64(xt)
+        total = xi @ wi.t()
+        product = total * xsc[:, None] * wsc
+        for b in (None, bias):
+            y = ops.int8_linear(xt, wq, ws, b)
+            want = product if b is None else product + b.double()
+            fits = (want.abs() < top * 0.99) & (product.abs() < torch.finfo(torch.float32).max * 0.99)
+            tol = 6 * U * product.abs() + (U + torch.finfo(dt).eps / 2) * want.abs() + 2.0 ** -149
+            tol = tol + 2.0 ** -150 * total.abs() * ((xsc < 2.0 ** -126)[:, None] * wsc + (wsc < 2.0 ** -126) * xsc[:, None])
+            if dtype == "bf16":
+                tol = tol + 2.0 ** -134
+            bad = ~((y.double() - want).abs() <= tol) & fits
+            assert not bad.any(), (int(bad.sum()), bad.nonzero()[:4].tolist())
+            over = want.abs() > top * 1.01
+            assert torch.isinf(y[over]).all() and (torch.sign(y[over].double()) == torch.sign(want[over])).all()
+            assert not torch.isnan(y).any()
+            xq, xs = ops.int8_quantize_rows(xt)
+            assert torch.equal(y, ops.int8_gemm(xq, xs, wq, ws, b, out_dtype=dt))
