@@ -538,7 +538,8 @@ SF_API int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const flo
  *   replaces: torch.nn.utils.clip_grad_norm_ between backward and optimizer.step of the training loop,
  *             legacy/main_llama.py:1997-2211.
  *   norm = sqrt(sum of g^2 over every element of every tensor), or the largest |g| (SF_NORM_INF)
- *   c    = min(1, max_norm / (norm + 1e-6)),  outs[i] = grads[i] * c, rounded once to the output's type
+ *   c    = min(1, max_norm / (norm + 1e-6)),  outs[i] = grads[i] * c
+ *   c is formed in fp64 and rounded to 24 bits, the product to fp32, and that to bf16 where the output is bf16.
  * grads, outs, sizes (elements), dtypes (SF_F32 / SF_BF16) are HOST arrays of `count` entries, read during the
  * call; the tensors are on the device, dense, of any size and element alignment (16-byte aligned ones move in
  * 16-byte accesses). norm is one fp32 on the device; scratch has sf_grad_norm_scratch_doubles(count) doubles,
@@ -549,7 +550,8 @@ SF_API int sf_int8_linear(const void* x, int64_t ld, const int8_t* wq, const flo
  * An output is its own input (clipping in place; with c = 1 it is left alone) or overlaps no other tensor of
  * the call, nor the norm; a call that breaks this, for example by naming a gradient twice, is refused.
  * sf_clip_grads takes the norm from the device (for example combined over ranks first); sf_clip_grad_norm forms it
- * and clips in one call, with the coefficient taken from the unrounded norm.
+ * and clips in one call, with the coefficient taken from the unrounded norm (which may lie beyond fp32 where the norm that
+ * is returned is infinite: finite gradients are clipped by what they amount to).
  */
 SF_API int64_t sf_grad_norm_scratch_doubles(int64_t count);
 SF_API int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,

@@ -1,7 +1,7 @@
 // Global norm of many gradient tensors, and clipping by it.
 //
 //   norm = sqrt(sum over every element of every tensor of g^2)      (or max |g|)
-//   c    = min(1, max_norm / (norm + 1e-6)),   out = g * c           (one rounding, to out's type)
+//   c    = min(1, max_norm / (norm + 1e-6)),   out = g * c           (c to 24 bits, the product to fp32 and then to out's type)
 //
 // The tensors of one call are described by a table that travels in the kernel's parameters: no copy of
 // pointers to the device, so a call is one launch for the norm and one for the scaling, and can be captured.
@@ -246,7 +246,11 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, 
         norm = (double)*norm_in;
     }
     const double ratio = max_norm / (norm + 1e-6);
-    const float c = ratio >= 1.0 ? 1.0f : (float)ratio;  // a NaN stays one
+    // A coefficient below fp32's normal range would lose bits (gradients near the top of the range, a small max_norm): it is
+    // held 2^126 higher there, and what it gives is moved back by an exact power of two.
+    const bool low = ratio < 0x1p-126;
+    const float c = ratio >= 1.0 ? 1.0f : (float)(low ? ratio * 0x1p126 : ratio);  // a NaN stays one
+    const float back = low ? 0x1p-126f : 1.0f;
     if (c == 1.0f && tab.all_in_place) return;
     const uint32_t chunks = tab.first[tab.count];
     for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
@@ -275,7 +279,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, 
                         float x[8];
                         unpack_bf16(r[u], x);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] *= c;
+                        for (int i = 0; i < 8; ++i) x[i] = x[i] * c * back;
                         Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(ov) + (v + u * kGnThreads) * kGnVec, x);
                     }
             }
@@ -298,7 +302,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, 
                         if (ib) unpack_bf16(r[u][0], x);
                         else unpack_f32(r[u][0], r[u][1], x);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[i] *= c;
+                        for (int i = 0; i < 8; ++i) x[i] = x[i] * c * back;
                         if (ob) Vec8<__nv_bfloat16>::store(reinterpret_cast<__nv_bfloat16*>(ov) + at, x);
                         else Vec8<float>::store(reinterpret_cast<float*>(ov) + at, x);
                     }
@@ -307,7 +311,7 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, 
         for (int j = threadIdx.x; j < len - nv * kGnVec; j += kGnThreads) {
             const int i = j < head ? j : j + nv * kGnVec;
             const float x = (ib ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(ip)[i])
-                                : reinterpret_cast<const float*>(ip)[i]) * c;
+                                : reinterpret_cast<const float*>(ip)[i]) * c * back;
             if (ob) reinterpret_cast<__nv_bfloat16*>(op)[i] = __float2bfloat16_rn(x);
             else reinterpret_cast<float*>(op)[i] = x;
         }

@@ -347,3 +347,36 @@ def test_every_alignment(dt, odt):
                 ref = g.double() * min(1.0, 0.5 / (w + 1e-6))
                 assert ((o.double() - ref).abs() <= _value_tol(o.dtype) * ref.abs() + 1e-40).all(), (go, oo, n)
                 assert (buf[:oo] == 7.0).all() and (buf[oo + n:] == 7.0).all()
+
+
+@pytest.mark.parametrize("p", [2.0, math.inf])
+@pytest.mark.parametrize("max_norm", [1.0, 1e-3, 1e-30, 1e-37])
+@pytest.mark.parametrize("size", [3e38, 1e36, 4e37])
+@pytest.mark.parametrize("dt,odt", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("bf16", "f32")])
+def test_coefficients_below_the_normal_range(dt, odt, size, max_norm, p):
+    """Gradients so large, or a limit so small, that max_norm / norm is subnormal or zero in fp32; with 5000 elements the
+    L2 norm itself is beyond fp32. Outputs are the formula's, to the tolerance of any other case and a subnormal step
+    (two half steps in fp32, half a step in bf16)."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(17)
+    src = [(torch.rand(n, device="cuda", generator=g) * 2 - 1).mul_(size).to(DT[dt]) for n in (5000, 37, 4099)]
+    want = _exact(src, p)
+    factor = max_norm / (want + 1e-6)
+    steps = 2.0 ** -149 + (2.0 ** -134 if odt == "bf16" else 0.0)
+
+    def check(out):
+        for s, o in zip(src, out):
+            ref = s.double() * factor
+            assert ((o.double() - ref).abs() <= _value_tol(o.dtype) * ref.abs() + steps).all()
+
+    out = [torch.empty_like(s, dtype=DT[odt]) for s in src]
+    norm = ops.clip_grad_norm(src, max_norm, p, out=out)
+    assert float(norm) == math.inf if want > 3.5e38 else abs(float(norm) - want) <= NORM_TOL * want
+    check(out)
+    if want < 3.4e38:
+        ops.clip_grads(src, norm, max_norm, out=out)
+        check(out)
+    if dt == odt:
+        here = [s.clone() for s in src]
+        ops.clip_grad_norm(here, max_norm, p)
+        check(here)
