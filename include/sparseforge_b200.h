@@ -627,6 +627,13 @@ SF_API int sf_multimem_reduce(const void* mc_src, void* out, int64_t n, int dtyp
 SF_API int sf_selftest_bounded_wait(double limit_ms, int32_t* status, void* stream);
 
 /*
+ * Bytes of gradients that launch number `launch` (of one per 448 tensors) of sf_grad_norm marks to stay in L2 for the
+ * scaling behind it: the rule by itself, on the host, nothing is launched; -1 for a bad argument. Over the launches of a
+ * call these are the list's last 64 MiB, in whole chunks. No counterpart in the reference.
+ */
+SF_API int64_t sf_selftest_grad_norm_kept_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t count, int64_t launch);
+
+/*
  * Issue-rate probe of the tensor cores (no counterpart in the reference): `ctas` thread blocks each
  * issue `iters` tcgen05.mma of shape 128 x n x 16 (bf16, fp32 accumulation) back to back, the A
  * operand read from shared memory (a_from_tmem = 0) or from tensor memory (1), and wait for them with a

@@ -89,6 +89,7 @@ _SIGNATURES = {
     "sf_multimem_reduce": (c_int, [_P, _P, c_int64, c_int, c_int, _P]),
     "sf_reduce_slots": (c_int, [_P, _P, c_int64, c_int64, c_int, _P]),
     "sf_selftest_bounded_wait": (c_int, [c_double, _P, _P]),
+    "sf_selftest_grad_norm_kept_bytes": (c_int64, [_P, _P, c_int64, c_int64]),
     "sf_selftest_mma_issue_rate": (c_int, [c_int, c_int, c_int, c_int, _P, _P, _P]),
     "sf_peer_handle_bytes": (c_int, []),
     "sf_peer_export": (c_int, [_P, _P, _P]),

@@ -18,6 +18,7 @@
 #include <cstdlib>
 
 #include <algorithm>
+#include <memory>
 #include <new>
 
 #include "common.cuh"
@@ -323,8 +324,9 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, 
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kGnCap = 448;       // tensors per launch: a table of 13 KiB, below the 32 KiB of kernel parameters
 constexpr int kGnCapSmall = 32;   // a table of 1 KiB for short lists
-// What the norm leaves in the 126 MB L2 for the scaling, which reads it first and marks it as the first to go. Norm and
-// clipping of 192 MB: 104 us with nothing kept, 100 with 32 MiB, 97 with 64, 99 with 100; 94.6 with the marked reads.
+// What the norm leaves in the 126 MB L2 for the scaling, which reads it first and marks it as the first to go: the last 64 MiB
+// of the list, over its launches. A norm alone cannot know whether a scaling follows (sf_clip_grads), so it marks them too. Norm and
+// clipping of 192 MB in bf16: 104 us with nothing kept, 100 with 32 MiB, 97 with 64, 99 with 100; 94.6 with the marked reads.
 constexpr int64_t kGnKeepBytes = 64 << 20;
 
 static int64_t gn_launches(int64_t count) { return count <= 0 ? 1 : (count + kGnCap - 1) / kGnCap; }
@@ -386,10 +388,16 @@ static int gn_grid(int64_t chunks, int blocks_per_sm) {
     return (int)std::max<int64_t>(1, std::min(chunks, cap));
 }
 
-// Fills the table with tensors [from, to). Returns the number of chunks.
+static int64_t gn_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t from, int64_t to) {
+    int64_t bytes = 0;
+    for (int64_t i = from; i < to; ++i) bytes += sizes[i] * (dtypes[i] == SF_BF16 ? 2 : 4);
+    return bytes;
+}
+
+// Fills the table with tensors [from, to), the last keep_bytes of which are marked to stay in L2. Returns the number of chunks.
 template <int CAP>
 static int64_t gn_fill(GnTable<CAP>& tab, const void* const* grads, void* const* outs, const int64_t* sizes,
-                       const int32_t* in_dt, const int32_t* out_dt, int64_t from, int64_t to) {
+                       const int32_t* in_dt, const int32_t* out_dt, int64_t from, int64_t to, int64_t keep_bytes = 0) {
     int64_t total = 0;
     for (int64_t i = from; i < to; ++i) total += sizes[i];
     // the longest chunk that still gives every block of a resident wave some; small sets get short chunks, huge
@@ -420,8 +428,16 @@ static int64_t gn_fill(GnTable<CAP>& tab, const void* const* grads, void* const*
         c += (uint32_t)((sizes[i] + chunk - 1) / chunk);
     }
     tab.first[tab.count] = c;
-    const int64_t keep = kGnKeepBytes / (chunk * 2);
-    tab.keep_from = (uint32_t)std::max<int64_t>(0, (int64_t)c - keep);
+    tab.keep_from = c;
+    for (int k = tab.count - 1; k >= 0; --k) {
+        const int64_t esize = tab.kind[k] & GN_IN_BF16 ? 2 : 4, bytes = tab.t[k].n * esize;
+        tab.keep_from = tab.first[k];
+        if (bytes > keep_bytes) {  // only the tensor's last chunks
+            tab.keep_from = tab.first[k + 1] - (uint32_t)(keep_bytes / (chunk * esize));
+            break;
+        }
+        keep_bytes -= bytes;
+    }
     return c;
 }
 
@@ -440,12 +456,18 @@ static cudaError_t gn_launch_dependent(void (*kern)(KArgs...), int grid, cudaStr
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// What the launch whose tensors end at `to` may leave in L2: the share of the whole list's last kGnKeepBytes that is not taken
+// by the launches behind it.
+static int64_t gn_keep_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t to, int64_t count) {
+    return std::max<int64_t>(0, kGnKeepBytes - gn_bytes(sizes, dtypes, to, count));
+}
+
 // Launches the partial sums of tensors [from, to); *slots grows by the number of slots written.
 template <int CAP>
 static int gn_partials_part(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t from, int64_t to,
-                            int kind, double* scratch, int* slots, cudaStream_t st) {
+                            int64_t keep_bytes, int kind, double* scratch, int* slots, cudaStream_t st) {
     GnTable<CAP> tab;
-    const int64_t chunks = gn_fill(tab, grads, nullptr, sizes, dtypes, nullptr, from, to);
+    const int64_t chunks = gn_fill(tab, grads, nullptr, sizes, dtypes, nullptr, from, to, keep_bytes);
     if (chunks == 0) return SF_OK;
     const int grid = gn_grid(chunks, kGnNormBlocks);
     if (kind == GN_INF) grad_norm_partial_kernel<CAP, true><<<grid, kGnThreads, 0, st>>>(tab, scratch + *slots);
@@ -459,10 +481,10 @@ static int gn_partials(const void* const* grads, const int64_t* sizes, const int
                        double* scratch, int* slots, cudaStream_t st) {
     *slots = 0;
     for (int64_t from = 0; from < count; from += kGnCap) {
-        const int64_t to = std::min(count, from + kGnCap);
+        const int64_t to = std::min(count, from + kGnCap), keep = gn_keep_bytes(sizes, dtypes, to, count);
         const int rc = to - from <= kGnCapSmall
-                           ? gn_partials_part<kGnCapSmall>(grads, sizes, dtypes, from, to, kind, scratch, slots, st)
-                           : gn_partials_part<kGnCap>(grads, sizes, dtypes, from, to, kind, scratch, slots, st);
+                           ? gn_partials_part<kGnCapSmall>(grads, sizes, dtypes, from, to, keep, kind, scratch, slots, st)
+                           : gn_partials_part<kGnCap>(grads, sizes, dtypes, from, to, keep, kind, scratch, slots, st);
         if (rc) return rc;
     }
     return SF_OK;
@@ -509,6 +531,23 @@ using namespace sf;
 extern "C" {
 
 int64_t sf_grad_norm_scratch_doubles(int64_t count) { return gn_launches(count) * kGnSlots; }
+
+int64_t sf_selftest_grad_norm_kept_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t count, int64_t launch) {
+    if (!sizes || !dtypes || count < 0 || launch < 0 || launch >= gn_launches(count)) return -1;
+    for (int64_t i = 0; i < count; ++i)
+        if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 42) || (dtypes[i] != SF_F32 && dtypes[i] != SF_BF16)) return -1;
+    const int64_t from = launch * kGnCap, to = std::min(count, from + kGnCap);
+    const std::unique_ptr<const void*[]> nowhere(new (std::nothrow) const void*[count ? count : 1]());
+    const std::unique_ptr<GnTable<kGnCap>> tab(new (std::nothrow) GnTable<kGnCap>);
+    if (!tab || !nowhere) return -1;
+    gn_fill(*tab, nowhere.get(), nullptr, sizes, dtypes, nullptr, from, to, gn_keep_bytes(sizes, dtypes, to, count));
+    int64_t kept = 0;
+    for (int k = 0; k < tab->count; ++k) {
+        const int64_t before = tab->keep_from > tab->first[k] ? (int64_t)(tab->keep_from - tab->first[k]) * tab->chunk : 0;
+        kept += std::max<int64_t>(0, tab->t[k].n - before) * (tab->kind[k] & GN_IN_BF16 ? 2 : 4);
+    }
+    return kept;
+}
 
 int sf_grad_norm(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,
                  float* norm, double* scratch, void* stream) {
