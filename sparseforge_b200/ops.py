@@ -18,6 +18,7 @@ from ._lib import SF_BF16, SF_F32, SF_I8, check, lib
 _GET_DTYPE = torch.Tensor.dtype.__get__
 _GRAD_DTYPES = {torch.float32, torch.bfloat16}
 _DT = {torch.float32: SF_F32, torch.bfloat16: SF_BF16, torch.int8: SF_I8}
+_GRAD_CODES = {d: _DT[d] for d in _GRAD_DTYPES}
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -445,14 +446,15 @@ def _grad_arrays(ts, what):
     if len(devices) != 1 or -1 in devices:
         _cuda(*ts)
         raise ValueError(f"{what}: all gradients of a call must live on one device")
-    dtypes = list(map(_GET_DTYPE, ts))
-    if not _GRAD_DTYPES.issuperset(dtypes):
-        raise TypeError(f"{what}: gradients must be float32 or bfloat16, got {sorted(map(str, set(dtypes)))}")
+    try:
+        codes = array("i", map(_GRAD_CODES.__getitem__, map(_GET_DTYPE, ts)))
+    except KeyError:
+        raise TypeError(f"{what}: gradients must be float32 or bfloat16, got {sorted({str(t.dtype) for t in ts})}") from None
     contiguous = all(map(torch.Tensor.is_contiguous, ts))  # raises for sparse layouts
     if not contiguous and not all(_dense_view(t).is_contiguous() for t in ts):
         raise RuntimeError("sparseforge_b200: tensors must be contiguous (or a dense permutation)")
     return (array("Q", map(torch.Tensor.data_ptr, ts)), array("q", map(torch.Tensor.numel, ts)),
-            array("i", map(_DT.__getitem__, dtypes)), contiguous)
+            codes, contiguous)
 
 
 def _clip_arrays(grads, out, what):
@@ -460,7 +462,6 @@ def _clip_arrays(grads, out, what):
     ptrs, sizes, codes, dense = _grad_arrays(grads, what)
     if out is None:
         return ptrs, ptrs, sizes, codes, codes
-    out = list(out)
     if len(out) != len(grads):
         raise ValueError(f"{what}: {len(grads)} gradients, {len(out)} outputs")
     optrs, osizes, ocodes, odense = _grad_arrays(out, what)
@@ -470,6 +471,10 @@ def _clip_arrays(grads, out, what):
                                                           for g, o in zip(grads, out))):
         raise ValueError(f"{what}: an output must have its gradient's size, and its shape and strides unless all are contiguous")
     return ptrs, optrs, sizes, codes, ocodes
+
+
+# torch's notice that a kernel it does not know wrote tensors in place: a graph that saved one of them refuses its backward
+_written = torch.autograd.graph.increment_version
 
 
 def _addr(a: array) -> int:
@@ -509,6 +514,7 @@ def clip_grads(grads, norm, max_norm, out=None) -> None:
     grads = list(grads)
     if not grads:
         return
+    out = None if out is None else list(out)
     ptrs, optrs, sizes, codes, ocodes = _clip_arrays(grads, out, "clip_grads")
     _cuda(norm)
     if norm.dtype != torch.float32 or norm.numel() != 1 or norm.device != grads[0].device:
@@ -516,6 +522,7 @@ def clip_grads(grads, norm, max_norm, out=None) -> None:
     with _on_device_of(norm):
         check(lib().sf_clip_grads(_addr(ptrs), _addr(optrs), _addr(sizes), _addr(codes), _addr(ocodes), len(grads),
                                   _p(norm), float(max_norm), _raw_stream(grads[0].get_device())), "sf_clip_grads")
+    _written(grads if out is None else out)
 
 
 def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
@@ -524,6 +531,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
     kind = _norm_kind(norm_type)
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda")
+    out = None if out is None else list(out)
     ptrs, optrs, sizes, codes, ocodes = _clip_arrays(grads, out, "clip_grad_norm")
     dev, n = grads[0].device, len(grads)
     with _on_device_of(grads[0]):
@@ -531,6 +539,7 @@ def clip_grad_norm(grads, max_norm, norm_type=2.0, out=None) -> torch.Tensor:
         scratch = torch.empty(int(lib().sf_grad_norm_scratch_doubles(n)), dtype=torch.float64, device=dev)
         check(lib().sf_clip_grad_norm(_addr(ptrs), _addr(optrs), _addr(sizes), _addr(codes), _addr(ocodes), n, kind,
                                       float(max_norm), _p(norm), _p(scratch), _raw_stream(grads[0].get_device())), "sf_clip_grad_norm")
+    _written(grads if out is None else out)
     return norm
 
 

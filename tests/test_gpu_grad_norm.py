@@ -380,3 +380,34 @@ def test_coefficients_below_the_normal_range(dt, odt, size, max_norm, p):
         here = [s.clone() for s in src]
         ops.clip_grad_norm(here, max_norm, p)
         check(here)
+
+
+@pytest.mark.parametrize("how", ["clip_grad_norm", "clip_grads", "utils"])
+def test_a_graph_that_saved_a_clipped_gradient_is_told(how):
+    """As after torch's own in-place clipping: the backward of a graph that saved the unclipped values raises instead of
+    using the clipped ones. Outputs count as written, inputs that went to other buffers do not."""
+    from sparseforge_b200 import utils
+
+    ops = _ops()
+    p = torch.nn.Parameter(torch.zeros(100, device="cuda"))
+    p.grad = torch.randn(100, device="cuda")
+    out = torch.empty_like(p.grad)
+    v = torch.ones(100, device="cuda", requires_grad=True)
+    (v * p.grad).sum().backward()
+    saved, kept = (v * p.grad).sum(), (v * out).sum()
+    ops.clip_grad_norm([p.grad], 0.5, out=[out])
+    saved.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()
+    if how == "utils":
+        utils.clip_grad_norm_([p], 0.5)
+    elif how == "clip_grad_norm":
+        ops.clip_grad_norm([p.grad], 0.5)
+    else:
+        ops.clip_grads([p.grad], ops.grad_norm([p.grad]), 0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
+    with torch.inference_mode():  # tensors without a version counter
+        g = torch.randn(10, device="cuda")
+        ops.clip_grad_norm([g], 0.5)
+        assert abs(_exact([g]) - 0.5) <= 1e-5
