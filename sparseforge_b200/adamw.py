@@ -51,6 +51,10 @@ class AdamW(Optimizer):
                     continue
                 if not p.is_cuda:
                     raise RuntimeError("sparseforge_b200.AdamW: parameters must live on a CUDA device")
+                owner = getattr(p, "_sf_owner", None)
+                layer = owner() if owner is not None else None
+                if layer is not None and layer._i8_source is not None:
+                    layer._i8_source = None  # the weight is about to move: an 8-bit form of it is out of date
                 grad = p.grad.data
                 if grad.shape != p.data.shape:
                     if grad.numel() == p.data.numel() and p.data.numel() > 0:
@@ -78,8 +82,6 @@ class AdamW(Optimizer):
                 if p.data.numel() % 8 != 0 or p.dtype not in (torch.float32, torch.bfloat16):
                     self._small_tensor_step(p, grad, mask, state, group)
                     continue
-                owner = getattr(p, "_sf_owner", None)
-                layer = owner() if owner is not None else None
                 wm, hx = (None, 1.0)
                 ams = state.get("max_exp_avg_sq") if group["amsgrad"] else None
                 fused = layer._optimizer_score_target() if (layer is not None and mask is not None and ams is None) \

@@ -363,6 +363,7 @@ class SparseLinear(nn.Linear):
         """``.to(dtype)`` / ``.half()`` / ``.bfloat16()`` convert the weight; the soft mask and the
         Hessian diagonal stay float32 (the kernels read them as such), moved to the new device."""
         keep = {n: getattr(self, n).data for n in ("mask", "hessian_diag") if not self._is_placeholder(n)}
+        int8_current = self._int8_current()
         out = super()._apply(fn, recurse) if recurse is not True else super()._apply(fn)
         for n, old in keep.items():
             prm = getattr(self, n)
@@ -371,6 +372,8 @@ class SparseLinear(nn.Linear):
         for n in ("_i8_weight", "_i8_scale", "_i8_status"):  # 8-bit inference form: moved, never converted
             if getattr(self, n, None) is not None:
                 setattr(self, n, getattr(self, n).to(self.weight.device))
+        if int8_current:  # the conversion of the weight is not a change that the 8-bit form misses
+            self._i8_source = self._int8_source(baked=self._i8_source[1] is not None)
         self.weight.mask = self.mask
         self.weight._sf_owner = weakref.ref(self)
         self._wm_key = None
@@ -556,7 +559,12 @@ class SparseLinear(nn.Linear):
     def invalidate_masked_weight(self):
         """Call after changing ``weight``, ``mask`` or ``hessian_diag`` through ``.data`` (edits that
         autograd's version counters do not see) outside ``update_mask`` / the AdamW of this package:
-        drops the cached masked weight and the score the optimizer pass may have left."""
+        drops the cached masked weight and the score the optimizer pass may have left; an 8-bit inference form counts as
+        out of date from then on."""
+        self._drop_caches()
+        self._i8_source = None
+
+    def _drop_caches(self):
         self._wm_key = None
         self._score_key = None
 
@@ -702,7 +710,10 @@ class SparseLinear(nn.Linear):
         ``"int8_forward"``: a call quantises its input rows on the fly, one scale per token, and multiplies in 8
         bits with an exact 32-bit sum (``ops.int8_linear``). Any hard view; float32 or bfloat16 weights of any size.
         ``bake=False`` takes the weight as it is (its zeros are already in place). No counterpart in the
-        reference, whose inference bake-in stays dense (legacy/eval_wiki_ppl.py:548-651). Forward only; the weight is kept."""
+        reference, whose inference bake-in stays dense (legacy/eval_wiki_ppl.py:548-651). Forward only; the weight is kept, and its
+        memory may be released. The 8-bit form is not in the state dict and does not follow the weight: after a change
+        of the weight (or of a baked mask: ``load_state_dict``, an optimizer step, a mask update,
+        ``invalidate_masked_weight``) the mode raises until this is called again; ``.to()`` and copies of the module keep it."""
         if self.weight.dtype not in (torch.float32, torch.bfloat16):
             raise TypeError(f"quantize_for_inference: float32 or bfloat16 weights expected, got {self.weight.dtype}")
         w = self.weight.data
@@ -710,21 +721,69 @@ class SparseLinear(nn.Linear):
             w = w * self._hard_mask_from_soft(self.mask.data).to(w.dtype)
         self._i8_weight, self._i8_scale = ops.int8_quantize_rows(w.contiguous())
         self._i8_status = torch.zeros(4, dtype=torch.int32, device=w.device)
+        self._i8_source = self._int8_source(baked=bake)
         self.mode = "int8_forward"
         self._inference_optimized = True
         return self
 
+    _i8_weight = None  # [out, in rounded up to 16] int8, or no 8-bit form
+    _i8_source = None  # what it was made from; None: nothing, or out of date
+
+    @staticmethod
+    def _content_state(t):
+        """(address, version): changes with the tensor's memory and with every write that autograd's version counters see.
+        Inference tensors have none (-1)."""
+        return t.data_ptr(), -1 if t.is_inference() else t._version
+
+    def _int8_source(self, baked: bool):
+        return self._content_state(self.weight), self._content_state(self.mask) if baked else None
+
+    def _int8_current(self) -> bool:
+        """The weight (and the mask, where it was baked in) are what the 8-bit form was made from, or their memory was
+        released since. Asked in every call."""
+        if self._i8_source is None:
+            return False
+        prm, (weight, mask) = self._parameters, self._i8_source
+        return self._is_as_it_was(prm.get("weight"), weight) and (mask is None or self._is_as_it_was(prm.get("mask"), mask))
+
+    @staticmethod
+    def _is_as_it_was(t, was) -> bool:
+        if t is None or (t.data_ptr() == was[0] and (was[1] < 0 or t._version == was[1])):
+            return True
+        return t.numel() == 0
+
+    def _int8_mask_written(self):
+        """A kernel wrote the mask (no version counter moved)."""
+        if self._i8_source is not None and self._i8_source[1] is not None:
+            self._i8_source = None
+
+    def __getstate__(self):
+        """Copies and pickles have memory of their own: whether the 8-bit form is current travels, not addresses."""
+        state = super().__getstate__().copy()
+        if self._i8_source is not None:
+            state["_i8_source"] = ("copied", self._i8_source[1] is not None) if self._int8_current() else None
+        return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if self._i8_source is not None:
+            self._i8_source = self._int8_source(baked=self._i8_source[1])
+
     def _int8_forward(self, x):
         if torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad and self.training):
             raise RuntimeError("mode 'int8_forward' is inference only; call it under torch.no_grad() / eval()")
-        if getattr(self, "_i8_weight", None) is None:
+        if self._i8_weight is None:
             raise RuntimeError("mode 'int8_forward' without an 8-bit weight: call quantize_for_inference()")
+        if not self._int8_current():
+            raise RuntimeError("mode 'int8_forward': the weight or the mask has changed since quantize_for_inference(); call it again")
         x2d = x.reshape(-1, self.in_features)
         if x2d.dtype not in (torch.float32, torch.bfloat16):
             x2d = x2d.to(torch.float32)  # float16 values are exact in float32
         if x2d.stride(1) != 1 or x2d.stride(0) < self.in_features:  # rows may be strided, not interleaved or repeated
             x2d = x2d.contiguous()
-        bias = self.bias if self.bias is None or self.bias.dtype == x2d.dtype else self.bias.to(x2d.dtype)
+        bias = self.bias
+        if bias is not None and bias.dtype != x2d.dtype:
+            bias = bias.to(x2d.dtype)
         y = ops.int8_linear(x2d, self._i8_weight, self._i8_scale, bias, status=self._i8_status)
         return y.view(*x.shape[:-1], self.out_features).to(x.dtype)
 
@@ -1127,6 +1186,7 @@ class SparseLinear(nn.Linear):
         self.weight.flipped_mask = _LazyInt(self._stats, _lib.MSTAT_FLIPS)
         self.weight.init_flipped_mask = 0
         self.weight.mask = self.mask
+        self._int8_mask_written()
 
     def _block_gate(self, step: int):
         """Per-block gate of legacy/sparse_modeling.py:1122-1157: RMS of the normalised score over each
@@ -1185,6 +1245,7 @@ class SparseLinear(nn.Linear):
         self.weight.flipped_mask = _LazyInt(self._stats, _lib.MSTAT_FLIPS)
         self.weight.init_flipped_mask = 0
         self.weight.mask = self.mask
+        self._int8_mask_written()
 
     def _launch_mask_update(self, score, norm, step, *, pen, pmode, tau, owner, score_bf16=False, pen_mask=None):
         """The fused update kernel on this layer's mask with the gate schedule (temperature, mask_lr,
@@ -1221,6 +1282,7 @@ class SparseLinear(nn.Linear):
         self.weight.flipped_mask = _LazyInt(self._stats, _lib.MSTAT_FLIPS)
         self.weight.init_flipped_mask = 0
         self.weight.mask = self.mask
+        self._int8_mask_written()
 
 
 class _LazyInt:

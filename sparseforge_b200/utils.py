@@ -51,7 +51,7 @@ def sync_weight(model, device=None):
         model = model.to(device)
     for m in _sparse_modules(model):
         m.sync_weight()
-        m.invalidate_masked_weight()
+        m._drop_caches()
 
 
 @torch.no_grad()
@@ -521,6 +521,7 @@ def optimize_sparse_model_for_inference(model, use_slorb: bool = False, compress
                 m.weight.data.mul_(hard_w)
             else:
                 m.mask.data.copy_(hard.to(m.mask.dtype))
+            m.invalidate_masked_weight()
         if can_dense:
             if int8 and m.weight.dtype in (torch.float32, torch.bfloat16):
                 m.quantize_for_inference(bake=False)
@@ -530,7 +531,7 @@ def optimize_sparse_model_for_inference(model, use_slorb: bool = False, compress
             else:
                 m.mode = "dense_forward"
         m._inference_optimized = True
-        m.invalidate_masked_weight()
+        m._drop_caches()
         optimized += 1
     return model
 

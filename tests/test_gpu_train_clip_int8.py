@@ -177,3 +177,58 @@ def test_clipping_feeds_the_optimizer_like_torch_does():
     assert abs(n1 - n2) <= 64 * 2.0 ** -24 * n2 and math.isfinite(n1) and n1 > 0.1
     assert (w1 - w2).abs().max() <= 1e-2 * 200 * 2.0 ** -24 + 2.0 ** -22 * w2.abs().max()
     assert (b1 - b2).abs().max() <= 1e-2 * 200 * 2.0 ** -24 + 2.0 ** -22 * b2.abs().max()
+
+
+def test_training_on_outdates_the_8_bit_form():
+    """An evaluation in 8 bits between training steps: the optimizer's kernel and the mask update write weight and mask
+    where no version counter sees it; the layer refuses to answer from the old weights until it is quantised again."""
+    import copy
+
+    import sparseforge_b200 as sf
+    from sparseforge_b200 import utils as U
+
+    x = torch.randn(12, 64, device=DEV)
+
+    def answers(layer):
+        mode, layer.mode = layer.mode, "int8_forward"
+        try:
+            with torch.no_grad():
+                return layer.eval()(x)
+        finally:
+            layer.mode = mode
+            layer.train()
+
+    for cfg in (dict(), dict(N=4, M=8), dict(mask_type="unstructured", hard_mask_type="block16", sparsity_ratio=0.5)):
+        layer = _layer(64, 48, torch.float32, change_mask=True, mask_metric="magnitude", **cfg).train()
+        opt = sf.AdamW(layer.parameters(), lr=1e-2, betas=(0.9, 0.95), weight_decay=0.1)
+        for step in range(3):
+            layer.quantize_for_inference()
+            layer.mode = "sparse_forward"
+            first = answers(layer)
+            assert torch.equal(answers(copy.deepcopy(layer)), first)
+            layer(x).square().mean().backward()
+            assert torch.equal(answers(layer), first)  # neither pass of a training step has moved anything yet
+            opt.step()
+            with pytest.raises(RuntimeError, match="changed"):
+                answers(layer)
+            layer.quantize_for_inference()
+            layer.mode = "sparse_forward"
+            answers(layer)
+            U.calculate_model_mask(layer, step)
+            with pytest.raises(RuntimeError, match="changed"):
+                answers(layer)
+            opt.zero_grad()
+    m = torch.nn.Sequential(_layer(64, 48, torch.bfloat16))
+    U.optimize_sparse_model_for_inference(m, int8=True)
+    with torch.no_grad():
+        y = m(x.bfloat16())
+    state = {k: torch.randn_like(v) for k, v in m.state_dict().items()}
+    m.load_state_dict(state)
+    with pytest.raises(RuntimeError, match="changed"), torch.no_grad():
+        m(x.bfloat16())
+    U.optimize_sparse_model_for_inference(m, int8=True)
+    w = m[0].weight.data
+    with torch.no_grad():
+        z = m(x.bfloat16())
+    _check(z, *_exact(x.bfloat16(), w, m[0].bias.data), torch.bfloat16)
+    assert not torch.equal(y, z)

@@ -479,3 +479,108 @@ def test_what_the_gradient_norm_leaves_in_l2():
     assert (a, b, c) == (0, 62 * MiB, 2 * MiB)
     assert kept([MiB] * 448 + [32 * MiB], [F] * 449) == [0, 64 * MiB]
     assert lib.sf_selftest_grad_norm_kept_bytes(None, None, 1, 0) == -1
+
+
+def _int8_layer_without_a_gpu(monkeypatch, baked):
+    """A layer in 8-bit mode; the two kernels are stood in for by plain products (there is no CPU path)."""
+    import sparseforge_b200 as sf
+    from sparseforge_b200 import ops
+
+    def quantize(w):
+        return w.clone(), torch.ones(w.shape[0])
+
+    def linear(x, wq, ws, bias=None, status=None):
+        return x @ wq.to(x.dtype).t() + (0 if bias is None else bias)
+
+    monkeypatch.setattr(ops, "int8_quantize_rows", quantize)
+    monkeypatch.setattr(ops, "int8_linear", linear)
+    layer = sf.SparseLinear(8, 16, sparselinear_config=sf.SparseLinearConfig(mask_type="structured"), bias=True).eval()
+    monkeypatch.setattr(layer, "_hard_mask_from_soft", lambda m: (m > 0.5).to(m.dtype))
+    return layer.quantize_for_inference(bake=baked)
+
+
+def _load(layer):
+    layer.load_state_dict({k: torch.randn_like(v) for k, v in layer.state_dict().items()})
+
+
+def _in_place(layer):
+    with torch.no_grad():
+        layer.weight.mul_(2.0)
+
+
+def _other_memory(layer):
+    layer.weight.data = torch.randn_like(layer.weight)
+
+
+def _through_data(layer):
+    layer.weight.data.mul_(2.0)
+    layer.invalidate_masked_weight()
+
+
+def _mask(layer):
+    with torch.no_grad():
+        layer.mask.fill_(0.0)
+
+
+@pytest.mark.parametrize("change", [_load, _in_place, _other_memory, _through_data, _mask])
+@pytest.mark.parametrize("baked", [False, True])
+def test_an_8_bit_form_of_other_weights_is_refused(monkeypatch, change, baked):
+    layer = _int8_layer_without_a_gpu(monkeypatch, baked)
+    x = torch.randn(3, 8)
+    with torch.no_grad():
+        before = layer(x)
+        change(layer)
+        if change is _mask and not baked:  # the mask is not part of this form
+            assert torch.equal(layer(x), before)
+            return
+        with pytest.raises(RuntimeError, match="changed"):
+            layer(x)
+        layer.quantize_for_inference(bake=baked)
+        w = layer.weight * (layer.mask > 0.5) if baked else layer.weight
+        assert torch.allclose(layer(x), x @ w.t() + layer.bias)
+
+
+@pytest.mark.parametrize("baked", [False, True])
+def test_an_8_bit_form_stays_with_a_layer_that_moves_or_is_copied(monkeypatch, baked):
+    import copy
+
+    layer = _int8_layer_without_a_gpu(monkeypatch, baked)
+    monkeypatch.undo()
+    monkeypatch.setattr("sparseforge_b200.ops.int8_linear", lambda x, wq, ws, bias=None, status=None: x @ wq.to(x.dtype).t() + bias)
+    x = torch.randn(3, 8)
+    with torch.no_grad():
+        want = layer(x)
+        # reading, mode changes, gradients, .to(), sync and a changed bias do not touch what the form was made from
+        layer.state_dict()
+        layer.requires_grad_(False).requires_grad_(True)
+        layer.mode = "dense_forward"
+        layer.mode = "int8_forward"
+        layer.sync_weight()
+        assert torch.equal(layer(x), want)
+        twin = copy.deepcopy(layer)
+        assert torch.equal(twin(x), want) and twin.weight.data_ptr() != layer.weight.data_ptr()
+        assert torch.equal(layer.double().float()(x), want)
+        with torch.inference_mode():
+            assert torch.equal(layer(x), want)
+        layer.weight.data = torch.empty(0)  # its memory released
+        assert torch.equal(layer(x), want)
+        # a copy knows of its own changes only, and a copy of an outdated layer is outdated
+        twin.weight.mul_(2.0)
+        assert torch.equal(layer(x), want)
+        for outdated in (twin, copy.deepcopy(twin)):
+            with pytest.raises(RuntimeError, match="changed"):
+                outdated(x)
+
+
+def test_sync_weight_keeps_an_8_bit_form(monkeypatch):
+    from sparseforge_b200 import utils
+
+    layer = _int8_layer_without_a_gpu(monkeypatch, True)
+    x = torch.randn(3, 8)
+    with torch.no_grad():
+        want = layer(x)
+        utils.sync_weight(torch.nn.Sequential(layer))
+        assert torch.equal(layer(x), want)
+        utils.initialize_model(torch.nn.Sequential(layer))  # the mask starts anew
+        with pytest.raises(RuntimeError, match="changed"):
+            layer(x)
