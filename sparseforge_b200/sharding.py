@@ -53,16 +53,17 @@ def clip_grad_norm_(model: nn.Module, max_norm, norm_type=2.0) -> torch.Tensor:
     numbers; nothing is read back to the host. Without a process group this is ``utils.clip_grad_norm_``."""
     from . import ops
 
+    ready = dist.is_available() and dist.is_initialized()
     local, groups = set(), set()
     for m in model.modules():
         if isinstance(m, (RowShardedLinear, PeerShardedLinear)):
             local.update(id(p) for p in m.shard.parameters())
-            groups.add(m.group)
+            groups.add(dist.group.WORLD if m.group is None and ready else m.group)  # two names of the default group
     if len(groups) > 1:
         raise ValueError("clip_grad_norm_: the model's sharded layers must share one process group")
     grads = [(p.grad, id(p) in local) for p in model.parameters() if p.grad is not None]
     group = next(iter(groups), None)
-    world = dist.get_world_size(group) if (groups and dist.is_available() and dist.is_initialized()) else 1
+    world = dist.get_world_size(group) if (groups and ready) else 1
     if world == 1:
         every = [g for g, _ in grads]
         return ops.clip_grad_norm(every, max_norm, norm_type) if every else torch.tensor(0.0)

@@ -235,3 +235,45 @@ def test_clipping_with_row_shards_uses_the_whole_models_norm():
     assert all(p.exitcode == 0 for p in procs), [p.exitcode for p in procs]
     results = dict(q.get(timeout=10) for _ in range(world))
     assert results == {0: True, 1: True}
+
+
+def _clip_default_group_worker(rank, world, port, out_q):
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port), RANK=str(rank), WORLD_SIZE=str(world))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    try:
+        from sparseforge_b200 import ops, sharding
+
+        ops.grad_norm, ops.clip_grads = _plain_norm, _plain_clip
+        g = torch.Generator().manual_seed(5)
+        full = [torch.randn(32, 8, generator=g), torch.randn(32, 8, generator=g)]
+        lo, hi = sharding.shard_bounds(32, world, rank)
+        model = torch.nn.Sequential(*(sharding.RowShardedLinear(torch.nn.Linear(8, hi - lo, bias=False), group)
+                                      for group in (None, dist.group.WORLD)))
+        for layer, f in zip(model, full):
+            layer.shard.weight.grad = f[lo:hi].clone()
+        norm = sharding.clip_grad_norm_(model, 0.5)
+        ok = torch.allclose(norm, _plain_norm(full), rtol=1e-6)
+        # a group that is another one stays refused
+        model[1].group = dist.new_group(list(range(world)))
+        try:
+            sharding.clip_grad_norm_(model, 0.5)
+            ok = False
+        except ValueError:
+            pass
+        out_q.put((rank, bool(ok)))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_clipping_knows_the_default_group_by_both_names():
+    world, port = 2, _free_port()
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_clip_default_group_worker, args=(r, world, port, q)) for r in range(world)]
+    for p in procs:
+        p.start()
+    for p in procs:
+        p.join(timeout=180)
+    assert all(p.exitcode == 0 for p in procs), [p.exitcode for p in procs]
+    results = dict(q.get(timeout=10) for _ in range(world))
+    assert results == {0: True, 1: True}
