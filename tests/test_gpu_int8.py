@@ -504,3 +504,50 @@ def test_rows_at_the_ends_of_the_range_through_the_product(T, k, n, dtype):
             assert not torch.isnan(y).any()
             xq, xs = ops.int8_quantize_rows(xt)
             assert torch.equal(y, ops.int8_gemm(xq, xs, wq, ws, b, out_dtype=dt))
+
+
+@pytest.mark.parametrize("T", [1, 2, 9, 40, 200, 600])
+@pytest.mark.parametrize("captured", [False, True])
+def test_values_of_a_forked_call(T, captured):
+    """A call on a second stream, right behind the kernel that writes its input there, while weight, scales and bias were
+    copied on the first stream ahead of the fork and the quantiser runs beside it: its values, eagerly and in a graph."""
+    ops = _ops()
+    k, n = 1024, 1500
+    g = torch.Generator(device="cuda").manual_seed(T + 1)
+    xs = [torch.randn(T, k, device="cuda", generator=g).bfloat16() for _ in range(4)]
+    ws = [ops.int8_quantize_rows(torch.randn(n, k, device="cuda", generator=g).bfloat16()) for _ in range(4)]
+    raw = torch.randn(n, k, device="cuda", generator=g).bfloat16()
+    bs = [torch.randn(n, device="cuda", generator=g).bfloat16() for _ in range(4)]
+    want = [ops.int8_linear(xs[i], *ws[i], bs[i]) for i in range(4)]
+    beside = [ops.int8_linear(xs[i], *ops.int8_quantize_rows(raw), bs[i]) for i in range(4)]
+    torch.cuda.synchronize()
+    x, wq, sc, b = torch.empty_like(xs[0]), torch.empty_like(ws[0][0]), torch.empty_like(ws[0][1]), torch.empty_like(bs[0])
+    got, got_beside = [torch.empty_like(y) for y in want], [torch.empty_like(y) for y in want]
+    side = torch.cuda.Stream()
+
+    def run():
+        now = torch.cuda.current_stream()
+        for i in range(4):
+            x.fill_(float("nan"))
+            sc.copy_(ws[i][1])
+            b.copy_(bs[i])
+            wq.copy_(ws[i][0])
+            side.wait_stream(now)
+            with torch.cuda.stream(side):
+                torch.add(xs[i], 0.0, out=x)
+                got[i].copy_(ops.int8_linear(x, wq, sc, b))
+            q, s = ops.int8_quantize_rows(raw)
+            now.wait_stream(side)
+            got_beside[i].copy_(ops.int8_linear(x, q, s, b))
+
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+    for _ in range(3):
+        for t in got + got_beside:
+            t.zero_()
+        graph.replay() if captured else run()
+        torch.cuda.synchronize()
+        for a, w in zip(got + got_beside, want + beside):
+            assert torch.equal(a, w)
