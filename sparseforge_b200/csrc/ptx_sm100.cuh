@@ -205,12 +205,6 @@ __host__ __device__ constexpr uint32_t make_idesc_i8(int m, int n) {
            ((uint32_t)(m >> 4) << 24);
 }
 
-// Untiled copy global -> shared (both addresses and the size multiples of 16 bytes), counted on an mbarrier.
-__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
-}
 // Asks for `bytes` (a multiple of 16, from a 16-byte boundary) to be brought into L2. Nothing reaches the SM: harmless
 // whatever another kernel does to the bytes meanwhile.
 __device__ __forceinline__ void prefetch_l2(const void* src, uint32_t bytes) {
