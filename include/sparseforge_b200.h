@@ -629,7 +629,7 @@ SF_API int sf_selftest_bounded_wait(double limit_ms, int32_t* status, void* stre
 /*
  * Bytes of gradients that launch number `launch` (of one per 448 tensors) of sf_grad_norm marks to stay in L2 for the
  * scaling behind it: the rule by itself, on the host, nothing is launched; -1 for a bad argument. Over the launches of a
- * call these are the list's last 64 MiB, in whole chunks. No counterpart in the reference.
+ * call these are the list's last 80 MiB, in whole chunks. No counterpart in the reference.
  */
 SF_API int64_t sf_selftest_grad_norm_kept_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t count, int64_t launch);
 

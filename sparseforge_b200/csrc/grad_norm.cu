@@ -324,10 +324,11 @@ grad_clip_kernel(const __grid_constant__ GnTable<CAP> tab, const double* slots, 
 // ---------------------------------------------------------------------------------------------------------
 constexpr int kGnCap = 448;       // tensors per launch: a table of 13 KiB, below the 32 KiB of kernel parameters
 constexpr int kGnCapSmall = 32;   // a table of 1 KiB for short lists
-// What the norm leaves in the 126 MB L2 for the scaling, which reads it first and marks it as the first to go: the last 64 MiB
-// of the list, over its launches. A norm alone cannot know whether a scaling follows (sf_clip_grads), so it marks them too. Norm and
-// clipping of 192 MB in bf16: 104 us with nothing kept, 100 with 32 MiB, 97 with 64, 99 with 100; 94.6 with the marked reads.
-constexpr int64_t kGnKeepBytes = 64 << 20;
+// What the norm leaves in the 126 MB L2 for the scaling, which reads it first and marks it as the first to go: the last 80 MiB
+// of the list, over its launches. A norm alone cannot know whether a scaling follows (sf_clip_grads), so it marks them too.
+// One decoder layer, inputs not in L2 before: with 64 / 80 / 96 / 128 MiB bf16 takes 197.4 / 197.8 / 198.3 / 199.0 us, fp32
+// clipped into bf16 (which displaces less) 324.0 / 320.9 / 320.9 / 321.7. Nothing kept: 7 % more on 192 MB of bf16.
+constexpr int64_t kGnKeepBytes = 80 << 20;
 
 static int64_t gn_launches(int64_t count) { return count <= 0 ? 1 : (count + kGnCap - 1) / kGnCap; }
 
