@@ -22,11 +22,12 @@ constexpr int kQVecResident = 2048;  // threads per SM of the register-resident 
 
 // The integer nearest to 127 x / a (ties to even) for |x| <= a, decided as if the quotient were exact, from a
 // multiplication by an approximate 127 / a (relative error below 2^-22: the reciprocal's 2^-23, two roundings).
-//  bf16: with gap the number of powers of two that |x| is below a, the quotient is about 2^(7 - gap); 127 x and a being integers of
+//  bf16: with gap the number of powers of two that |x| is below a, the quotient is below 2^(7 - gap); 127 x and a being integers of
 //        15 and 8 bits times a power of two, a quotient that is not half-way between integers is at least 2^-(9 + gap) away
-//        from it, and the product is within 2^-(15 + gap): it decides all but ties. A tie needs 254 x / a odd: x = a / 2
-//        (63.5, to the even 64), since 127 divides no 8-bit significand but 254. So the factor is raised by 2^-21,
-//        more than its error, which sends ties away from zero; rows whose a has the significand 254 take quotients.
+//        from it. A tie needs 254 x / a odd: x = a / 2 (63.5, to the even 64), since 127 divides no 8-bit significand but
+//        254. So the factor is raised by 2^-21, more than its error, which sends ties away from zero; with the raise the
+//        product is within 2^-(13.4 + gap) of the quotient (2^-21 + 2^-22 of it), which decides everything else. Rows whose a
+//        has the significand 254 take quotients.
 //  fp32: where the product is closer than 2^-14 to a half the quotient is formed, in fp64 (31 and 53 bits, as above).
 // Where the reciprocal would leave the normal range every element of the row takes the quotient.
 constexpr float kClear = 0.5f - 0x1p-14f;  // a rounding that moved the value by no more leaves no doubt
@@ -341,7 +342,8 @@ __device__ __forceinline__ void i8_tile_coords(int tile, int tiles_m, int tiles_
 // Results leave through a turn buffer in shared memory, 128 bytes of 32 rows at a time (64 bf16 or 32 fp32 columns): a
 // thread holds one row, a store instruction then covers whole rows: four rows x 128 bytes in 16-byte pieces, or, where
 // rows are not on 16-byte boundaries, 32 consecutive elements of one row. Stored straight from the threads that hold a row
-// each, an odd number of channels cost [8192, 4096] x [4095, 4096] 348 us instead of 88.
+// each, an odd number of channels cost [8192, 4096] x [4095, 4096] 348 us instead of 88 in bf16. In fp32, where a row of 128 bytes
+// holds half as many columns, unaligned rows still cost more: [2048, 512] x [9001, 512] 47 us, x [9000, 512] 25 us.
 constexpr int I8_TURN_ROW = 128 + 16;  // padding against bank conflicts
 constexpr int I8_TURN_BYTES = 32 * I8_TURN_ROW;
 
@@ -574,7 +576,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
 // never more than one piece long. The first pieces are requested before the block quantises the tokens into shared
 // memory: each block repeats that small work, which saves a launch and a wait. Pieces' sums meet in shared memory (integer
 // additions: their order does not matter). [1, 4096] x [4096, 4096]: 5.9 us, x [11008, 4096]: 10.2 us, [1, 11008] x [4096,
-// 11008]: 11.0 us back to back; from the end of the kernel ahead the weights are in within 5.8 us of the 10.2.
+// 11008]: 11.0 us back to back; from the end of the kernel ahead the weights are in within 5.8 us of the 10.2. The 64 registers of
+// 1024 threads do not hold both pieces beside the quantiser: 20 to 92 bytes per thread are spilled around it.
 // ---------------------------------------------------------------------------------------------------------
 constexpr int GV_WARPS = 32, GV_THREADS = 32 * GV_WARPS;
 constexpr int GV_LOADS = 4, GV_PIECE = GV_LOADS * 512;
@@ -1032,8 +1035,11 @@ template <typename T>
 static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* scale, int64_t rows, int64_t cols,
                           cudaStream_t st) {
     const int pitch = (int)((cols + 15) / 16 * 16);
-    // A warp per row up to 1024 elements, a block per row up to 32768, all of the row in registers. [8192, 4096] bf16: 17.7 us
-    // (5.7 TB/s) with 128 threads per row, 18.9 with 256, 21.5 with 512; [8192, 11008]: 44.3 us (6.1 TB/s).
+    // A warp per row up to 1024 elements, a block per row up to 32768, the row and the next one held in registers: [8192, 4096]
+    // bf16: 17.7 us (5.7 TB/s) with 128 threads per row, 18.9 with 256, 21.5 with 512; [8192, 11008]: 44.3 us (6.1 TB/s). fp32
+    // rows take twice the registers: [8192, 4096] 30.5 us (5.5 TB/s), [8192, 11008] 106 us (4.2 TB/s). In fp32 beyond 16384 two rows do
+    // not fit the 64 registers of 1024 threads (368 bytes of spills per thread): [2048, 20000] 80 us, [2048, 32768] 101 us
+    // (2.5 and 3.3 TB/s).
 #define SF_I8_QUANT(THREADS, TPR, NV)                                                                                 \
     do {                                                                                                              \
         auto kern = int8_quantize_vec_kernel<T, THREADS, TPR, NV>;                                                    \
@@ -1052,7 +1058,8 @@ static int quantize_typed(const T* x, bool vec, int64_t ld, int8_t* q, float* sc
     } else if (vec && cols <= 32768) {
         SF_I8_QUANT(1024, 1024, 4);
 #undef SF_I8_QUANT
-    // unaligned rows; a warp per row where there are many short ones
+    // Unaligned rows; a warp per row where there are many short ones. Blocks leave after their rows, with nothing under way
+    // while they reduce and round: [8192, 4095] bf16 30 us (3.4 TB/s), fp32 35 us (4.8 TB/s), [512, 11007] bf16 7.3 us.
 #define SF_I8_QUANT_ANY(TPR, NV)                                                                                      \
     SF_CHECK_CUDA(launch_dependent(int8_quantize_any_kernel<T, TPR, NV>, (int)((rows + kQThreads / TPR - 1) / (kQThreads / TPR)), \
                                    kQThreads, 0, 1, true, st, x, ld, q, scale, (int)rows, (int)cols, pitch))
@@ -1160,10 +1167,16 @@ static int gemm_typed(const int8_t* xq, const float* xs, const int8_t* wq, const
     const int pitch = (int)((in + 15) / 16 * 16);
     if (rows <= 16) return launch_few<T, 16, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
     if (rows <= 32) return launch_few<T, 32, 1>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);
-    // More rows. While 128 x 64 tiles fit the chip at two per SM they are the fastest ([512, 4096] x [4096, 4096]: 16.0 us, 256 x
-    // 256 tiles cut in two 16.4, persistent 17.5; [128, 4096] x [11008, 4096]: 16.0, 18.4, 19.1), but their operands are
-    // loaded more often: past 256 rows a long reduction takes 256 x 256 tiles cut in two where those fill half of the SMs and
-    // fit all ([512, 11008] x [4096, 11008]: 25.4 us against 31.8 and 33.6). Beyond that, persistent tiles.
+    // More rows. While 128 x 64 tiles fit the chip at two per SM they are mostly the fastest, but their operands are loaded more
+    // often: past 256 rows a long reduction takes 256 x 256 tiles cut in two where those fill half of the SMs and fit all. Beyond
+    // that, persistent tiles. Graph times in us of 128 x 64 / cut / persistent tiles, over weights not in L2:
+    //   [512, 4096] x [4096, 4096]   17.7 / 18.2 / 19.6     [512, 12288] x [4096, 12288]  39.1 / 30.6 / 41.3
+    //   the reduction (8192):  [512, 6144] x [4096, 6144] 22.7 / 22.0 / 25.5, [320, 8192] x [4096, 8192] 26.6 / 23.3 / 29.6
+    //   the count (19 to 37):  16 tiles, [320, 8192] x [2048, 8192] 18.1 / 21.9 / 28.8; 48 tiles, [320, 8192] x [6144, 8192]
+    //                          28.1 / 33.1 / 30.7
+    //   the rows (256):        [128, 8192] x [8192, 8192] 22.1 / 21.6 / 29.9, but [192, 8192] x [8192, 8192] 28.5 / 23.0 / 29.8 and
+    //                          [256, 12288] x [6144, 12288] 38.7 / 29.2 / 39.8: at 129 to 256 rows of that length the rule is not
+    //                          the best choice.
     const int64_t small = ((out + 127) / 128) * ((rows + 63) / 64), large = ((out + 255) / 256) * ((rows + 255) / 256);
     if (rows > 256 && pitch >= 8192 && large * 4 <= sm_count() && large * 8 >= sm_count())
         return launch_few<T, 256, 2>(xq, xs, wq, ws, bias, y, rows, pitch, out, status, dependent, st);

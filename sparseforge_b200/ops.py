@@ -508,7 +508,8 @@ def grad_norm(grads, norm_type=2.0) -> torch.Tensor:
 
 
 def clip_grads(grads, norm, max_norm, out=None) -> None:
-    """``out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))`` with ``norm`` an fp32 scalar on the device (for
+    """``out[i] = grads[i] * min(1, max_norm / (norm + 1e-6))`` (the coefficient rounded to 24 bits, the product to fp32,
+    then to the output's type) with ``norm`` an fp32 scalar on the device (for
     example ``grad_norm``'s, or one combined over ranks). In place without ``out``; an output has its gradient's
     number of elements and may have the other of the two dtypes (bf16 gradients from fp32 accumulators)."""
     grads = list(grads)

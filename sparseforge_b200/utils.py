@@ -160,7 +160,9 @@ def grad_sync_context(model, is_last_micro: bool):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False, foreach=None):
     """Scales the gradients of ``parameters`` in place so that their common norm is at most ``max_norm`` and returns
     the norm they had; the training loop's call between ``backward`` and ``optimizer.step``
-    (legacy/main_llama.py:1997-2211), with the arguments of ``torch.nn.utils.clip_grad_norm_``.
+    (legacy/main_llama.py:1997-2211), with the arguments of ``torch.nn.utils.clip_grad_norm_``, for what that loop holds:
+    float32 and bfloat16 gradients on one device, without gaps in memory. Other types and norms, gradients on several
+    devices, and one gradient tensor under two parameters (which torch scales twice) are refused.
 
     Two launches for up to 448 gradients. The norm is one fp32 scalar on the device that was never rounded to the
     gradients' dtype; gradients that need no scaling are read once and not written. ``norm_type``: 2 or ``inf``.
