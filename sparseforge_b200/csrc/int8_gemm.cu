@@ -300,7 +300,7 @@ __device__ __forceinline__ float int8_out_usual(int acc, float xs, float ws, flo
     return __fmaf_rn(__fmul_rn(__int2float_rn(acc), xs), ws, bias);
 }
 __device__ __forceinline__ float int8_out(int acc, float xs, float ws, float bias) {
-    return xs >= kHugeScale ? int8_out_huge(acc, xs, ws, bias) : int8_out_usual(acc, xs, ws, bias);
+    return fabsf(xs) >= kHugeScale ? int8_out_huge(acc, xs, ws, bias) : int8_out_usual(acc, xs, ws, bias);
 }
 
 // ---------------------------------------------------------------------------------------------------------
@@ -555,7 +555,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                 }
             };
             // a loop of its own for huge rows: a test inside one loop took [8192, 64] x [12288, 64] from 89 to 99 us
-            if (__any_sync(0xffffffffu, rs >= kHugeScale)) put([](int a, float x, float w, float b) { return int8_out(a, x, w, b); });
+            if (__any_sync(0xffffffffu, fabsf(rs) >= kHugeScale)) put([](int a, float x, float w, float b) { return int8_out(a, x, w, b); });
             else put([](int a, float x, float w, float b) { return int8_out_usual(a, x, w, b); });
         }
     }
@@ -906,7 +906,7 @@ int8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__
         for (int c = threadIdx.x - 64; c < BN; c += 128) {
             const float scale = t0 + c < rows ? xs[t0 + c] : 0.0f;
             tail->xs[c] = scale;
-            if (scale >= kHugeScale) tail->any_huge = 1;
+            if (fabsf(scale) >= kHugeScale) tail->any_huge = 1;
         }
         const bool done = ptx::mbar_wait(ptx::smem_u32(&tail->tmem_full), 0, abort_flag, status, 54);
         if (done) {

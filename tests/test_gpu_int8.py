@@ -551,3 +551,18 @@ def test_values_of_a_forked_call(T, captured):
         torch.cuda.synchronize()
         for a, w in zip(got + got_beside, want + beside):
             assert torch.equal(a, w)
+
+
+@pytest.mark.parametrize("T,k,n", [(1, 256, 40), (5, 2048, 70), (60, 512, 130), (2048, 256, 1303)])
+def test_scales_of_either_sign(T, k, n):
+    """A caller's own scales may be negative: huge ones are no exception. Powers of two, so that only the sum is rounded."""
+    ops = _ops()
+    g = torch.Generator(device="cuda").manual_seed(3)
+    xq = torch.randint(-127, 128, (T, k), device="cuda", generator=g, dtype=torch.int8)
+    wq = torch.randint(-127, 128, (n, k), device="cuda", generator=g, dtype=torch.int8)
+    xs = torch.tensor([2.0 ** 110, -(2.0 ** 110), -1.0, -(2.0 ** 96), 2.0 ** 95], device="cuda")[torch.arange(T, device="cuda") % 5]
+    xs[0] = -(2.0 ** 110)
+    ws = torch.tensor([2.0 ** -80, -(2.0 ** -100)], device="cuda")[torch.arange(n, device="cuda") % 2]
+    want = (xq.double() @ wq.double().t()) * xs.double()[:, None] * ws.double()
+    y = ops.int8_gemm(xq, xs, wq, ws, out_dtype=torch.float32)
+    assert ((y.double() - want).abs() <= U * want.abs()).all()
