@@ -390,12 +390,6 @@ static int gn_grid(int64_t chunks, int blocks_per_sm) {
     return (int)std::max<int64_t>(1, std::min(chunks, cap));
 }
 
-static int64_t gn_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t from, int64_t to) {
-    int64_t bytes = 0;
-    for (int64_t i = from; i < to; ++i) bytes += sizes[i] * (dtypes[i] == SF_BF16 ? 2 : 4);
-    return bytes;
-}
-
 // Fills the table with tensors [from, to), the last keep_bytes of which are marked to stay in L2. Returns the number of chunks.
 template <int CAP>
 static int64_t gn_fill(GnTable<CAP>& tab, const void* const* grads, void* const* outs, const int64_t* sizes,
@@ -458,11 +452,21 @@ static cudaError_t gn_launch_dependent(void (*kern)(KArgs...), int grid, cudaStr
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
-// What the launch whose tensors end at `to` may leave in L2: the share of the whole list's last kGnKeepBytes that is not taken
-// by the launches behind it.
-static int64_t gn_keep_bytes(const int64_t* sizes, const int32_t* dtypes, int64_t to, int64_t count) {
-    return std::max<int64_t>(0, kGnKeepBytes - gn_bytes(sizes, dtypes, to, count));
-}
+// What each launch may leave in L2: the share of the whole list's last kGnKeepBytes that is not taken by the launches behind
+// it. Asked launch by launch, in order; one walk over the list in all.
+struct GnKeep {
+    const int64_t* sizes;
+    const int32_t* dtypes;
+    int64_t start, behind = 0;  // bytes from tensor `start` on (kGnKeepBytes or more, or all), then from the launch's end on
+    GnKeep(const int64_t* sizes_, const int32_t* dtypes_, int64_t count) : sizes(sizes_), dtypes(dtypes_), start(count) {
+        while (start > 0 && behind < kGnKeepBytes) behind += bytes(--start);
+    }
+    int64_t bytes(int64_t i) const { return sizes[i] * (dtypes[i] == SF_BF16 ? 2 : 4); }
+    int64_t of_launch(int64_t from, int64_t to) {
+        for (int64_t i = std::max(from, start); i < to; ++i) behind -= bytes(i);
+        return to <= start ? 0 : std::max<int64_t>(0, kGnKeepBytes - behind);
+    }
+};
 
 // Launches the partial sums of tensors [from, to); *slots grows by the number of slots written.
 template <int CAP>
@@ -482,8 +486,9 @@ static int gn_partials_part(const void* const* grads, const int64_t* sizes, cons
 static int gn_partials(const void* const* grads, const int64_t* sizes, const int32_t* dtypes, int64_t count, int kind,
                        double* scratch, int* slots, cudaStream_t st) {
     *slots = 0;
+    GnKeep keeping(sizes, dtypes, count);
     for (int64_t from = 0; from < count; from += kGnCap) {
-        const int64_t to = std::min(count, from + kGnCap), keep = gn_keep_bytes(sizes, dtypes, to, count);
+        const int64_t to = std::min(count, from + kGnCap), keep = keeping.of_launch(from, to);
         const int rc = to - from <= kGnCapSmall
                            ? gn_partials_part<kGnCapSmall>(grads, sizes, dtypes, from, to, keep, kind, scratch, slots, st)
                            : gn_partials_part<kGnCap>(grads, sizes, dtypes, from, to, keep, kind, scratch, slots, st);
@@ -539,10 +544,13 @@ int64_t sf_selftest_grad_norm_kept_bytes(const int64_t* sizes, const int32_t* dt
     for (int64_t i = 0; i < count; ++i)
         if (sizes[i] < 0 || sizes[i] > ((int64_t)1 << 42) || (dtypes[i] != SF_F32 && dtypes[i] != SF_BF16)) return -1;
     const int64_t from = launch * kGnCap, to = std::min(count, from + kGnCap);
+    GnKeep keeping(sizes, dtypes, count);
+    int64_t keep = 0;
+    for (int64_t part = 0; part <= launch; ++part) keep = keeping.of_launch(part * kGnCap, std::min(count, (part + 1) * kGnCap));
     const std::unique_ptr<const void*[]> nowhere(new (std::nothrow) const void*[count ? count : 1]());
     const std::unique_ptr<GnTable<kGnCap>> tab(new (std::nothrow) GnTable<kGnCap>);
     if (!tab || !nowhere) return -1;
-    gn_fill(*tab, nowhere.get(), nullptr, sizes, dtypes, nullptr, from, to, gn_keep_bytes(sizes, dtypes, to, count));
+    gn_fill(*tab, nowhere.get(), nullptr, sizes, dtypes, nullptr, from, to, keep);
     int64_t kept = 0;
     for (int k = 0; k < tab->count; ++k) {
         const int64_t before = tab->keep_from > tab->first[k] ? (int64_t)(tab->keep_from - tab->first[k]) * tab->chunk : 0;
